@@ -89,7 +89,9 @@ typedef enum {
   GB_FMT_DENSE = 3
 } gb_weight_format;
 
-typedef enum { GB_DTYPE_F32 = 0, GB_DTYPE_BF16 = 1 } gb_dtype;
+/* GB_DTYPE_F16: the paged-cache operators and gb_sample only; MoE weights,
+ * routers and biases are F32 or BF16. */
+typedef enum { GB_DTYPE_F32 = 0, GB_DTYPE_BF16 = 1, GB_DTYPE_F16 = 2 } gb_dtype;
 
 /* Everything gb_moe_create needs.  Zero-initialise, set struct_size =
  * sizeof(gb_moe_desc), then fill in.  Host pointers; the library copies what
@@ -439,6 +441,178 @@ int gb_decoder_stage_times(gb_decoder* d, float ms_out[3], void* stream);
 int gb_decoder_device_status(gb_decoder* d, void* stream);
 
 int gb_decoder_destroy(gb_decoder* d);
+
+/* ---- Paged KV cache ------------------------------------------------------
+ * Operators of a serving loop whose sequences keep their keys and values in
+ * pages of one pool per layer: a batch is ragged (each sequence brings its
+ * own number of new tokens and its own cached length), where the decode stack
+ * above runs sequences in lockstep on a contiguous cache.  They stand alone
+ * like gb_route_noalloc: every buffer is the caller's, on the current device;
+ * nothing is allocated and the calls are asynchronous on `stream` and may be
+ * captured into a CUDA graph.  A first call of each kind on a device sets
+ * kernel attributes, so make it before a capture.
+ *
+ * A pool holds n_pages pages of page_size slots of n_kv_heads heads of
+ * head_dim elements; element (page, slot, head, d) lies at
+ *   page * page_stride + slot * slot_stride + head * head_stride + d,
+ * strides in elements, so both [page][slot][head][dim] and
+ * [page][head][slot][dim] are one call.  K and V pools have the same shape
+ * and strides.  Sequence b owns rows q_start[b] .. q_start[b + 1] - 1 of the
+ * call's rows and the cached positions 0 .. kv_len[b] - 1, its new tokens
+ * included: its row i sits at position kv_len[b] - q_len[b] + i.  Position p
+ * lives in slot p % page_size of page page_table[b][p / page_size].  Rows at
+ * or past q_start[n_seqs] belong to no sequence and are left as they are. */
+typedef struct gb_paged_batch {
+  uint32_t struct_size;          /* sizeof(gb_paged_batch) */
+  int32_t dtype;                 /* the pools': GB_DTYPE_BF16 or GB_DTYPE_F16 */
+  int32_t n_kv_heads;
+  int32_t head_dim;              /* 64, 128 or 256 */
+  int32_t page_size;             /* a power of two, 8 .. 1024 */
+  int32_t n_pages;
+  int64_t page_stride;           /* elements, multiples of 8 */
+  int64_t slot_stride;
+  int64_t head_stride;
+  int32_t n_seqs;
+  int32_t total_q;               /* rows of q and out (at least q_start[n_seqs]) */
+  int32_t max_q_len;             /* at least the longest q_len of the batch */
+  int32_t max_kv_len;            /* at least the longest kv_len of the batch */
+  const int32_t* q_start_dev;    /* [n_seqs + 1], ascending from 0 */
+  const int32_t* kv_len_dev;     /* [n_seqs] */
+  const int32_t* page_table_dev; /* [n_seqs][table_stride] page numbers */
+  int64_t table_stride;          /* entries per sequence */
+  int32_t* error_dev;            /* one word, nullable: gb_paged_error bits are ORed into it */
+} gb_paged_batch;
+
+/* What a kernel found wrong with a batch's device arrays.  It reads and
+ * writes nothing out of range for it: see each bit. */
+typedef enum {
+  GB_PAGED_BAD_PAGE = 1,     /* a needed page number outside [0, n_pages): its keys count as
+                                masked, its stores are dropped */
+  GB_PAGED_BAD_LENGTH = 2,   /* q_start not ascending within [0, total_q], a q_len or kv_len
+                                outside [0, max] or past the page table: clamped to it */
+  GB_PAGED_BAD_POSITION = 4, /* a row before position 0 or past the cos / sin tables: the row
+                                is dropped */
+  GB_PAGED_TIMEOUT = 8       /* a bounded pipeline wait ran out: the output is invalid */
+} gb_paged_error;
+
+/* RMS norm of each query and key head, position rotation, and the keys and
+ * values of the batch's rows stored into their pages, in one pass
+ * (rms norm x / sqrt(mean(x^2) + eps) * w over the head, then the halves
+ * layout of pos_enc.rs:199-217 on the first rot_dim elements: x1' = x1 cos -
+ * x2 sin, x2' = x1 sin + x2 cos, x2 = rot_dim / 2 elements after x1).
+ * Arithmetic in f32, one rounding to the pool's type at the end. */
+typedef struct gb_rope_args {
+  uint32_t struct_size;          /* sizeof(gb_rope_args) */
+  int32_t in_dtype;              /* q, k, v: gb_dtype */
+  int32_t n_heads;               /* query heads */
+  int32_t rot_dim;               /* rotated elements of a head: 0 (none) or a multiple of 16 up
+                                    to head_dim */
+  const void* q_dev;             /* [total_q][n_heads][head_dim], strides below; with n_heads 0
+                                    no queries are read or written */
+  const void* k_dev;             /* [total_q][n_kv_heads][head_dim] */
+  const void* v_dev;
+  int64_t q_row_stride;          /* elements; every row and head starts on 16 bytes */
+  int64_t q_head_stride;
+  int64_t k_row_stride;
+  int64_t k_head_stride;
+  int64_t v_row_stride;
+  int64_t v_head_stride;
+  void* q_out_dev;               /* the pool's type; may be q_dev itself when the types agree */
+  int64_t out_row_stride;
+  int64_t out_head_stride;
+  const float* q_norm_dev;       /* [head_dim] norm weights, NULL: no norm */
+  const float* k_norm_dev;
+  const float* cos_dev;          /* [table_rows][rot_dim / 2], row = position */
+  const float* sin_dev;
+  int64_t table_rows;
+  void* k_pool_dev;
+  void* v_pool_dev;
+  float eps;
+} gb_rope_args;
+int gb_paged_rope_append(const gb_paged_batch* batch, const gb_rope_args* args, void* stream);
+
+/* Causal attention of the batch's rows over their sequences' pages
+ * (gpt_oss_q.rs:57-107 without its projections): a row at position p sees
+ * positions max(0, p - window + 1) .. p (window 0: from 0), scores are
+ * (q . k) * scale, and a head's sink logit, when given, joins the softmax's
+ * denominator.  Query head h reads KV head h / (n_heads / n_kv_heads).  A row
+ * that sees nothing gives zeros.  Positions that no row of a sequence sees
+ * are not read: their pages may be gone (any page number, -1 say).  What a
+ * row does not see has no part in its result, whatever its bits.  Scores,
+ * softmax statistics and sums are f32; each probability is rounded to the
+ * pool's type before it multiplies V.
+ * workspace_dev: gb_paged_attention_workspace bytes, 256-byte aligned, its
+ * contents meaningless between calls; calls (or graph replays) that overlap
+ * on the GPU need one each. */
+typedef struct gb_attn_args {
+  uint32_t struct_size;          /* sizeof(gb_attn_args) */
+  int32_t n_heads;               /* a multiple of n_kv_heads, at most 16 per KV head */
+  int32_t window;                /* keys a row sees, its own included; 0 = all */
+  int32_t out_dtype;             /* the pool's type, or GB_DTYPE_F32 */
+  float scale;
+  const void* q_dev;             /* [total_q][n_heads][head_dim] in the pool's type */
+  int64_t q_row_stride;          /* elements; every row and head starts on 16 bytes */
+  int64_t q_head_stride;
+  const void* k_pool_dev;
+  const void* v_pool_dev;
+  const float* sinks_dev;        /* [n_heads], NULL: none */
+  void* out_dev;                 /* [total_q][n_heads][head_dim]; not q_dev */
+  int64_t out_row_stride;
+  int64_t out_head_stride;
+  void* workspace_dev;
+  int64_t workspace_bytes;
+} gb_attn_args;
+int gb_paged_attention(const gb_paged_batch* batch, const gb_attn_args* args, void* stream);
+
+/* Workspace bytes of gb_paged_attention for this batch's sizes (the device
+ * arrays are not read), the same on every device of this library. */
+int gb_paged_attention_workspace(const gb_paged_batch* batch, int32_t n_heads, int64_t* bytes);
+
+/* Copies page src[i] to page dst[i], i < n, in each of n_pools pools of
+ * n_pages pages of page_bytes bytes, page_stride bytes apart (multiples of
+ * 16; pools start on 16 bytes): the K and V pools of every layer in one call,
+ * for a fork's last page or a compaction.  src and dst are host arrays, read
+ * during the call (a captured call keeps the lists it was given).  A page
+ * may be copied to several others; GB_ERR_INVALID_ARG if a page is out of
+ * range, is written twice, or is both read and written. */
+int gb_paged_copy(void* const* pools_dev, int32_t n_pools, int64_t n_pages, int64_t page_bytes,
+                  int64_t page_stride, const int32_t* src, const int32_t* dst, int32_t n,
+                  void* stream);
+
+/* ---- Sampling --------------------------------------------------------------
+ * One token per row of logits, drawn with a uniform number that the caller
+ * gives (sampling.rs:7-173 draws from its own generator): beside the greedy
+ * token of the decode stack.  Per row, with x the logits:
+ *   - the tokens in order of falling logit, equal ones by rising id; NaN counts
+ *     as -inf;
+ *   - weights w = e^((x - max) / temperature); a temperature <= 0 keeps the
+ *     first token alone;
+ *   - top_k > 0 keeps the first top_k tokens; top_p < 1 then keeps a token
+ *     while the weight before it is below top_p of those tokens' weight;
+ *     min_p keeps those with w >= min_p; the first token always stays;
+ *   - the token is the first in order of id whose kept weights, summed over
+ *     the ids up to it, exceed u times all of them (u is clamped to [0, 1)).
+ * Weights are computed in 64 bits and summed as integers of 2^-45 of the
+ * largest, so the choice does not depend on the order of the sums; a token
+ * below 2^-46 of the largest is never drawn.  A row with no finite logit and
+ * no +inf gives token -1 and log-probability -inf; +inf logits share the
+ * weight equally. */
+typedef struct gb_sample_args {
+  uint32_t struct_size;          /* sizeof(gb_sample_args) */
+  int32_t dtype;                 /* logits: gb_dtype */
+  int32_t rows;
+  int32_t vocab;                 /* at most 400000 */
+  const void* logits_dev;        /* [rows][vocab], row_stride elements apart */
+  int64_t row_stride;
+  const float* u_dev;            /* [rows] */
+  const float* temperature_dev;  /* [rows], NULL: 1 */
+  const int32_t* top_k_dev;      /* [rows], <= 0 keeps all; NULL: all */
+  const float* top_p_dev;        /* [rows], >= 1 keeps all; NULL: all */
+  const float* min_p_dev;        /* [rows], <= 0 keeps all; NULL: all */
+  int32_t* token_dev;            /* [rows] */
+  float* logprob_dev;            /* [rows], nullable: log of the token's share of the kept weight */
+} gb_sample_args;
+int gb_sample(const gb_sample_args* args, void* stream);
 
 /* Expert parallel: a fresh 128-byte ncclUniqueId (rank 0 calls this and
  * shares the bytes with the other ranks). */

@@ -36,6 +36,7 @@ pub const GB_FMT_DENSE: i32 = 3;
 // gb_dtype
 pub const GB_DTYPE_F32: i32 = 0;
 pub const GB_DTYPE_BF16: i32 = 1;
+pub const GB_DTYPE_F16: i32 = 2;
 
 // gb_expert_path
 pub const GB_PATH_AUTO: i32 = 0;
@@ -186,6 +187,103 @@ pub struct gb_decoder {
     _private: [u8; 0],
 }
 
+// gb_paged_error
+pub const GB_PAGED_BAD_PAGE: i32 = 1;
+pub const GB_PAGED_BAD_LENGTH: i32 = 2;
+pub const GB_PAGED_BAD_POSITION: i32 = 4;
+pub const GB_PAGED_TIMEOUT: i32 = 8;
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct gb_paged_batch {
+    pub struct_size: u32,
+    pub dtype: i32,
+    pub n_kv_heads: i32,
+    pub head_dim: i32,
+    pub page_size: i32,
+    pub n_pages: i32,
+    pub page_stride: i64,
+    pub slot_stride: i64,
+    pub head_stride: i64,
+    pub n_seqs: i32,
+    pub total_q: i32,
+    pub max_q_len: i32,
+    pub max_kv_len: i32,
+    pub q_start_dev: *const i32,
+    pub kv_len_dev: *const i32,
+    pub page_table_dev: *const i32,
+    pub table_stride: i64,
+    pub error_dev: *mut i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct gb_rope_args {
+    pub struct_size: u32,
+    pub in_dtype: i32,
+    pub n_heads: i32,
+    pub rot_dim: i32,
+    pub q_dev: *const c_void,
+    pub k_dev: *const c_void,
+    pub v_dev: *const c_void,
+    pub q_row_stride: i64,
+    pub q_head_stride: i64,
+    pub k_row_stride: i64,
+    pub k_head_stride: i64,
+    pub v_row_stride: i64,
+    pub v_head_stride: i64,
+    pub q_out_dev: *mut c_void,
+    pub out_row_stride: i64,
+    pub out_head_stride: i64,
+    pub q_norm_dev: *const f32,
+    pub k_norm_dev: *const f32,
+    pub cos_dev: *const f32,
+    pub sin_dev: *const f32,
+    pub table_rows: i64,
+    pub k_pool_dev: *mut c_void,
+    pub v_pool_dev: *mut c_void,
+    pub eps: f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct gb_attn_args {
+    pub struct_size: u32,
+    pub n_heads: i32,
+    pub window: i32,
+    pub out_dtype: i32,
+    pub scale: f32,
+    pub q_dev: *const c_void,
+    pub q_row_stride: i64,
+    pub q_head_stride: i64,
+    pub k_pool_dev: *const c_void,
+    pub v_pool_dev: *const c_void,
+    pub sinks_dev: *const f32,
+    pub out_dev: *mut c_void,
+    pub out_row_stride: i64,
+    pub out_head_stride: i64,
+    pub workspace_dev: *mut c_void,
+    pub workspace_bytes: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct gb_sample_args {
+    pub struct_size: u32,
+    pub dtype: i32,
+    pub rows: i32,
+    pub vocab: i32,
+    pub logits_dev: *const c_void,
+    pub row_stride: i64,
+    pub u_dev: *const f32,
+    pub temperature_dev: *const f32,
+    pub top_k_dev: *const i32,
+    pub top_p_dev: *const f32,
+    pub min_p_dev: *const f32,
+    pub token_dev: *mut i32,
+    pub logprob_dev: *mut f32,
+}
+
 extern "C" {
     pub fn gb_moe_create(desc: *const gb_moe_desc, out: *mut *mut gb_moe) -> c_int;
     pub fn gb_moe_forward(m: *mut gb_moe, x_dev: *const f32, t: i64, out_dev: *mut f32,
@@ -224,6 +322,16 @@ extern "C" {
         -> c_int;
     pub fn gb_decoder_device_status(d: *mut gb_decoder, stream: *mut c_void) -> c_int;
     pub fn gb_decoder_destroy(d: *mut gb_decoder) -> c_int;
+    pub fn gb_paged_rope_append(batch: *const gb_paged_batch, args: *const gb_rope_args,
+                                stream: *mut c_void) -> c_int;
+    pub fn gb_paged_attention(batch: *const gb_paged_batch, args: *const gb_attn_args,
+                              stream: *mut c_void) -> c_int;
+    pub fn gb_paged_attention_workspace(batch: *const gb_paged_batch, n_heads: i32,
+                                        bytes: *mut i64) -> c_int;
+    pub fn gb_paged_copy(pools_dev: *const *mut c_void, n_pools: i32, n_pages: i64,
+                         page_bytes: i64, page_stride: i64, src: *const i32, dst: *const i32,
+                         n: i32, stream: *mut c_void) -> c_int;
+    pub fn gb_sample(args: *const gb_sample_args, stream: *mut c_void) -> c_int;
     pub fn gb_nccl_unique_id(out: *mut u8) -> c_int;
     pub fn gb_last_error() -> *const c_char;
     pub fn gb_abi_version() -> c_int;

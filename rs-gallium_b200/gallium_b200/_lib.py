@@ -45,6 +45,7 @@ GB_PATH_TENSOR_CORES_F16 = 3
 GB_PATH_FUSED_DECODE = 4
 GB_DTYPE_F32 = 0
 GB_DTYPE_BF16 = 1
+GB_DTYPE_F16 = 2
 
 
 class GalliumError(RuntimeError):
@@ -164,6 +165,97 @@ class DecoderDesc(ctypes.Structure):
     ]
 
 
+class PagedBatchDesc(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("dtype", c_int32),
+        ("n_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("page_size", c_int32),
+        ("n_pages", c_int32),
+        ("page_stride", c_int64),
+        ("slot_stride", c_int64),
+        ("head_stride", c_int64),
+        ("n_seqs", c_int32),
+        ("total_q", c_int32),
+        ("max_q_len", c_int32),
+        ("max_kv_len", c_int32),
+        ("q_start_dev", c_void_p),
+        ("kv_len_dev", c_void_p),
+        ("page_table_dev", c_void_p),
+        ("table_stride", c_int64),
+        ("error_dev", c_void_p),
+    ]
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("in_dtype", c_int32),
+        ("n_heads", c_int32),
+        ("rot_dim", c_int32),
+        ("q_dev", c_void_p),
+        ("k_dev", c_void_p),
+        ("v_dev", c_void_p),
+        ("q_row_stride", c_int64),
+        ("q_head_stride", c_int64),
+        ("k_row_stride", c_int64),
+        ("k_head_stride", c_int64),
+        ("v_row_stride", c_int64),
+        ("v_head_stride", c_int64),
+        ("q_out_dev", c_void_p),
+        ("out_row_stride", c_int64),
+        ("out_head_stride", c_int64),
+        ("q_norm_dev", c_void_p),
+        ("k_norm_dev", c_void_p),
+        ("cos_dev", c_void_p),
+        ("sin_dev", c_void_p),
+        ("table_rows", c_int64),
+        ("k_pool_dev", c_void_p),
+        ("v_pool_dev", c_void_p),
+        ("eps", c_float),
+    ]
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("n_heads", c_int32),
+        ("window", c_int32),
+        ("out_dtype", c_int32),
+        ("scale", c_float),
+        ("q_dev", c_void_p),
+        ("q_row_stride", c_int64),
+        ("q_head_stride", c_int64),
+        ("k_pool_dev", c_void_p),
+        ("v_pool_dev", c_void_p),
+        ("sinks_dev", c_void_p),
+        ("out_dev", c_void_p),
+        ("out_row_stride", c_int64),
+        ("out_head_stride", c_int64),
+        ("workspace_dev", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("dtype", c_int32),
+        ("rows", c_int32),
+        ("vocab", c_int32),
+        ("logits_dev", c_void_p),
+        ("row_stride", c_int64),
+        ("u_dev", c_void_p),
+        ("temperature_dev", c_void_p),
+        ("top_k_dev", c_void_p),
+        ("top_p_dev", c_void_p),
+        ("min_p_dev", c_void_p),
+        ("token_dev", c_void_p),
+        ("logprob_dev", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES = {
     "gb_moe_create": (c_int, [POINTER(MoeDesc), POINTER(c_void_p)]),
@@ -193,6 +285,12 @@ SIGNATURES = {
     "gb_decoder_stage_times": (c_int, [c_void_p, POINTER(c_float), c_void_p]),
     "gb_decoder_device_status": (c_int, [c_void_p, c_void_p]),
     "gb_decoder_destroy": (c_int, [c_void_p]),
+    "gb_paged_rope_append": (c_int, [POINTER(PagedBatchDesc), POINTER(RopeArgs), c_void_p]),
+    "gb_paged_attention": (c_int, [POINTER(PagedBatchDesc), POINTER(AttnArgs), c_void_p]),
+    "gb_paged_attention_workspace": (c_int, [POINTER(PagedBatchDesc), c_int32, POINTER(c_int64)]),
+    "gb_paged_copy": (c_int, [POINTER(c_void_p), c_int32, c_int64, c_int64, c_int64,
+                              POINTER(c_int32), POINTER(c_int32), c_int32, c_void_p]),
+    "gb_sample": (c_int, [POINTER(SampleArgs), c_void_p]),
     "gb_nccl_unique_id": (c_int, [POINTER(c_uint8)]),
     "gb_last_error": (c_char_p, []),
     "gb_abi_version": (c_int, []),
