@@ -53,6 +53,7 @@ template <typename T>
 struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
+  static constexpr int kType = GB_DTYPE_BF16;
   // log2 of the weight that a softmax gives its maximum: f16 weights of 2^8 keep
   // those down to 2^-22 of the maximum normal; bf16 has f32's range.
   static constexpr float kTop = 0.0f;
@@ -67,6 +68,7 @@ struct Elem<__nv_bfloat16> {
 };
 template <>
 struct Elem<__half> {
+  static constexpr int kType = GB_DTYPE_F16;
   static constexpr float kTop = 8.0f;
   static constexpr uint32_t kExpMask = 0x7c00u;
   __device__ static __forceinline__ uint32_t pack(float lo, float hi) {

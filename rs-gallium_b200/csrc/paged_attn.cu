@@ -1,209 +1,13 @@
 // paged_attn.cu -- causal attention of a ragged batch's new rows over their
-// sequences' pages (gb_paged_attention).
-//
-//   o = sum_j e^(s_j - m) v_j / (e^(sink - m) + sum_j e^(s_j - m)),  s_j = scale (q . k_j)
-//
-// in one pass over K and V with a running maximum and sum.
-//
-// Work.  The query heads that share a KV head are rows of one tile, so each
-// key is read once for all of them: kRows rows = (kRows / group) tokens x
-// group heads.  A tile's keys are split over several CTAs when the batch has
-// too few tiles to fill the GPU, each split writes its unnormalised sum with
-// its maximum and its sum of weights, and a second kernel joins them in the
-// order of the splits.  The lengths are on the device, so every CTA works out
-// its own item from them (a scan over the sequences), and the grid is sized
-// from the host's bounds.
-#include <algorithm>
-
-#include "paged.cuh"
-#include "ptx.cuh"
+// sequences' pages (gb_paged_attention): the kernel of decoding sequences, the
+// joining kernel, and the entry points.
+#include "paged_attn.cuh"
 
 namespace gb {
 namespace paged {
 namespace {
 
-// 2^x by the hardware's approximation (relative error 2^-22); 2^-inf = 0.
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kTargetItems = 296;              // two CTAs on each of 148 SMs
-constexpr int kMaxSlots = 2 * kTargetItems;    // items of split tiles, at most (see Plan)
-constexpr int kUnit = 64;                      // keys per unit of work
-constexpr int kMinUnits = 2;                   // units per split, at least
-constexpr int kRows = 16;                      // rows of a tile
 constexpr int kThreads = 128;
-constexpr int kMaxGroup = 16;                  // query heads per KV head
-
-struct Group {  // a split tile, for the joining kernel
-  int row0, tokens, g, slot0, splits;
-};
-
-struct AttnArgs {
-  Batch b;
-  int nh, group, window, out_f32;
-  float scale;  // scale * log2 e
-  const void* q;
-  int64_t q_row, q_head;
-  const void *k_pool, *v_pool;
-  const float* sinks;
-  void* out;
-  int64_t o_row, o_head;
-  // workspace
-  int* n_groups;
-  Group* groups;       // [kTargetItems]
-  float2* part_ml;     // [kMaxSlots][kRows]: maximum (log2), sum
-  float* part_o;       // [kMaxSlots][kRows][head_dim]
-};
-
-size_t workspace_layout(int head_dim, char* base, AttnArgs* a) {
-  size_t at = 0;
-  auto take = [&](size_t bytes) {
-    char* p = base ? base + at : nullptr;
-    at += (bytes + 255) & ~(size_t)255;
-    return p;
-  };
-  char* n = take(sizeof(int));
-  char* g = take(sizeof(Group) * kTargetItems);
-  char* ml = take(sizeof(float2) * kMaxSlots * kRows);
-  char* o = take(sizeof(float) * (size_t)kMaxSlots * kRows * head_dim);
-  if (a) {
-    a->n_groups = reinterpret_cast<int*>(n);
-    a->groups = reinterpret_cast<Group*>(g);
-    a->part_ml = reinterpret_cast<float2*>(ml);
-    a->part_o = reinterpret_cast<float*>(o);
-  }
-  return at;
-}
-
-// What a CTA does: rows of `tokens` tokens from row `row0`, the first at
-// position pos0, KV head g, units [u0, u1) of kUnit keys.
-struct Item {
-  int seq, row0, tokens, pos0, g, u0, u1;
-  int slot;  // of the partial result, -1: the tile is not split
-};
-
-// Splitting.  n = the units a sequence's rows see, t = ceil(W / kTargetItems)
-// units per split (W: the units of all tiles), so a sequence has ceil(n / t)
-// splits.  Tiles with more than one split have n > t, hence at most W / t such
-// tiles and at most 2 W / t <= kMaxSlots of their splits.
-struct SeqWork {
-  int tiles, units;
-};
-__device__ __forceinline__ int first_unit(int pos, int window) {
-  return window > 0 && pos >= window ? (pos - window + 1) / kUnit : 0;
-}
-__device__ __forceinline__ SeqWork seq_work(const Seq& q, int tpt, int window) {
-  SeqWork w{0, 0};
-  w.tiles = (q.q_len + tpt - 1) / tpt;
-  const int last = q.kv_len - 1;
-  if (w.tiles && last >= 0)
-    w.units = last / kUnit - first_unit(max(q.kv_len - q.q_len, 0), window) + 1;
-  return w;
-}
-
-template <typename V>
-__device__ __forceinline__ V warp_inclusive(V v) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const V t = __shfl_up_sync(kFullMask, v, o);
-    if ((threadIdx.x & 31) >= o) v += t;
-  }
-  return v;
-}
-
-// Finds the CTA's item; false: there is none.  Called by the whole CTA.
-__device__ bool find_item(const AttnArgs& a, int tpt, Item* out) {
-  __shared__ unsigned long long red[kThreads / 32];
-  __shared__ unsigned long long run[kThreads / 32][2];
-  __shared__ Item found;
-  __shared__ int have;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Batch& b = a.b;
-  Seq mine{0, 0, 0};  // of the first kThreads sequences
-  unsigned long long w = 0;
-  for (int s = tid; s < b.n_seqs; s += kThreads) {
-    const Seq q = load_seq(b, s, blockIdx.x == 0);
-    if (s == tid) mine = q;
-    const SeqWork x = seq_work(q, tpt, a.window);
-    w += (unsigned long long)x.tiles * x.units;
-  }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) w += __shfl_xor_sync(kFullMask, w, o);
-  if (lane == 0) red[warp] = w;
-  if (tid == 0) have = 0;
-  __syncthreads();
-  w = 0;
-#pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) w += red[i];
-  w *= b.nkv;
-  const unsigned long long t64 = (w + kTargetItems - 1) / kTargetItems;
-  const int t = (int)(t64 < kMinUnits ? kMinUnits : t64 > (1u << 30) ? (1u << 30) : t64);
-  // prefixes over the sequences: items (low half) and split items; split tiles
-  unsigned long long base_items = 0, base_groups = 0;
-  for (int s0 = 0; s0 < b.n_seqs; s0 += kThreads) {
-    const int s = s0 + tid;
-    Seq q{0, 0, 0};
-    if (s < b.n_seqs) q = s0 ? load_seq(b, s, false) : mine;
-    const SeqWork x = seq_work(q, tpt, a.window);
-    const int splits = max(1, (x.units + t - 1) / t);
-    const unsigned long long tiles = (unsigned long long)x.tiles * b.nkv;
-    const unsigned long long items = tiles * splits;
-    const unsigned long long groups = splits > 1 ? (items << 32) | tiles : 0;
-    const unsigned long long ii = warp_inclusive(items), gg = warp_inclusive(groups);
-    __syncthreads();
-    if (lane == 31) {
-      run[warp][0] = ii;
-      run[warp][1] = gg;
-    }
-    __syncthreads();
-    unsigned long long bi = base_items, bg = base_groups;
-    for (int i = 0; i < kThreads / 32; ++i) {
-      if (i < warp) {
-        bi += run[i][0];
-        bg += run[i][1];
-      }
-      base_items += run[i][0];
-      base_groups += run[i][1];
-    }
-    const unsigned long long before = bi + ii - items;
-    if (blockIdx.x >= before && blockIdx.x < before + items) {
-      const unsigned long long j = blockIdx.x - before;
-      const unsigned long long gb = bg + gg - groups;
-      Item it;
-      it.seq = s;
-      it.g = (int)(j % b.nkv);
-      const unsigned long long js = j / b.nkv;
-      const int split = (int)(js % splits), tile = (int)(js / splits);
-      it.row0 = q.row0 + tile * tpt;
-      it.tokens = min(tpt, q.q_len - tile * tpt);
-      it.pos0 = q.kv_len - q.q_len + tile * tpt;
-      const int last = it.pos0 + it.tokens - 1;
-      const int lo = first_unit(it.pos0, a.window);
-      const int n = last < 0 ? 0 : last / kUnit - lo + 1;
-      const int per = (n + splits - 1) / splits;
-      it.u0 = lo + min(split * per, n);
-      it.u1 = lo + min((split + 1) * per, n);
-      it.slot = -1;
-      if (splits > 1) {
-        const int group = (int)(uint32_t)gb + tile * b.nkv + it.g;
-        const int slot0 = (int)(gb >> 32) + (tile * b.nkv + it.g) * splits;
-        it.slot = slot0 + split;
-        if (split == 0) a.groups[group] = Group{it.row0, it.tokens, it.g, slot0, splits};
-      }
-      found = it;
-      have = 1;
-    }
-  }
-  if (blockIdx.x == 0 && tid == 0) *a.n_groups = (int)(uint32_t)base_groups;
-  __syncthreads();
-  if (!have) return false;
-  *out = found;
-  return true;
-}
 
 // ---- mma.sync building blocks (16 rows) --------------------------------------
 template <typename T>
@@ -248,12 +52,6 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ bool any_nonfinite(uint32_t w) {
-  constexpr uint32_t m = Elem<T>::kExpMask;
-  return (w & m) == m || (w & (m << 16)) == (m << 16);
-}
-
 // Keys per warp and step; a CTA's four warps take a unit of 64.
 constexpr int kStep = 16;
 
@@ -265,16 +63,6 @@ template <int HD>
 constexpr int q_bytes() { return kRows * HD * 2; }
 template <int HD>
 constexpr int smem_bytes() { return 4 * warp_bytes<HD>() + q_bytes<HD>(); }
-
-template <typename T>
-__device__ __forceinline__ void store_out(const AttnArgs& a, int row, int head, int d, float x,
-                                          float y) {
-  const int64_t at = row * a.o_row + head * a.o_head + d;
-  if (a.out_f32)
-    *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(x, y);
-  else
-    *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at) = Elem<T>::pack(x, y);
-}
 
 // A CTA per item: four warps, each with keys of its own (16 of every unit) and
 // its own pipeline of cp.async stages, so no barrier stands in the loop; their
@@ -288,7 +76,8 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tpt = kRows / a.group;
   Item it;
-  const bool have = find_item(a, tpt, &it);
+  constexpr Plan kPlan = kRowsPlan;
+  const bool have = find_item<true, kThreads>(a, kPlan, a.rows, tpt, &it);
   pdl_trigger();
   if (!have) return;
   const int n_rows = it.tokens * a.group;
@@ -339,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
   const int page_mask = (1 << a.b.page_shift) - 1;
   // the element offset of key lane & 15 of step u; -1: not to be read, -2: its page is bad
   auto key_offset = [&](int u) -> int64_t {
-    const int key = (it.u0 + u) * kUnit + warp * kStep + (lane & 15);
+    const int key = (it.u0 + u) * kPlan.unit + warp * kStep + (lane & 15);
     if (u >= n || key < key_lo || key > last) return -1;
     const int page = __ldg(table + (key >> a.b.page_shift));
     if ((unsigned)page >= (unsigned)a.b.n_pages) {
@@ -378,7 +167,7 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
     cp_wait<kStages - 1>();
     __syncwarp();
     const uint32_t ks_ = wbase + (u % kStages) * kStageBytes, vs_ = ks_ + kStep * HD * 2;
-    const int key0 = (it.u0 + u) * kUnit + warp * kStep;
+    const int key0 = (it.u0 + u) * kPlan.unit + warp * kStep;
     if (key0 <= last && key0 + kStep > key_lo) {  // the same on the whole warp
       float s[2][4];
 #pragma unroll
@@ -541,9 +330,9 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
       y += o.y * f;
     }
     if (it.slot >= 0) {
-      *reinterpret_cast<float2*>(a.part_o + ((int64_t)it.slot * kRows + r) * HD + d) =
+      *reinterpret_cast<float2*>(a.rows.o + ((int64_t)it.slot * kRows + r) * HD + d) =
           make_float2(x, y);
-      if (d == 0) a.part_ml[it.slot * kRows + r] = make_float2(M, L);
+      if (d == 0) a.rows.ml[it.slot * kRows + r] = make_float2(M, L);
     } else {
       const float inv = L == 0.0f ? 0.0f : 1.0f / L;
       store_out<T>(a, it.row0 + tok, h, d, x * inv, y * inv);
@@ -551,18 +340,30 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
   }
 }
 
-// Joins a split tile: a warp per row, its splits in order.
+// Joins the split tiles: a warp per row, its splits in order.  CTAs 0 ..
+// kRowsPlan.target - 1 take the 16-row tiles, the others 16 rows each of the
+// larger ones.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kRows * 32) attn_join_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kRows * 32)
+    attn_join_kernel(const __grid_constant__ AttnArgs a, int small_ctas) {
   pdl_wait();
-  if ((int)blockIdx.x >= __ldcg(a.n_groups)) return;
-  const Group g = a.groups[blockIdx.x];
-  const int r = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (r >= g.tokens * a.group) return;
+  constexpr int kTileRows = tile_plan<HD>().tile_rows, kParts = kTileRows / kRows;
+  const bool small = (int)blockIdx.x < small_ctas;
+  const Partials& part = small ? a.rows : a.tiles;
+  const int cta = small ? blockIdx.x : blockIdx.x - small_ctas;
+  const int group = small ? cta : cta / kParts, rows = small ? kRows : kTileRows;
+  if (group >= __ldcg(part.n_groups)) return;
+  const Group g = part.groups[group];
+  const int r = (small ? 0 : cta % kParts * kRows) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= g.rows) return;
   const int tok = r / a.group, h = g.g * a.group + r - tok * a.group;
+  // A large tile's rows are in sub-tiles of 128, each of whole tokens.
+  const int per = small ? kRows : 128 / a.group * a.group;
+  const int at_row = r / per * 128 + r % per;
   const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
   float M = sink;
-  for (int s = lane; s < g.splits; s += 32) M = fmaxf(M, a.part_ml[(g.slot0 + s) * kRows + r].x);
+  for (int s = lane; s < g.splits; s += 32)
+    M = fmaxf(M, part.ml[(int64_t)(g.slot0 + s) * rows + at_row].x);
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFullMask, M, o));
   float L = M == -INFINITY ? 0.0f : ex2(sink - M);
@@ -570,14 +371,14 @@ __global__ void __launch_bounds__(kRows * 32) attn_join_kernel(const __grid_cons
 #pragma unroll
   for (int i = 0; i < HD / 32; ++i) acc[i] = 0.0f;
   for (int s = 0; s < g.splits; ++s) {
-    const int64_t at = (int64_t)(g.slot0 + s) * kRows + r;
-    const float2 ml = a.part_ml[at];
+    const int64_t at = (int64_t)(g.slot0 + s) * rows + at_row;
+    const float2 ml = part.ml[at];
     if (ml.x == -INFINITY) continue;
     const float f = ex2(ml.x - M);
     L += ml.y * f;
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i) {
-      const float2 o = *reinterpret_cast<const float2*>(a.part_o + at * HD + i * 64 + lane * 2);
+      const float2 o = *reinterpret_cast<const float2*>(part.o + at * HD + i * 64 + lane * 2);
       acc[2 * i] += o.x * f;
       acc[2 * i + 1] += o.y * f;
     }
@@ -588,30 +389,57 @@ __global__ void __launch_bounds__(kRows * 32) attn_join_kernel(const __grid_cons
     store_out<T>(a, g.row0 + tok, h, i * 64 + lane * 2, acc[2 * i] * inv, acc[2 * i + 1] * inv);
 }
 
+size_t workspace_layout(int head_dim, char* base, AttnArgs* a) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    char* p = base ? base + at : nullptr;
+    at += (bytes + 255) & ~(size_t)255;
+    return p;
+  };
+  auto part = [&](const Plan& pl, Partials* p) {
+    char* n = take(sizeof(int));
+    char* g = take(sizeof(Group) * pl.target);
+    char* ml = take(sizeof(float2) * pl.slots() * pl.tile_rows);
+    char* o = take(sizeof(float) * (size_t)pl.slots() * pl.tile_rows * head_dim);
+    if (p)
+      *p = Partials{reinterpret_cast<int*>(n), reinterpret_cast<Group*>(g),
+                    reinterpret_cast<float2*>(ml), reinterpret_cast<float*>(o)};
+  };
+  part(kRowsPlan, a ? &a->rows : nullptr);
+  part(head_dim == 256 ? tile_plan<256>() : tile_plan<64>(), a ? &a->tiles : nullptr);
+  return at;
+}
+
 template <typename T, int HD>
-cudaError_t launch_attn(const AttnArgs& a, cudaStream_t st) {
-  const int tpt = kRows / a.group;
-  // tiles: a sequence's last one may be partial
-  const int64_t tiles = std::min<int64_t>((int64_t)a.b.total_q / tpt + a.b.n_seqs, a.b.total_q) * a.b.nkv;
-  // items (see Plan): unsplit tiles, and at most 2 kTargetItems splits
-  const int64_t units = (int64_t)a.b.max_kv / kUnit + 1;
-  const bool splits = units > kMinUnits;
-  const int64_t grid = std::min(tiles + (splits ? kMaxSlots : 0), tiles * units);
+cudaError_t launch_attn(const AttnArgs& a, int dtype, cudaStream_t st) {
+  constexpr Plan tp = tile_plan<HD>();
+  // Decoding sequences: one tile per KV head each.  Nothing on the host says
+  // that there are none, so the kernel runs for every batch (its CTAs without
+  // an item leave at once).
+  const int64_t grid = grid_bound(a, kRowsPlan, (int64_t)std::min(a.b.n_seqs, a.b.total_q) * a.b.nkv);
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   auto kern = attn_rows_kernel<T, HD>;
   cudaError_t e = set_smem_limit(kern, smem_bytes<HD>());
   if (e != cudaSuccess) return e;
   kern<<<(unsigned)grid, kThreads, smem_bytes<HD>(), st>>>(a);
   e = cudaGetLastError();
-  if (e != cudaSuccess || !splits) return e;
-  return launch_pdl(attn_join_kernel<T, HD>, dim3(kTargetItems), dim3(kRows * 32), 0, st, a);
+  if (e != cudaSuccess) return e;
+  const bool tiles = (int64_t)a.b.max_q * a.group > kRows;
+  if (tiles && (e = launch_attn_tiles(a, dtype, HD, true, st)) != cudaSuccess) return e;
+  const bool join_small = a.b.max_kv / kRowsPlan.unit + 1 > kRowsPlan.min_units;
+  const bool join_tiles = tiles && a.b.max_kv / tp.unit + 1 > tp.min_units;
+  const int small_ctas = join_small ? kRowsPlan.target : 0;
+  const int ctas = small_ctas + (join_tiles ? tp.target * (tp.tile_rows / kRows) : 0);
+  if (!ctas) return cudaSuccess;
+  return launch_pdl(attn_join_kernel<T, HD>, dim3(ctas), dim3(kRows * 32), 0, st, a, small_ctas);
 }
 
 template <typename T>
 cudaError_t launch_attn_hd(const AttnArgs& a, int hd, cudaStream_t st) {
-  if (hd == 64) return launch_attn<T, 64>(a, st);
-  if (hd == 128) return launch_attn<T, 128>(a, st);
-  return launch_attn<T, 256>(a, st);
+  const int dt = Elem<T>::kType;
+  if (hd == 64) return launch_attn<T, 64>(a, dt, st);
+  if (hd == 128) return launch_attn<T, 128>(a, dt, st);
+  return launch_attn<T, 256>(a, dt, st);
 }
 
 }  // namespace
@@ -666,6 +494,10 @@ extern "C" int gb_paged_attention(const gb_paged_batch* batch, const gb_attn_arg
       !stride_ok(args->out_head_stride, os))
     return set_error(GB_ERR_INVALID_ARG,
                      "buffers must be 16-byte aligned, strides non-negative multiples of 16 bytes");
+  const int64_t hd = batch->head_dim;
+  if ((batch->total_q > 1 && (args->q_row_stride < hd || args->out_row_stride < hd)) ||
+      (args->n_heads > 1 && (args->q_head_stride < hd || args->out_head_stride < hd)))
+    return set_error(GB_ERR_INVALID_ARG, "row and head strides must be at least head_dim");
   if (args->out_dev == args->q_dev) return set_error(GB_ERR_INVALID_ARG, "out must not be q");
   if (reinterpret_cast<uintptr_t>(args->workspace_dev) & 255)
     return set_error(GB_ERR_INVALID_ARG, "the workspace must be 256-byte aligned");

@@ -1,0 +1,244 @@
+// paged_attn.cuh -- what the two attention kernels share: arguments, the split of
+// a batch into work items, and the output store.
+//
+//   o = sum_j e^(s_j - m) v_j / (e^(sink - m) + sum_j e^(s_j - m)),  s_j = scale (q . k_j)
+//
+// in one pass over K and V with a running maximum and sum.
+//
+// Work.  The query heads that share a KV head are rows of one tile, so each
+// key is read once for all of them: a tile is (rows / group) tokens x group
+// heads.  A sequence with at most kRows such rows (a decoding one) is one
+// 16-row tile of attn_rows_kernel, any other goes to attn_tile_kernel's tiles
+// of 256 (or 128) rows.  A tile's keys are split over several CTAs when the
+// batch has too few tiles to fill the GPU: each split writes its unnormalised
+// sum with its maximum and its sum of weights, and a last kernel joins them in
+// the order of the splits.  The lengths are on the device, so every CTA works
+// out its own item from them (a scan over the sequences), and the grids are
+// sized from the host's bounds.
+#pragma once
+
+#include <algorithm>
+
+#include "paged.cuh"
+#include "ptx.cuh"
+
+namespace gb {
+namespace paged {
+
+// 2^x by the hardware's approximation (relative error 2^-22); 2^-inf = 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRows = 16;      // rows of a decoding sequence's tile, and of a joining CTA
+constexpr int kMaxGroup = 16;  // query heads per KV head
+
+// Splitting.  n = the units (of `unit` keys) a sequence's rows see, t = ceil(W /
+// target) units per split (W: the units of all tiles), so a sequence has
+// ceil(n / t) splits.  Tiles with more than one split have n > t, hence there
+// are at most W / t <= target such tiles (Plan::target entries of `groups`)
+// with at most 2 W / t <= 2 target splits (`slots`).
+struct Plan {
+  int tile_rows;  // rows per tile
+  int unit;       // keys per unit
+  int target;     // items to aim for
+  int min_units;  // units per split, at least
+  __host__ __device__ constexpr int slots() const { return 2 * target; }
+};
+constexpr Plan kRowsPlan{kRows, 64, 296, 2};  // two CTAs on each of 148 SMs
+template <int HD>
+constexpr Plan tile_plan() {
+  return HD == 256 ? Plan{128, 64, 148, 8} : Plan{256, 128, 148, 4};  // one CTA per SM
+}
+
+struct Group {  // a split tile, for the joining kernel
+  int row0, rows, g, slot0, splits;
+};
+
+struct Partials {
+  int* n_groups;
+  Group* groups;    // [target]
+  float2* ml;       // [slots][tile_rows]: reference maximum (log2), sum of weights
+  float* o;         // [slots][tile_rows][head_dim]
+};
+
+struct AttnArgs {
+  Batch b;
+  int nh, group, window, out_f32;
+  float scale;  // scale * log2 e
+  const void* q;
+  int64_t q_row, q_head;
+  const void *k_pool, *v_pool;
+  const float* sinks;
+  void* out;
+  int64_t o_row, o_head;
+  Partials rows, tiles;
+};
+
+// What a CTA does: `tokens` tokens of sequence seq from row row0, the first at
+// position pos0, KV head g, units [u0, u1).
+struct Item {
+  int seq, row0, tokens, pos0, g, u0, u1;
+  int slot;  // of the partial result, -1: the tile is not split
+};
+
+__device__ __forceinline__ int first_unit(int pos, int window, int unit) {
+  return window > 0 && pos >= window ? (pos - window + 1) / unit : 0;
+}
+
+struct SeqWork {
+  int tiles, units;
+};
+template <bool SMALL>
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, const Plan& pl, const Seq& q,
+                                            int tpt) {
+  SeqWork w{0, 0};
+  if ((q.q_len * a.group <= kRows) != SMALL) return w;
+  w.tiles = (q.q_len + tpt - 1) / tpt;
+  const int last = q.kv_len - 1;
+  if (w.tiles && last >= 0)
+    w.units = last / pl.unit - first_unit(max(q.kv_len - q.q_len, 0), a.window, pl.unit) + 1;
+  return w;
+}
+
+template <typename V>
+__device__ __forceinline__ V warp_inclusive(V v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V t = __shfl_up_sync(kFullMask, v, o);
+    if ((threadIdx.x & 31) >= o) v += t;
+  }
+  return v;
+}
+
+// Finds the CTA's item among the sequences of one kind (SMALL: at most kRows
+// rows); false: there is none.  Called by the first THREADS threads of the CTA
+// with `bar` a barrier over them.  tpt: tokens per tile.
+template <bool SMALL, int THREADS>
+__device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& part, int tpt,
+                          Item* out) {
+  constexpr int kW = THREADS / 32;
+  __shared__ unsigned long long red[kW];
+  __shared__ unsigned long long run[kW][2];
+  __shared__ Item found;
+  __shared__ int have;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Batch& b = a.b;
+  Seq mine{0, 0, 0};  // of the first THREADS sequences
+  unsigned long long w = 0;
+  for (int s = tid; s < b.n_seqs; s += THREADS) {
+    const Seq q = load_seq(b, s, blockIdx.x == 0);
+    if (s == tid) mine = q;
+    const SeqWork x = seq_work<SMALL>(a, pl, q, tpt);
+    w += (unsigned long long)x.tiles * x.units;
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) w += __shfl_xor_sync(kFullMask, w, o);
+  if (lane == 0) red[warp] = w;
+  if (tid == 0) have = 0;
+  __syncthreads();
+  w = 0;
+#pragma unroll
+  for (int i = 0; i < kW; ++i) w += red[i];
+  w *= b.nkv;
+  const unsigned long long t64 = (w + pl.target - 1) / pl.target;
+  const int t = (int)(t64 < (unsigned)pl.min_units ? pl.min_units
+                      : t64 > (1u << 30)           ? (1u << 30)
+                                                   : t64);
+  // prefixes over the sequences: items; splits (high half) and tiles of split sequences
+  unsigned long long base_items = 0, base_groups = 0;
+  for (int s0 = 0; s0 < b.n_seqs; s0 += THREADS) {
+    const int s = s0 + tid;
+    Seq q{0, 0, 0};
+    if (s < b.n_seqs) q = s0 ? load_seq(b, s, false) : mine;
+    const SeqWork x = seq_work<SMALL>(a, pl, q, tpt);
+    const int splits = max(1, (x.units + t - 1) / t);
+    const unsigned long long tiles = (unsigned long long)x.tiles * b.nkv;
+    const unsigned long long items = tiles * splits;
+    const unsigned long long groups = splits > 1 ? (items << 32) | tiles : 0;
+    const unsigned long long ii = warp_inclusive(items), gg = warp_inclusive(groups);
+    __syncthreads();
+    if (lane == 31) {
+      run[warp][0] = ii;
+      run[warp][1] = gg;
+    }
+    __syncthreads();
+    unsigned long long bi = base_items, bg = base_groups;
+    for (int i = 0; i < kW; ++i) {
+      if (i < warp) {
+        bi += run[i][0];
+        bg += run[i][1];
+      }
+      base_items += run[i][0];
+      base_groups += run[i][1];
+    }
+    const unsigned long long before = bi + ii - items;
+    if (blockIdx.x >= before && blockIdx.x < before + items) {
+      const unsigned long long j = blockIdx.x - before;
+      const unsigned long long first = bg + gg - groups;
+      Item it;
+      it.seq = s;
+      it.g = (int)(j % b.nkv);
+      const unsigned long long js = j / b.nkv;
+      // the last tile, which sees most keys, first
+      const int split = (int)(js % splits), tile = x.tiles - 1 - (int)(js / splits);
+      it.row0 = q.row0 + tile * tpt;
+      it.tokens = min(tpt, q.q_len - tile * tpt);
+      it.pos0 = q.kv_len - q.q_len + tile * tpt;
+      const int last = it.pos0 + it.tokens - 1;
+      const int lo = first_unit(it.pos0, a.window, pl.unit);
+      const int n = last < 0 ? 0 : last / pl.unit - lo + 1;
+      const int per = (n + splits - 1) / splits;
+      it.u0 = lo + min(split * per, n);
+      it.u1 = lo + min((split + 1) * per, n);
+      it.slot = -1;
+      if (splits > 1) {
+        const int nth = tile * b.nkv + it.g;
+        const int slot0 = (int)(first >> 32) + nth * splits;
+        it.slot = slot0 + split;
+        if (split == 0)
+          part.groups[(int)(uint32_t)first + nth] =
+              Group{it.row0, it.tokens * a.group, it.g, slot0, splits};
+      }
+      found = it;
+      have = 1;
+    }
+  }
+  if (blockIdx.x == 0 && tid == 0) *part.n_groups = (int)(uint32_t)base_groups;
+  __syncthreads();
+  if (!have) return false;
+  *out = found;
+  return true;
+}
+
+template <typename T>
+__device__ __forceinline__ bool any_nonfinite(uint32_t w) {
+  constexpr uint32_t m = Elem<T>::kExpMask;
+  return (w & m) == m || (w & (m << 16)) == (m << 16);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnArgs& a, int row, int head, int d, float x,
+                                          float y) {
+  const int64_t at = row * a.o_row + head * a.o_head + d;
+  if (a.out_f32)
+    *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(x, y);
+  else
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at) = Elem<T>::pack(x, y);
+}
+
+// Grid bound of one kind of tiles: unsplit tiles, and at most plan.slots() splits.
+inline int64_t grid_bound(const AttnArgs& a, const Plan& pl, int64_t tiles) {
+  const int64_t units = (int64_t)a.b.max_kv / pl.unit + 1;
+  return std::min(tiles + (units > pl.min_units ? pl.slots() : 0), tiles * units);
+}
+
+// The tile kernel (paged_attn_tc.cu).  pdl: launched while attn_rows_kernel, on
+// the same stream, still runs; it ends after it.
+cudaError_t launch_attn_tiles(const AttnArgs& a, int dtype, int hd, bool pdl, cudaStream_t st);
+
+}  // namespace paged
+}  // namespace gb

@@ -1,0 +1,620 @@
+// paged_attn_tc.cu -- attention of chunks of new tokens (gb_paged_attention's
+// sequences of more than 16 rows) on the 5th-generation tensor cores.
+//
+// A CTA takes NT row tiles of 128 rows (tokens x the query heads of one KV
+// head) and streams the keys they see in tiles of KT:
+//   S_w = Q_w K^T            tcgen05.mma, A and B in shared memory, S in TMEM
+//   P_w = 2^(S_w scale - m)  a warpgroup per row tile, a thread per row: S from
+//                            TMEM into registers, P back over S as 16-bit pairs
+//   O_w += P_w V             tcgen05.mma, A in TMEM, V as stored (its keys are
+//                            the MMA's K: B is "MN-major")
+// The two row tiles alternate, so the tensor cores work on one while the other
+// is in its softmax.  K and V tiles come by TMA from the pages as stored: a
+// box per page and 64 columns (the 128-byte swizzle), the page number read by
+// a lane of the producer warp; a page that is not needed, or bad, is read as
+// out of range, which TMA fills with zeros.
+//
+// The reference maximum of a row moves only when a score passes the maximum by
+// 2^6 (the weights stay below 2^(kTop + 6)); then the row's warpgroup scales O
+// in TMEM, after its last MMA.  Sums of weights are f32, P is rounded to the
+// pool's type, O accumulates in f32 in TMEM.
+//
+// A tile that some row sees only in part is masked score by score, and its V
+// rows are looked over in shared memory first: rows that no row of the CTA sees
+// are cleared (0 x NaN is NaN), and values that are not finite are cleared and
+// noted: the rows that do see them add them at the end.
+//
+// Warps: 0-3 row tile 0, 4-7 row tile 1 (NT = 2), then a warpgroup with the TMA
+// producer and the MMA issuer (and two idle warps, so that registers can be
+// shifted to the softmax warpgroups, which hold a row of S).  Every wait is
+// bounded, as in the expert GEMMs.
+#include "paged_attn.cuh"
+#include "umma.cuh"
+
+namespace gb {
+namespace paged {
+namespace {
+
+template <int HD>
+struct Cfg {
+  static constexpr int NT = HD == 256 ? 1 : 2;
+  static constexpr int KT = HD == 256 ? 64 : 128;
+  static constexpr int kSub = HD / 64;                      // 64-column blocks
+  static constexpr int kQBytes = NT * 128 * HD * 2;
+  static constexpr int kTileBytes = KT * HD * 2;            // a K or V tile
+  static constexpr int kRing = HD == 64 ? 8 : 5;            // K and V tiles in flight
+  static constexpr int kSoftmax = NT * 128;                 // softmax threads
+  static constexpr int kThreads = kSoftmax + 128;
+  static constexpr int kBarBytes = 256;
+  static constexpr int kSmem = 1024 + kQBytes + kRing * kTileBytes + kBarBytes;
+  static constexpr int kOCol = 256;                         // TMEM: S_0, S_1 below, O_w above
+  static constexpr int kSCol = 128;                         // columns between S_0 and S_1
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                            int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Shared-memory descriptor of an MN-major B matrix (V): 64-element (128-byte
+// swizzled) rows along N, `lbo` bytes between blocks of 64, 8-row groups along
+// K 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lbo) {
+  uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(lbo >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// kind::f16, D = f32, A and B of type T, M = 128, N = n; mn: B is MN-major.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc(int n, bool mn) {
+  const uint32_t t = Elem<T>::kType == GB_DTYPE_BF16 ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+
+#define GB_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), \
+                    "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define GB_W8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), \
+                    "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+// 32 columns of the thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : GB_R8(v, 0), GB_R8(v, 8), GB_R8(v, 16), GB_R8(v, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15};" ::GB_W8(v, 0),
+      GB_W8(v, 8), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Element (row, column) of a K or V tile: blocks of 64 columns, 128-byte rows,
+// 16-byte pieces swizzled by the row.
+template <int HD>
+__device__ __forceinline__ uint32_t tile_offset(int row, int piece) {
+  return (uint32_t)((piece >> 3) * (Cfg<HD>::KT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
+    attn_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a) {
+  using C = Cfg<HD>;
+  constexpr int KT = C::KT, NT = C::NT;
+  constexpr Plan kPlan = tile_plan<HD>();
+  extern __shared__ uint8_t smem_raw[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tpt = 128 / a.group;  // tokens per row tile
+  Item it;
+  const bool have = find_item<false, C::kThreads>(a, kPlan, a.tiles, NT * tpt, &it);
+  pdl_trigger();
+  if (!have) {
+    pdl_wait();  // this grid ends after the kernel it was launched beside
+    return;
+  }
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* ring = smem + C::kQBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::kRing * C::kTileBytes);
+  uint64_t* kv_full = bars;                // [kRing]
+  uint64_t* kv_empty = bars + C::kRing;    // [kRing]
+  uint64_t* q_full = bars + 2 * C::kRing;
+  uint64_t* s_full = q_full + 1;           // [2]
+  uint64_t* p_full = s_full + 2;           // [2]
+  uint64_t* o_done = p_full + 2;           // [2]
+  uint64_t* v_clean = o_done + 2;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word, err_word, poisoned;
+  volatile int* abort_flag = &abort_word;
+
+  // The tiles: row tile w has tokens [w tpt, w tpt + n_w); key tiles [u0, u1).
+  const int n0 = min(it.tokens, tpt), n1 = it.tokens - n0;
+  const int last = it.pos0 + it.tokens - 1;
+  const int key_lo = a.window > 0 ? max(0, it.pos0 - a.window + 1) : 0;
+  const int all_lo = a.window > 0 ? max(0, last - a.window + 1) : 0;
+  // key tiles that row tile w sees any key of
+  const int hi0 = min(it.u1, it.pos0 + n0 - 1 < 0 ? 0 : (it.pos0 + n0 - 1) / KT + 1);
+  const int lo1 = max(it.u0, first_unit(it.pos0 + tpt, a.window, KT));
+  auto active = [&](int w, int j) {
+    return w == 0 ? j < hi0 : n1 > 0 && j >= lo1;
+  };
+  // a tile with a key that some row does not see
+  const int32_t* table = a.b.table + it.seq * a.b.table_stride;
+  const int page_size = 1 << a.b.page_shift;
+  // keys of the tile on bad pages, a bit per page of the tile (lane = page)
+  auto bad_pages = [&](int j) -> unsigned {
+    bool bad = false;
+    const int key = j * KT + lane * page_size;
+    if (lane * page_size < KT && key <= last && key + page_size > key_lo)
+      bad = (unsigned)__ldg(table + (key >> a.b.page_shift)) >= (unsigned)a.b.n_pages;
+    return __ballot_sync(kFullMask, bad);
+  };
+  auto edge = [&](int j) { return j * KT + KT - 1 > it.pos0 || j * KT < all_lo; };
+
+  if (tid == 0) {
+    for (int i = 0; i < C::kRing; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(v_clean, C::kSoftmax);
+    abort_word = err_word = poisoned = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) tmem_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(bar, parity & 1, abort_flag, &err_word);
+  };
+
+  // 384 threads are launched with 168 registers each: 216 + 216 + 72 is that sum.
+  if (warp < C::kSoftmax / 32) {
+    if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // ---------------- softmax: thread = row ---------------------------------------
+    const int w = warp >> 2;               // row tile
+    const int r = tid & 127;               // row of the tile
+    const int tok = r / a.group;           // token of the tile
+    const bool live = tok < (w ? n1 : n0) && r < tpt * a.group;
+    const int head = it.g * a.group + r - tok * a.group;
+    const int pos = live ? it.pos0 + w * tpt + tok : -1;
+    const int first = live && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + w * C::kSCol + lane_base;
+    const uint32_t o_addr = tmem + C::kOCol + w * HD + lane_base;
+    constexpr float kTop = Elem<T>::kTop;
+    float m = -INFINITY, l = 0.0f;  // reference maximum, sum of weights
+    int steps = 0;
+    bool ok = true;
+    for (int j = it.u0; j < it.u1 && ok; ++j) {
+      const bool at_edge = edge(j);
+      if (at_edge) {
+        // look over this thread's share of the V tile
+        const int t = 2 * (j - it.u0) + 1;
+        ok = wait(&kv_full[t % C::kRing], (t / C::kRing) & 1);
+        if (!ok) break;
+        uint8_t* v = ring + (t % C::kRing) * C::kTileBytes;
+        constexpr int kPieces = HD / 8;
+        bool found = false;
+        for (int i = tid; i < KT * kPieces; i += C::kSoftmax) {
+          const int row = i / kPieces, key = j * KT + row;
+          uint4* p = reinterpret_cast<uint4*>(v + tile_offset<HD>(row, i % kPieces));
+          if (key > last || key < key_lo) {
+            *p = make_uint4(0, 0, 0, 0);
+          } else {
+            const uint4 x = *p;
+            if (any_nonfinite<T>(x.x) || any_nonfinite<T>(x.y) || any_nonfinite<T>(x.z) ||
+                any_nonfinite<T>(x.w)) {
+              uint32_t e[4] = {x.x, x.y, x.z, x.w};
+              constexpr uint32_t em = Elem<T>::kExpMask;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                if ((e[c] & em) == em) e[c] &= 0xffff0000u;
+                if ((e[c] & (em << 16)) == (em << 16)) e[c] &= 0xffffu;
+              }
+              *p = make_uint4(e[0], e[1], e[2], e[3]);
+              found = true;
+            }
+          }
+        }
+        if (found) *(volatile int*)&poisoned = 1;
+        fence_proxy_async_smem();
+        mbar_arrive(v_clean);
+      }
+      if (!active(w, j)) continue;
+      const unsigned bad = bad_pages(j);
+      ok = wait(&s_full[w], steps & 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t sb[KT];
+#pragma unroll
+      for (int c = 0; c < KT; c += 32) tmem_ld32(s_addr + c, sb + c);
+      tmem_wait_ld();
+      float* s = reinterpret_cast<float*>(sb);
+      if (at_edge || bad) {
+        const int hi = pos - j * KT, lo = first - j * KT;
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+          if (i > hi || i < lo) s[i] = -INFINITY;
+        for (unsigned left = bad; left; left &= left - 1) {
+          const int b0 = (__ffs(left) - 1) << a.b.page_shift, b1 = b0 + page_size;
+#pragma unroll
+          for (int i = 0; i < KT; ++i)
+            if (i >= b0 && i < b1) s[i] = -INFINITY;
+        }
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int i = 4; i < KT; i += 4)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[i + c]);
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale - kTop;
+      if (__any_sync(kFullMask, top > m + 6.0f)) {
+        const float nm = fmaxf(m, top);
+        const float f = nm == -INFINITY ? 1.0f : ex2(m - nm);
+        m = nm;
+        l *= f;
+        if (steps) {  // O is this row tile's, all its MMAs done
+          ok = wait(&o_done[w], (steps - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(o_addr + c, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < KT / 2; c += 16) {
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = ex2(__fmaf_rn(s[2 * (c + i)], a.scale, -ref));
+          const float y = ex2(__fmaf_rn(s[2 * (c + i) + 1], a.scale, -ref));
+          sum[(2 * i) & 3] += x;
+          sum[(2 * i + 1) & 3] += y;
+          p[i] = Elem<T>::pack(x, y);
+        }
+        tmem_st16(s_addr + c, p);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[w]);
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      ++steps;
+    }
+    // ---- the row's result
+    if (ok && steps) {
+      ok = wait(&o_done[w], (steps - 1) & 1);
+      tc_fence_after();
+    }
+    if (!*abort_flag && ok && (w == 0 || n1 > 0)) {
+      const bool split = it.slot >= 0;
+      float M = m, L = l, inv;
+      if (!split && a.sinks && live) {
+        const float sink = a.sinks[head] * kLog2e;
+        M = fmaxf(m, sink);
+        L = M == -INFINITY ? 0.0f : l * ex2(m - M) + ex2(sink - M);
+      }
+      inv = split ? 1.0f : L == 0.0f || m == -INFINITY ? 0.0f : ex2(m - M) / L;
+      const int out_row = it.row0 + w * tpt + tok;
+      const int64_t part_row = split ? (int64_t)it.slot * kPlan.tile_rows + w * 128 + r : 0;
+      if (split && live) a.tiles.ml[part_row] = make_float2(m, l);
+      const bool poison = *(volatile int*)&poisoned != 0;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        if (steps) {
+          tmem_ld32(o_addr + c, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (!live) continue;
+        if (poison) {
+          // values that are not finite, of the keys this row sees in edge tiles
+          for (int key = max(first, it.u0 * KT); key <= min(pos, it.u1 * KT - 1); ++key) {
+            if (!edge(key / KT)) continue;
+            const int page = __ldg(table + (key >> a.b.page_shift));
+            if ((unsigned)page >= (unsigned)a.b.n_pages) continue;
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(
+                static_cast<const T*>(a.v_pool) + page * a.b.page_stride +
+                (key & (page_size - 1)) * a.b.slot_stride + it.g * a.b.head_stride + c);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t x = __ldg(v + i);
+              if (!any_nonfinite<T>(x)) continue;
+              const float2 f = Elem<T>::unpack(x);
+              constexpr uint32_t em = Elem<T>::kExpMask;
+              if ((x & em) == em) o[2 * i] = __float_as_uint(__uint_as_float(o[2 * i]) + f.x);
+              if ((x & (em << 16)) == (em << 16))
+                o[2 * i + 1] = __float_as_uint(__uint_as_float(o[2 * i + 1]) + f.y);
+            }
+          }
+        }
+        if (split) {
+          float4* d = reinterpret_cast<float4*>(a.tiles.o + part_row * HD + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            d[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                               __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+        } else {
+          const int64_t at = out_row * a.o_row + head * a.o_head + c;
+          float y[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * inv;
+          if (a.out_f32) {
+            float4* d = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              d[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+          } else {
+            uint4* d = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              d[i] = make_uint4(Elem<T>::pack(y[8 * i], y[8 * i + 1]),
+                                Elem<T>::pack(y[8 * i + 2], y[8 * i + 3]),
+                                Elem<T>::pack(y[8 * i + 4], y[8 * i + 5]),
+                                Elem<T>::pack(y[8 * i + 6], y[8 * i + 7]));
+          }
+        }
+      }
+    }
+  } else {
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == C::kSoftmax / 32) {
+      // ---------------- TMA producer: Q, then K and V tiles in turn ---------------
+      bool ok = true;
+      if (lane == 0) {
+        // a box holds the tokens of a row tile with the group's heads: row = token * group + head
+        const uint32_t bytes = (uint32_t)(n1 > 0 ? 2 : 1) * C::kSub * tpt * a.group * 128;
+        mbar_arrive_expect_tx(q_full, bytes);
+        for (int w = 0; w < (n1 > 0 ? 2 : 1); ++w)
+          for (int s = 0; s < C::kSub; ++s)
+            tma_load_3d(smem + (w * C::kSub + s) * 128 * 128, &map_q, s * 64, it.g * a.group,
+                        it.row0 + w * tpt, q_full);
+      }
+      const int box = min(page_size, KT);            // keys per copy
+      const int boxes = KT / box;                    // per 64 columns
+      int slot = 0;
+      uint32_t phase = 0;
+      for (int j = it.u0; j < it.u1 && ok; ++j) {
+        // lane b holds the page of the tile's keys [b box, b box + box)
+        int page = a.b.n_pages, in_page = 0;
+        {
+          const int key = j * KT + lane * box;
+          in_page = key & (page_size - 1);
+          if (lane < boxes && key <= last && key + box > key_lo) {
+            const int p = __ldg(table + (key >> a.b.page_shift));
+            if ((unsigned)p < (unsigned)a.b.n_pages)
+              page = p;
+            else
+              flag(a.b, GB_PAGED_BAD_PAGE);
+          }
+        }
+        for (int kv = 0; kv < 2 && ok; ++kv) {
+          ok = wait(&kv_empty[slot], phase ^ 1);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], C::kTileBytes);
+          __syncwarp();
+          const uint32_t dst = smem_u32(ring + slot * C::kTileBytes);
+          const CUtensorMap* map = kv ? &map_v : &map_k;
+          if (lane < boxes) {
+#pragma unroll
+            for (int s = 0; s < C::kSub; ++s)
+              tma_load_4d(dst + s * KT * 128 + lane * box * 128, map, s * 64, in_page, it.g, page,
+                          &kv_full[slot]);
+          }
+          if (++slot == C::kRing) {
+            slot = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {  // copies in flight land within microseconds
+        const uint64_t t0 = globaltimer();
+        while (globaltimer() - t0 < 2000000ull) {
+        }
+      }
+    } else if (warp == C::kSoftmax / 32 + 1) {
+      // ---------------- MMA issuer -------------------------------------------------
+      if (lane == 0) {
+        bool ok = wait(q_full, 0);
+        // tile t of the ring's order (K of j: 2 (j - u0), V: one more)
+        auto ring_at = [&](int t) { return t % C::kRing; };
+        auto full = [&](int t) { return wait(&kv_full[ring_at(t)], (t / C::kRing) & 1); };
+        uint32_t p_phase[2] = {0, 0}, clean_phase = 0;
+        bool o_any[2] = {false, false};
+        auto issue_s = [&](int w, int j) {
+          const uint32_t q = smem_u32(smem + w * C::kSub * 128 * 128);
+          const uint32_t k = smem_u32(ring + ring_at(2 * (j - it.u0)) * C::kTileBytes);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            mma_ss(tmem + w * C::kSCol, sw128_desc(q + (kk >> 2) * 128 * 128 + (kk & 3) * 32),
+                   sw128_desc(k + (kk >> 2) * KT * 128 + (kk & 3) * 32), idesc<T>(KT, false), kk != 0);
+          mma_commit(&s_full[w]);
+        };
+        if (ok && it.u0 < it.u1) {
+          ok = full(0);
+          tc_fence_after();
+          if (ok) {
+            for (int w = 0; w < NT; ++w)
+              if (active(w, it.u0)) issue_s(w, it.u0);
+            mma_commit(&kv_empty[ring_at(0)]);
+          }
+        }
+        for (int j = it.u0; j < it.u1 && ok; ++j) {
+          const int tk = 2 * (j - it.u0);
+          bool v_ready = false, k_ready = false;
+          for (int w = 0; w < NT && ok; ++w) {
+            if (active(w, j)) {
+              if (!v_ready) {
+                ok = full(tk + 1);
+                if (ok && edge(j)) ok = wait(v_clean, clean_phase);
+                v_ready = true;
+              }
+              ok = ok && wait(&p_full[w], p_phase[w]);
+              if (!ok) break;
+              p_phase[w] ^= 1;
+              tc_fence_after();
+              const uint32_t v = smem_u32(ring + ring_at(tk + 1) * C::kTileBytes);
+#pragma unroll
+              for (int kk = 0; kk < KT / 16; ++kk)
+                mma_ts(tmem + C::kOCol + w * HD, tmem + w * C::kSCol + kk * 8,
+                       sw128_mn_desc(v + kk * 2048, KT * 128), idesc<T>(HD, true),
+                       o_any[w] || kk != 0);
+              o_any[w] = true;
+              mma_commit(&o_done[w]);
+            }
+            if (j + 1 < it.u1 && active(w, j + 1)) {
+              if (!k_ready) {
+                ok = full(tk + 2);
+                tc_fence_after();
+                k_ready = true;
+              }
+              if (ok) issue_s(w, j + 1);
+            }
+          }
+          if (!ok) break;
+          if (!v_ready) {  // neither row tile sees it (the window between them): still in order
+            ok = full(tk + 1);
+            if (ok && edge(j)) ok = wait(v_clean, clean_phase);
+          }
+          if (edge(j)) clean_phase ^= 1;
+          if (ok) mma_commit(&kv_empty[ring_at(tk + 1)]);
+          if (j + 1 < it.u1) {
+            if (ok && !k_ready) ok = full(tk + 2);
+            if (ok) mma_commit(&kv_empty[ring_at(tk + 2)]);
+          }
+        }
+        if (!ok) {  // issued MMAs read shared memory and TMEM: let them finish
+          const uint64_t t0 = globaltimer();
+          while (globaltimer() - t0 < 2000000ull) {
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+  if (tid == 0 && *abort_flag) flag(a.b, GB_PAGED_TIMEOUT);
+  pdl_wait();
+}
+
+cudaError_t make_map(CUtensorMap* m, int dtype, const void* base, int rank, const cuuint64_t* dims,
+                     const cuuint64_t* strides, const cuuint32_t* box) {
+  auto encode = tensor_map_encoder();
+  if (!encode) return cudaErrorNotSupported;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUresult r = encode(
+      m, dtype == GB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+      rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <typename T, int HD>
+cudaError_t launch(const AttnArgs& a, bool pdl, cudaStream_t st) {
+  using C = Cfg<HD>;
+  const int tpt = 128 / a.group;
+  constexpr int dt = Elem<T>::kType;
+  CUtensorMap mq, mk, mv;
+  const int page_size = 1 << a.b.page_shift;
+  // A dimension of one has no stride of its own; the encoder wants a valid one.
+  auto stride = [](int64_t s, int64_t n) { return (cuuint64_t)(n > 1 ? s * 2 : HD * 2); };
+  {
+    const cuuint64_t dims[3] = {HD, (cuuint64_t)a.nh, (cuuint64_t)a.b.total_q};
+    const cuuint64_t strides[2] = {stride(a.q_head, a.nh), stride(a.q_row, a.b.total_q)};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)tpt};
+    const cudaError_t e = make_map(&mq, dt, a.q, 3, dims, strides, box);
+    if (e != cudaSuccess) return e;
+  }
+  for (int v = 0; v < 2; ++v) {
+    const cuuint64_t dims[4] = {HD, (cuuint64_t)page_size, (cuuint64_t)a.b.nkv,
+                                (cuuint64_t)a.b.n_pages};
+    const cuuint64_t strides[3] = {stride(a.b.slot_stride, page_size), stride(a.b.head_stride, a.b.nkv),
+                                   stride(a.b.page_stride, a.b.n_pages)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)std::min(page_size, C::KT), 1, 1};
+    const cudaError_t e = make_map(v ? &mv : &mk, dt, v ? a.v_pool : a.k_pool, 4, dims, strides, box);
+    if (e != cudaSuccess) return e;
+  }
+  const int64_t per = (int64_t)C::NT * tpt;
+  const int64_t tiles = std::min<int64_t>(a.b.total_q / per + a.b.n_seqs, a.b.total_q) * a.b.nkv;
+  const int64_t grid = grid_bound(a, tile_plan<HD>(), tiles);
+  if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  auto kern = attn_tile_kernel<T, HD>;
+  cudaError_t e = set_smem_limit(kern, C::kSmem);
+  if (e != cudaSuccess) return e;
+  if (pdl)
+    return launch_pdl(kern, dim3((unsigned)grid), dim3(C::kThreads), C::kSmem, st, mq, mk, mv, a);
+  kern<<<(unsigned)grid, C::kThreads, C::kSmem, st>>>(mq, mk, mv, a);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_hd(const AttnArgs& a, int hd, bool pdl, cudaStream_t st) {
+  if (hd == 64) return launch<T, 64>(a, pdl, st);
+  if (hd == 128) return launch<T, 128>(a, pdl, st);
+  return launch<T, 256>(a, pdl, st);
+}
+
+}  // namespace
+
+cudaError_t launch_attn_tiles(const AttnArgs& a, int dtype, int hd, bool pdl, cudaStream_t st) {
+  return dtype == GB_DTYPE_BF16 ? launch_hd<__nv_bfloat16>(a, hd, pdl, st)
+                                : launch_hd<__half>(a, hd, pdl, st);
+}
+
+}  // namespace paged
+}  // namespace gb

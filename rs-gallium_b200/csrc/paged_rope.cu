@@ -398,6 +398,9 @@ extern "C" int gb_paged_rope_append(const gb_paged_batch* batch, const gb_rope_a
       !stride_ok(args->v_row_stride, es) || !stride_ok(args->v_head_stride, es))
     return set_error(GB_ERR_INVALID_ARG,
                      "row and head strides must be non-negative multiples of 16 bytes");
+  if (q && ((batch->total_q > 1 && args->out_row_stride < batch->head_dim) ||
+            (args->n_heads > 1 && args->out_head_stride < batch->head_dim)))
+    return set_error(GB_ERR_INVALID_ARG, "q_out's strides must be at least head_dim");
   if (q && args->q_out_dev == args->q_dev &&
       (in != batch->dtype || args->out_row_stride != args->q_row_stride ||
        args->out_head_stride != args->q_head_stride))
