@@ -288,8 +288,8 @@ SIGNATURES = {
     "gb_paged_rope_append": (c_int, [POINTER(PagedBatchDesc), POINTER(RopeArgs), c_void_p]),
     "gb_paged_attention": (c_int, [POINTER(PagedBatchDesc), POINTER(AttnArgs), c_void_p]),
     "gb_paged_attention_workspace": (c_int, [POINTER(PagedBatchDesc), c_int32, POINTER(c_int64)]),
-    "gb_paged_copy": (c_int, [POINTER(c_void_p), c_int32, c_int64, c_int64, c_int64,
-                              POINTER(c_int32), POINTER(c_int32), c_int32, c_void_p]),
+    "gb_paged_copy": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                              c_int32, c_void_p]),
     "gb_sample": (c_int, [POINTER(SampleArgs), c_void_p]),
     "gb_nccl_unique_id": (c_int, [POINTER(c_uint8)]),
     "gb_last_error": (c_char_p, []),

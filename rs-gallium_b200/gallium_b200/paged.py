@@ -11,22 +11,32 @@ current stream of the tensors' device and synchronises nothing:
 from __future__ import annotations
 
 import ctypes
-import math
+from array import array
 from typing import List, Optional, Sequence
 
 from . import _lib
 from ._lib import AttnArgs, GalliumError, PagedBatchDesc, RopeArgs, load_library
 
-_DTYPES = None
+_ROPE_SIZE, _ATTN_SIZE = ctypes.sizeof(RopeArgs), ctypes.sizeof(AttnArgs)
+
+torch = None  # imported by the first call: the package loads without it
+_DTYPES = {}
+_lib_handle = None
+
+
+def _start():
+    global torch, _lib_handle
+    if _lib_handle is None:
+        import torch as t
+
+        torch = t
+        _DTYPES.update({t.float32: _lib.GB_DTYPE_F32, t.bfloat16: _lib.GB_DTYPE_BF16,
+                        t.float16: _lib.GB_DTYPE_F16})
+        _lib_handle = load_library()
+    return _lib_handle
 
 
 def _dtype(t) -> int:
-    global _DTYPES
-    if _DTYPES is None:
-        import torch
-
-        _DTYPES = {torch.float32: _lib.GB_DTYPE_F32, torch.bfloat16: _lib.GB_DTYPE_BF16,
-                   torch.float16: _lib.GB_DTYPE_F16}
     d = _DTYPES.get(t)
     if d is None:
         raise GalliumError(_lib.GB_ERR_UNSUPPORTED, f"dtype {t}: float32, bfloat16 or float16")
@@ -44,26 +54,20 @@ def _check(rc: int) -> None:
 
 def _on(device, name, t):
     if t.device != device:
-        _bad(f"{name} is on {t.device}, the batch on {device}")
+        _bad(f"{name} is on {t.device}, not on {device}")
 
 
-class _Call:
-    """The device's current stream, with that device current during the call."""
-
-    def __init__(self, device):
-        import torch
-
-        self._guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
-        self.stream = torch.cuda.current_stream(device).cuda_stream
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def _call(fn, device, *args) -> None:
+    """fn(*args, stream) on the device's current stream, that device current during the call."""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)  # torch.cuda.current_stream without the Stream object
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc)
 
 
 class PagedBatch:
@@ -79,8 +83,7 @@ class PagedBatch:
 
     def __init__(self, q_start, kv_len, page_table, *, page_size: int, total_q: int, max_q_len: int,
                  max_kv_len: int):
-        import torch
-
+        _start()
         for name, t, nd in (("q_start", q_start, 1), ("kv_len", kv_len, 1), ("page_table", page_table, 2)):
             if t.dtype != torch.int32 or t.dim() != nd or not t.is_cuda:
                 _bad(f"{name} must be an int32 CUDA tensor of {nd} dimension(s)")
@@ -108,14 +111,11 @@ class PagedBatch:
             # kernels bound a position by table_stride entries: keep them inside the tensor
             d.max_kv_len = min(max_kv_len, page_table.shape[1] * page_size)
         d.error_dev = self.error.data_ptr()
+        self.total_q = total_q
         self._desc = d
         self._ref = ctypes.byref(d)
         self._workspace = {}
         self._pool = None
-
-    @property
-    def total_q(self) -> int:
-        return self._desc.total_q
 
     def check(self) -> None:
         """Raises GalliumError when a kernel of this batch flagged its device
@@ -132,39 +132,53 @@ class PagedBatch:
 
     def _set_pool(self, k_pool, v_pool) -> None:
         """Puts the pools' shape, strides and type into the descriptor."""
-        key = (k_pool.shape, k_pool.stride(), k_pool.dtype)
-        if v_pool.shape != key[0] or v_pool.stride() != key[1] or v_pool.dtype != key[2]:
+        shape, strides, dtype = k_pool.shape, k_pool.stride(), k_pool.dtype
+        if v_pool.shape != shape or v_pool.stride() != strides or v_pool.dtype != dtype:
             _bad("the K and V pools differ in shape, strides or dtype")
         _on(self.device, "k_pool", k_pool)
         _on(self.device, "v_pool", v_pool)
-        if key == self._pool:
+        was = self._pool
+        if was is not None and was[0] == shape and was[1] == strides and was[2] == dtype:
             return
-        if k_pool.dim() != 4 or k_pool.shape[1] != self._desc.page_size or (
-                k_pool.shape[3] > 1 and k_pool.stride(3) != 1):
-            _bad(f"a pool is [n_pages, {self._desc.page_size}, n_kv_heads, head_dim] with a contiguous last "
-                 f"dimension, got {tuple(k_pool.shape)} with strides {k_pool.stride()}")
         d = self._desc
-        d.dtype = _dtype(k_pool.dtype)
-        d.n_pages, _, d.n_kv_heads, d.head_dim = k_pool.shape
-        d.page_stride, d.slot_stride, d.head_stride, _ = k_pool.stride()
-        self._pool = key
+        if len(shape) != 4 or shape[1] != d.page_size or (shape[3] > 1 and strides[3] != 1):
+            _bad(f"a pool is [n_pages, {d.page_size}, n_kv_heads, head_dim] with a contiguous last "
+                 f"dimension, got {tuple(shape)} with strides {strides}")
+        d.dtype = _dtype(dtype)
+        d.n_pages, _, d.n_kv_heads, d.head_dim = shape
+        d.page_stride, d.slot_stride, d.head_stride, _ = strides
+        self._pool = (shape, strides, dtype)
 
     def _workspace_bytes(self, n_heads: int) -> int:
         key = (n_heads, self._desc.n_kv_heads, self._desc.head_dim)
         got = self._workspace.get(key)
         if got is None:
             n = ctypes.c_int64()
-            _check(load_library().gb_paged_attention_workspace(self._ref, n_heads, ctypes.byref(n)))
+            _check(_lib_handle.gb_paged_attention_workspace(self._ref, n_heads, ctypes.byref(n)))
             got = self._workspace[key] = n.value
         return got
 
 
 def _rows(name, x, batch, heads, dim):
-    if x.dim() != 3 or x.shape[0] != batch.total_q or (heads is not None and x.shape[1] != heads) or (
-            x.shape[2] != dim) or (dim > 1 and x.stride(2) != 1):
-        _bad(f"{name} must be [{batch.total_q}, {heads or 'heads'}, {dim}] with a contiguous last dimension, "
-             f"got {tuple(x.shape)} with strides {x.stride()}")
-    _on(batch.device, name, x)
+    """The row and head strides of x [total_q, heads, dim]."""
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or shape[0] != batch.total_q or shape[2] != dim or strides[2] != 1 or (
+            heads is not None and shape[1] != heads):
+        _bad(f"{name} must be [{batch.total_q}, {'heads' if heads is None else heads}, {dim}] with a "
+             f"contiguous last dimension, got {tuple(shape)} with strides {strides}")
+    if x.device != batch.device:
+        _on(batch.device, name, x)
+    return strides
+
+
+def _vector(name, x, n, device, dtype=None):
+    """The address of x, a contiguous vector of n values (float32 by default)."""
+    dtype = dtype or torch.float32
+    if x.dtype != dtype or x.dim() != 1 or x.shape[0] != n or not x.is_contiguous():
+        _bad(f"{name} must be a contiguous {dtype} ({n},)")
+    if x.device != device:
+        _on(device, name, x)
+    return x.data_ptr()
 
 
 def rope_append(batch: PagedBatch, q, k, v, k_pool, v_pool, cos=None, sin=None, *, q_norm=None, k_norm=None,
@@ -175,51 +189,44 @@ def rope_append(batch: PagedBatch, q, k, v, k_pool, v_pool, cos=None, sin=None, 
     [total_q, heads, head_dim] f32, bf16 or f16, any row and head strides.
     Returns the queries in the pools' dtype (q_out, when given; q itself is
     allowed when the dtypes agree).  Rows of no sequence keep q_out's values."""
-    import torch
-
     batch._set_pool(k_pool, v_pool)
     d = batch._desc
-    _rows("q", q, batch, None, d.head_dim)
-    _rows("k", k, batch, d.n_kv_heads, d.head_dim)
-    _rows("v", v, batch, d.n_kv_heads, d.head_dim)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    dim, device = d.head_dim, batch.device
+    a = RopeArgs()
+    a.q_row_stride, a.q_head_stride, _ = _rows("q", q, batch, None, dim)
+    a.k_row_stride, a.k_head_stride, _ = _rows("k", k, batch, d.n_kv_heads, dim)
+    a.v_row_stride, a.v_head_stride, _ = _rows("v", v, batch, d.n_kv_heads, dim)
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
         _bad("q, k and v must have one dtype")
+    heads = q.shape[1]
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=k_pool.dtype, device=batch.device)
+        q_out = torch.empty_like(q, dtype=k_pool.dtype)
+        a.out_row_stride, a.out_head_stride, _ = q_out.stride()
     else:
-        _rows("q_out", q_out, batch, q.shape[1], d.head_dim)
+        a.out_row_stride, a.out_head_stride, _ = _rows("q_out", q_out, batch, heads, dim)
         if q_out.dtype != k_pool.dtype:
             _bad(f"q_out must be {k_pool.dtype}")
-    a = RopeArgs()
-    a.struct_size = ctypes.sizeof(RopeArgs)
-    if (cos is None) != (sin is None):
-        _bad("cos and sin come together")
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None:
-            if w.dtype != torch.float32 or w.shape != (d.head_dim,) or not w.is_contiguous():
-                _bad(f"{name} must be a contiguous float32 ({d.head_dim},)")
-            _on(batch.device, name, w)
-    if cos is not None:
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or (
-                cos.shape != sin.shape) or not cos.is_contiguous() or not sin.is_contiguous():
+    a.struct_size = _ROPE_SIZE
+    if cos is not None and sin is not None:
+        shape = cos.shape
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or (
+                sin.shape != shape) or not cos.is_contiguous() or not sin.is_contiguous():
             _bad("cos and sin must be contiguous float32 (positions, rot_dim / 2)")
-        _on(batch.device, "cos", cos)
-        _on(batch.device, "sin", sin)
-        a.rot_dim, a.table_rows = 2 * cos.shape[1], cos.shape[0]
+        _on(device, "cos", cos)
+        _on(device, "sin", sin)
+        a.rot_dim, a.table_rows = 2 * shape[1], shape[0]
         a.cos_dev, a.sin_dev = cos.data_ptr(), sin.data_ptr()
-    a.in_dtype, a.n_heads, a.eps = _dtype(q.dtype), q.shape[1], eps
-    a.q_dev, a.k_dev, a.v_dev, a.q_out_dev = q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr()
-    a.q_row_stride, a.q_head_stride, _ = q.stride()
-    a.k_row_stride, a.k_head_stride, _ = k.stride()
-    a.v_row_stride, a.v_head_stride, _ = v.stride()
-    a.out_row_stride, a.out_head_stride, _ = q_out.stride()
+    elif cos is not None or sin is not None:
+        _bad("cos and sin come together")
     if q_norm is not None:
-        a.q_norm_dev = q_norm.data_ptr()
+        a.q_norm_dev = _vector("q_norm", q_norm, dim, device)
     if k_norm is not None:
-        a.k_norm_dev = k_norm.data_ptr()
+        a.k_norm_dev = _vector("k_norm", k_norm, dim, device)
+    a.in_dtype, a.n_heads, a.eps = _dtype(dtype), heads, eps
+    a.q_dev, a.k_dev, a.v_dev, a.q_out_dev = q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr()
     a.k_pool_dev, a.v_pool_dev = k_pool.data_ptr(), v_pool.data_ptr()
-    with _Call(batch.device) as stream:
-        _check(load_library().gb_paged_rope_append(batch._ref, ctypes.byref(a), stream))
+    _call(_lib_handle.gb_paged_rope_append, device, batch._ref, ctypes.byref(a))
     return q_out
 
 
@@ -230,38 +237,33 @@ def attention(batch: PagedBatch, q, k_pool, v_pool, *, sinks=None, window: int =
     sinks (n_heads,) f32: a sink logit per head; scale defaults to
     head_dim^-1/2.  Returns out (q's shape; the pools' dtype, or float32 when
     such an `out` is given).  Rows of no sequence keep out's values."""
-    import torch
-
     batch._set_pool(k_pool, v_pool)
     d = batch._desc
-    _rows("q", q, batch, None, d.head_dim)
+    dim, device = d.head_dim, batch.device
+    a = AttnArgs()
+    a.q_row_stride, a.q_head_stride, _ = _rows("q", q, batch, None, dim)
     if q.dtype != k_pool.dtype:
         _bad(f"q must be {k_pool.dtype}, as the pools")
     heads = q.shape[1]
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=batch.device)
+        out = torch.empty_like(q)
+        a.out_row_stride, a.out_head_stride, _ = out.stride()
+        a.out_dtype = d.dtype
     else:
-        _rows("out", out, batch, heads, d.head_dim)
+        a.out_row_stride, a.out_head_stride, _ = _rows("out", out, batch, heads, dim)
+        a.out_dtype = _dtype(out.dtype)
     if sinks is not None:
-        if sinks.dtype != torch.float32 or sinks.shape != (heads,) or not sinks.is_contiguous():
-            _bad(f"sinks must be a contiguous float32 ({heads},)")
-        _on(batch.device, "sinks", sinks)
-    a = AttnArgs()
-    a.struct_size = ctypes.sizeof(AttnArgs)
-    a.n_heads, a.window, a.out_dtype = heads, window, _dtype(out.dtype)
-    a.scale = d.head_dim ** -0.5 if scale is None else scale
+        a.sinks_dev = _vector("sinks", sinks, heads, device)
+    a.struct_size = _ATTN_SIZE
+    a.n_heads, a.window = heads, window
+    a.scale = dim ** -0.5 if scale is None else scale
     a.q_dev, a.out_dev = q.data_ptr(), out.data_ptr()
-    a.q_row_stride, a.q_head_stride, _ = q.stride()
-    a.out_row_stride, a.out_head_stride, _ = out.stride()
     a.k_pool_dev, a.v_pool_dev = k_pool.data_ptr(), v_pool.data_ptr()
-    if sinks is not None:
-        a.sinks_dev = sinks.data_ptr()
-    a.workspace_bytes = batch._workspace_bytes(heads)
-    with _Call(batch.device) as stream:
-        # torch's allocator orders the workspace's next use after this stream's work
-        ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=batch.device)
-        a.workspace_dev = ws.data_ptr()
-        _check(load_library().gb_paged_attention(batch._ref, ctypes.byref(a), stream))
+    a.workspace_bytes = size = batch._workspace_bytes(heads)
+    # torch's allocator orders the workspace's next use after this stream's work
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    a.workspace_dev = workspace.data_ptr()
+    _call(_lib_handle.gb_paged_attention, device, batch._ref, ctypes.byref(a))
     return out
 
 
@@ -271,42 +273,42 @@ def copy_pages(pools, src: Sequence[int], dst: Sequence[int]) -> None:
     shape, dtype and strides, whose pages are dense (a page's elements fill one
     block of memory).  src and dst are host integers; a page may be copied to
     several others, none may be written twice or both read and written."""
-    import torch
-
-    if len(src) != len(dst):
+    lib = _start()
+    n = len(src)
+    if n != len(dst):
         _bad("src and dst differ in length")
     if torch.is_tensor(pools):
-        one, n_pools = pools[0] if pools.shape[0] else None, pools.shape[0]
+        one, n_pools = pools, pools.shape[0]
+        shape, strides = pools.shape[1:], pools.stride()[1:]
     else:
         n_pools = len(pools)
-        one = pools[0] if n_pools else None
+        if not n_pools:
+            return
+        one = pools[0]
+        shape, strides, dtype, device = one.shape, one.stride(), one.dtype, one.device
         for p in pools:
-            if p.shape != one.shape or p.stride() != one.stride() or p.dtype != one.dtype or (
-                    p.device != one.device):
+            if p.shape != shape or p.stride() != strides or p.dtype != dtype or p.device != device:
                 _bad("the pools differ in shape, strides, dtype or device")
-    if one is None:
-        return
-    if not one.is_cuda or one.dim() < 2:
+    if not one.is_cuda or len(shape) < 2:
         _bad("a pool is a CUDA tensor of [n_pages, ...]")
-    elems = one[0].numel()
     dense = 1
-    for size, stride in sorted(((z, s) for z, s in zip(one.shape[1:], one.stride()[1:]) if z > 1),
-                               key=lambda v: v[1]):
-        if stride != dense:
-            _bad(f"a pool's pages must be dense, got shape {tuple(one.shape)} with strides {one.stride()}")
-        dense *= size
+    for stride, extent in sorted(zip(strides[1:], shape[1:])):
+        if extent > 1 and stride != dense:
+            _bad(f"a pool's pages must be dense, got shape {tuple(shape)} with strides {strides}")
+        dense *= extent
     size = one.element_size()
-    page_stride = one.stride(0) * size if one.shape[0] > 1 else elems * size
-    if torch.is_tensor(pools):
+    page_stride = strides[0] * size if shape[0] > 1 else dense * size
+    if one is pools:
         step, base = pools.stride(0) * size, pools.data_ptr()
-        ptrs = (ctypes.c_void_p * n_pools)(*[base + i * step for i in range(n_pools)])
+        ptrs = array("Q", [base + i * step for i in range(n_pools)])
     else:
-        ptrs = (ctypes.c_void_p * n_pools)(*[p.data_ptr() for p in pools])
-    n = len(src)
-    s, t = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
-    with _Call(one.device) as stream:
-        _check(load_library().gb_paged_copy(ptrs, n_pools, one.shape[0], elems * size, page_stride, s, t, n,
-                                            stream))
+        ptrs = array("Q", [p.data_ptr() for p in pools])
+    try:
+        s, t = array("i", src), array("i", dst)
+    except (OverflowError, TypeError) as e:
+        _bad(f"src and dst must be 32-bit integers: {e}")
+    _call(lib.gb_paged_copy, one.device, ptrs.buffer_info()[0], n_pools, shape[0], dense * size, page_stride,
+          s.buffer_info()[0], t.buffer_info()[0], n)
 
 
 class PagePool:

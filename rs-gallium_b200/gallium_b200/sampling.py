@@ -4,9 +4,11 @@ from __future__ import annotations
 
 import ctypes
 
-from . import _lib
-from ._lib import SampleArgs, load_library
-from .paged import _bad, _Call, _check, _dtype, _on
+from . import paged
+from ._lib import SampleArgs
+from .paged import _bad, _call, _dtype, _vector
+
+_SIZE = ctypes.sizeof(SampleArgs)
 
 
 def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprobs=None):
@@ -17,30 +19,35 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, t
     equals.  Returns (tokens (rows,) int32, logprobs (rows,) f32): each token
     and the log of its probability among those kept; -1 and -inf for a row with
     nothing above -inf."""
-    import torch
-
-    if logits.dim() != 2 or not logits.is_cuda or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    lib = paged._start()
+    torch = paged.torch
+    shape = logits.shape
+    if len(shape) != 2 or not logits.is_cuda or (shape[1] > 1 and logits.stride(1) != 1):
         _bad("logits must be a CUDA tensor (rows, vocab) with contiguous rows")
-    rows, dev = logits.shape[0], logits.device
-    f32, i32 = torch.float32, torch.int32
-    if tokens is None:
-        tokens = torch.empty(rows, dtype=i32, device=dev)
-    if logprobs is None:
-        logprobs = torch.empty(rows, dtype=f32, device=dev)
+    rows, dev = shape[0], logits.device
     a = SampleArgs()
-    for name, t, want, field in (("u", u, f32, "u_dev"), ("temperature", temperature, f32, "temperature_dev"),
-                                 ("top_k", top_k, i32, "top_k_dev"), ("top_p", top_p, f32, "top_p_dev"),
-                                 ("min_p", min_p, f32, "min_p_dev"), ("tokens", tokens, i32, "token_dev"),
-                                 ("logprobs", logprobs, f32, "logprob_dev")):
-        if t is not None:
-            if t.dtype != want or t.shape != (rows,) or not t.is_contiguous():
-                _bad(f"{name} must be a contiguous {want} ({rows},)")
-            _on(dev, name, t)
-            setattr(a, field, t.data_ptr())
-    a.struct_size = ctypes.sizeof(SampleArgs)
-    a.dtype, a.rows, a.vocab = _dtype(logits.dtype), rows, logits.shape[1]
-    a.row_stride = logits.stride(0) if rows > 1 else logits.shape[1]
+    a.u_dev = _vector("u", u, rows, dev)
+    if tokens is None:
+        tokens = torch.empty_like(u, dtype=torch.int32)
+        a.token_dev = tokens.data_ptr()
+    else:
+        a.token_dev = _vector("tokens", tokens, rows, dev, torch.int32)
+    if logprobs is None:
+        logprobs = torch.empty_like(u)
+        a.logprob_dev = logprobs.data_ptr()
+    else:
+        a.logprob_dev = _vector("logprobs", logprobs, rows, dev)
+    if temperature is not None:
+        a.temperature_dev = _vector("temperature", temperature, rows, dev)
+    if top_k is not None:
+        a.top_k_dev = _vector("top_k", top_k, rows, dev, torch.int32)
+    if top_p is not None:
+        a.top_p_dev = _vector("top_p", top_p, rows, dev)
+    if min_p is not None:
+        a.min_p_dev = _vector("min_p", min_p, rows, dev)
+    a.struct_size = _SIZE
+    a.dtype, a.rows, a.vocab = _dtype(logits.dtype), rows, shape[1]
+    a.row_stride = logits.stride(0) if rows > 1 else shape[1]
     a.logits_dev = logits.data_ptr()
-    with _Call(dev) as stream:
-        _check(load_library().gb_sample(ctypes.byref(a), stream))
+    _call(lib.gb_sample, dev, ctypes.byref(a))
     return tokens, logprobs

@@ -160,9 +160,9 @@ def test_page_copy_refuses_bad_lists(kw, needle):
     kw = dict(dict(src=[0], dst=[1], page_bytes=64, page_stride=64, pool=P, n_pools=1), **kw)
     n = len(kw["src"])
     i32 = ctypes.c_int32 * n
-    pools = (ctypes.c_void_p * 1)(kw["pool"])
-    rc, msg = _call("gb_paged_copy", pools, kw["n_pools"], 4, kw["page_bytes"], kw["page_stride"], i32(*kw["src"]),
-                    i32(*kw["dst"]), n, None)
+    pools, src, dst = (ctypes.c_void_p * 1)(kw["pool"]), i32(*kw["src"]), i32(*kw["dst"])
+    rc, msg = _call("gb_paged_copy", ctypes.addressof(pools), kw["n_pools"], 4, kw["page_bytes"], kw["page_stride"],
+                    ctypes.addressof(src), ctypes.addressof(dst), n, None)
     assert rc == INV and needle in msg, (rc, msg)
     assert _call("gb_paged_copy", None, 0, 4, 64, 64, None, None, 0, None)[0] == _lib.GB_OK
 
