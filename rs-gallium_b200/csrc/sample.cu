@@ -6,21 +6,29 @@
 // works on shared memory, with the CTAs' results exchanged through distributed
 // shared memory.  No workspace, one launch.
 //
-// The kept set of top-k and top-p is a prefix of the tokens in order (falling
-// logit, rising id), so each filter is the search for the element at which a
-// running sum -- of ones for top-k, of weights for top-p -- reaches a target:
-//   1. a histogram of 1024 bins over (max - x), 1/32 of a nat of the scaled
-//      logits each, finds the bin that crosses the target;
-//   2. that bin's elements (tens, usually) are listed on every CTA, and each
-//      thread sums what stands before its element; one of them crosses.
-// A bin of more than kList elements is split again by the bits of its
-// elements' keys, down to a single key, where equal logits go by id.
+// The kept set is a prefix of the tokens in order (falling logit, rising id).
+// The short way, for a filtered row:
+//   1. a histogram of counts, bins of 1/32 of a nat of the scaled logits on an
+//      absolute grid (so that it needs no common maximum), tells from which bin
+//      on no token can be kept;
+//   2. the candidates before it, when they are at most kCand, go to the
+//      cluster's first CTA, which sorts them, applies the filters exactly,
+//      sorts the kept ones by id and draws.
+// Where top-p is over the whole row, its total weight is summed in f32: that
+// decides the cut unless the cut lies within kSlack of a border.
+// The long way, for what remains: each filter is the search for the element at
+// which a running sum -- of ones for top-k, of weights for top-p -- reaches a
+// target, by histograms of 1024 bins (the second and later ones over the bits
+// of the logits, down to a single value, where equal logits go by id); then all
+// kept weights are summed in order of id.  An unfiltered row takes that last
+// step alone.
 //
 // Weights are e^z 2^45, z = (x - max) / T <= 0, rounded to integers: their sums
 // are exact, so neither the order of the sums nor that of the atomics matters.
 // e^z is evaluated in double precision by table and polynomial (Tang's method):
 // z = n ln2 / 32 + r, |r| <= ln2 / 64, e^z = 2^(n div 32) 2^((n mod 32) / 32) P(r)
-// with P the Taylor series to r^6 (the next term is below 2^-58).
+// with P the Taylor series to r^5 (the next term is below 2^-48, an eighth of the
+// largest weight's resolution).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -37,6 +45,13 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;      // portable
 constexpr int kBins = 1024;
 constexpr int kList = 512;          // elements of a bin resolved in one step
+constexpr int kCand = 1024;         // candidates sorted by one CTA: two per thread
+constexpr float kGrid = 32.0f;      // bins per nat
+// Bound of the relative error of an f32 sum of weights: three roundings of an
+// argument of up to 46 (2^z) move a weight by 46 ln 2 x 3 x 2^-24 = 5.7e-6, ex2
+// itself by 2^-22, and sums in parts of at most 98, 21 and 8 terms by 127 x
+// 2^-24 = 7.6e-6; together below 1.4e-5.
+constexpr double kSlack = 1.0 / 32768;
 constexpr int kMaxVocab = 400000;   // 8 x 200 KB of shared memory
 constexpr int kOneBits = 45;        // the largest weight is 2^45: 400000 of them stay below 2^64
 constexpr double kNoWeight = -32.0; // e^z 2^45 rounds to 0 below -46 ln 2 = -31.9
@@ -59,25 +74,36 @@ struct Item {
   int idx;
 };
 
-struct Shared {
+// 16-byte size: the slice lies behind it and is read as float4.
+struct alignas(16) Shared {
   union {
-    struct {  // a bin's sum: 64 bits in two words, because shared memory adds 32 bits natively
-      uint32_t lo[kBins], hi[kBins];
-    };
-    struct {  // after the histogram has been read (gather's exchange)
-      Item all[kList];  // the cluster's elements of the crossing bin
-      uint64_t weight[kList];
+    uint16_t count[kBins];  // the short way's histogram (a slice is below 2^16)
+    uint32_t count2[kBins / 2];
+    uint32_t lo[kBins];     // a bin's sum, low words (shared memory adds 32 bits natively)
+    Item all[kList];        // the cluster's elements of the crossing bin, once the bins are read
+  };
+  union {
+    uint64_t cand[kCand];  // the short way's candidates: key and ~id
+    struct {
+      union {
+        uint32_t hi[kBins];      // the bins' high words
+        uint64_t weight[kList];  // of `all`
+      };
+      Item list[kList];  // this CTA's elements of the crossing bin
     };
   };
-  Item list[kList];  // this CTA's elements of the crossing bin
   double exp_table[32];
   uint64_t warp_sum[kWarps];
+  float warp_sum_f[kWarps];
   uint64_t ex64[2][kMaxCluster];  // exchange slots, by parity of the exchange
   uint32_t ex32[2][kMaxCluster];
   uint64_t above;
   int bin, n_list, answer;
+  int bin_k, bin_p, n_cand;  // the short way: bins that hold the cuts, candidates
   uint32_t key_lo, key_hi;
 };
+
+static_assert(sizeof(Shared) % 16 == 0, "the slice behind Shared is read as float4");
 
 // Logit order as unsigned order: a larger logit has the larger key.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -99,17 +125,17 @@ __device__ __constant__ uint64_t kExpTable[32] = {
     0x3ffae89f995ad3adull, 0x3ffb7f76f2fb5e47ull, 0x3ffc199bdd85529cull, 0x3ffcb720dcef9069ull,
     0x3ffd5818dcfba487ull, 0x3ffdfc97337b9b5full, 0x3ffea4afa2a490daull, 0x3fff50765b6e4540ull};
 
-// The integer weight of a scaled logit z <= 0 (round(e^z 2^45)).
+// The integer weight of a scaled logit z <= 0 (round(e^z 2^45)); no branches, so
+// that several run side by side.
 __device__ __forceinline__ uint64_t weight_of(double z, const double* table) {
-  if (!(z > kNoWeight)) return 0;  // -inf and NaN too
   constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+  const bool none = !(z > kNoWeight);            // -inf and NaN too
+  z = none ? 0.0 : z;
   const double t = fma(z, 0x1.71547652b82fep+5, kMagic);
   const int n = __double2loint(t);
   const double nd = t - kMagic;
-  double r = fma(-nd, 0x1.62e42fef00000p-6, z);
-  r = fma(-nd, 0x1.473de6af278edp-39, r);
-  double p = fma(r, 1.0 / 720, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
+  const double r = fma(-nd, 0x1.62e42fefa39efp-6, z);  // the constant's rounding moves z by at most 32 x 2^-53
+  double p = fma(r, 1.0 / 120, 1.0 / 24);
   p = fma(p, r, 1.0 / 6);
   p = fma(p, r, 0.5);
   p = fma(p, r, 1.0);
@@ -119,7 +145,7 @@ __device__ __forceinline__ uint64_t weight_of(double z, const double* table) {
   const double sc = __hiloint2double(__double2hiint(s) + (e << 20), __double2loint(s));
   // + 2^52: the sum's low mantissa bits are the integer nearest to p sc
   const double w = fma(p, sc, 4503599627370496.0);
-  return (uint64_t)__double_as_longlong(w) & 0xfffffffffffffull;
+  return none ? 0 : (uint64_t)__double_as_longlong(w) & 0xfffffffffffffull;
 }
 
 __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int o) {
@@ -143,8 +169,8 @@ struct Row {
     return k > cut_key || (k == cut_key && idx <= cut_idx);
   }
   __device__ __forceinline__ uint64_t weight(float v) const {
-    if (v == top) return 1ull << kOneBits;  // also where both are +inf
-    return weight_of(((double)v - (double)top) * inv_t, sh.exp_table);
+    const uint64_t w = weight_of(((double)v - (double)top) * inv_t, sh.exp_table);
+    return v == top ? 1ull << kOneBits : w;  // also where both are +inf
   }
   // The first histogram's bin: a non-decreasing function of top - v, since each
   // rounding is monotone.  NaN (0 * inf: T near 0, or infinite) converts to 0.
@@ -152,6 +178,21 @@ struct Row {
     if (v == top) return 0;
     const float d = (top - v) * bin_scale;
     return d < (float)(kBins - 1) ? (int)d : d == d ? kBins - 1 : 0;
+  }
+
+  // f(logit, id) over this CTA's slice, four in flight (the slice is padded with
+  // -inf to a multiple of four).
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const int n4 = (n + 3) / 4;
+#pragma unroll 2
+    for (int q = threadIdx.x; q < n4; q += kThreads) {
+      const float4 v = reinterpret_cast<const float4*>(x)[q];
+      f(v.x, base + 4 * q);
+      f(v.y, base + 4 * q + 1);
+      f(v.z, base + 4 * q + 2);
+      f(v.w, base + 4 * q + 3);
+    }
   }
 
   // Every CTA's value, to be read from ex64[parity] / ex32[parity] until the
@@ -199,11 +240,21 @@ struct Row {
     uint64_t v[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) v[i] = 0;
-    for (int r = 0; r < ranks; ++r) {
-      const Shared* o = cl.map_shared_rank(&sh, r);
+    static_assert(kPer == 2, "a thread reads two bins at once");
+    uint2 l[kMaxCluster], h[kMaxCluster];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        v[i] += (uint64_t)o->lo[j0 + i] | ((uint64_t)o->hi[j0 + i] << 32);
+    for (int r = 0; r < kMaxCluster; ++r) {  // every load before the first is used
+      l[r] = h[r] = make_uint2(0, 0);
+      if (r < ranks) {
+        const Shared* o = cl.map_shared_rank(&sh, r);
+        l[r] = *reinterpret_cast<const uint2*>(o->lo + j0);
+        h[r] = *reinterpret_cast<const uint2*>(o->hi + j0);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      v[0] += (uint64_t)l[r].x | ((uint64_t)h[r].x << 32);
+      v[1] += (uint64_t)l[r].y | ((uint64_t)h[r].y << 32);
     }
     uint64_t mine = 0;
 #pragma unroll
@@ -252,14 +303,13 @@ struct Row {
   __device__ int gather(P pred) {
     if (threadIdx.x == 0) sh.n_list = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const float v = x[i];
+    each([&](float v, int id) {
       const uint32_t k = key_of(v);
-      if (pred(k, v, base + i)) {
+      if (pred(k, v, id)) {
         const int s = atomicAdd(&sh.n_list, 1);
-        if (s < kList) sh.list[s] = Item{k, base + i};
+        if (s < kList) sh.list[s] = Item{k, id};
       }
-    }
+    });
     __syncthreads();
     const int par = exchange(0, (uint32_t)sh.n_list);
     int total = 0;
@@ -360,14 +410,13 @@ struct Row {
     }
     // the bin's span of keys
     uint32_t lo = 0xffffffffu, hi = 0;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const float v = x[i];
+    each([&](float v, int id) {
       const uint32_t k = key_of(v);
-      if (kept(k, base + i) && bin_of(v) == j) {
+      if (kept(k, id) && bin_of(v) == j) {
         lo = min(lo, k);
         hi = max(hi, k);
       }
-    }
+    });
     lo = __reduce_min_sync(kFullMask, lo);
     hi = __reduce_max_sync(kFullMask, hi);
     if (threadIdx.x == 0) {
@@ -392,14 +441,13 @@ struct Row {
       int shift = 0;
       while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
       clear_bins();
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const float v = x[i];
+      each([&](float v, int id) {
         const uint32_t k = key_of(v);
-        if (k >= lo && k <= hi && kept(k, base + i)) {
+        if (k >= lo && k <= hi && kept(k, id)) {
           const uint64_t w = MASS ? weight(v) : 1;
           if (w) add_bin((int)((hi - k) >> shift), w);
         }
-      }
+      });
       find_bin(above, target);
       above = sh.above;
       const uint32_t nh = hi - (min((uint32_t)sh.bin, (hi - lo) >> shift) << shift);
@@ -420,6 +468,214 @@ struct Row {
     cut_tie(lo, need);
   }
 };
+
+// ---- the short way -----------------------------------------------------------
+
+// The grid bin of a logit: a non-decreasing function of v (each rounding is
+// monotone, 0 x inf converts to 0, between the ends).
+__device__ __forceinline__ int grid_of(float v, float scale) {
+  const int g = __float2int_rd(v * scale);
+  return max(-(1 << 28), min(1 << 28, g));
+}
+
+struct Settings {
+  bool use_k, use_p, use_min;
+  int k;
+  float p, least;
+};
+
+// Descending bitonic sort of a[0, m), m a power of two of at most 2 kThreads.
+__device__ __forceinline__ void sort_desc(uint64_t* a, int m) {
+  for (int size = 2; size <= m; size <<= 1)
+    for (int d = size >> 1; d >= 1; d >>= 1) {
+      // pairs of one warp stay within its 64 elements for d <= 32
+      if (d >= 32 || d == size >> 1) __syncthreads();
+      else __syncwarp();
+      const int t = threadIdx.x;
+      if (t < m / 2) {
+        const int i = (t / d) * 2 * d + (t & (d - 1)), j = i + d;
+        const uint64_t x = a[i], y = a[j];
+        if ((x < y) == ((i & size) == 0)) {
+          a[i] = y;
+          a[j] = x;
+        }
+      }
+    }
+  __syncthreads();
+}
+
+// The inclusive sums of the CTA's values, two in a row per thread; total: all.
+template <typename V>
+__device__ __forceinline__ void block_scan2(Shared& sh, V (&v)[2], V* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v[1] += v[0];
+  V inc = v[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V t = __shfl_up_sync(kFullMask, inc, o);
+    if (lane >= o) inc += t;
+  }
+  __syncthreads();
+  if (lane == 31) sh.warp_sum[warp] = inc;
+  __syncthreads();
+  // the warps' sums, scanned by every warp for itself
+  V ws = lane < kWarps ? (V)sh.warp_sum[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const V t = __shfl_up_sync(kFullMask, ws, o);
+    if (lane >= o) ws += t;
+  }
+  const V all = __shfl_sync(kFullMask, ws, kWarps - 1);
+  const V upto = __shfl_sync(kFullMask, ws, (warp + 31) & 31);
+  const V before = inc - v[1] + (warp ? upto : 0);
+  v[0] += before;
+  v[1] += before;
+  *total = all;
+}
+
+__device__ __forceinline__ int pow2_from(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
+
+// The same for few candidates (n <= kFew), a thread each: sums over the pairs
+// instead of sorts, three barriers in all.
+constexpr int kFew = 128;
+__device__ bool finish_few(Row& R, const Settings& st, int n, double approx_total, bool all_min, float u,
+                           int32_t* token, float* logprob) {
+  Shared& sh = R.sh;
+  const int t = threadIdx.x;
+  uint64_t* w = sh.cand + kFew;      // weights
+  uint64_t* wk = sh.cand + 2 * kFew;  // of the kept
+  uint64_t me = 0, mine = 0;
+  if (t < n) {
+    me = sh.cand[t];
+    mine = R.weight(logit_of((uint32_t)(me >> 32)));
+    w[t] = mine;
+  }
+  if (t == 0) sh.above = 0;
+  __syncthreads();
+  int rank = 0;
+  uint64_t before = 0;
+  if (t < n) {
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const bool first = sh.cand[i] > me;
+      rank += first;
+      before += first ? w[i] : 0;
+    }
+    if (st.use_k && rank == min(st.k, n) - 1) sh.above = before + mine;  // the weight of the top k
+  }
+  __syncthreads();
+  bool kept = false, maybe = false;
+  if (t < n && !(st.use_k && rank >= st.k)) {
+    double lo = INFINITY, hi = INFINITY;
+    if (st.use_p) {
+      const double z = (double)st.p * (st.use_k ? (double)sh.above : approx_total * (double)(1ull << kOneBits));
+      lo = st.use_k ? z : z * (1.0 - kSlack);
+      hi = st.use_k ? z : z * (1.0 + kSlack);
+    }
+    const bool big = !st.use_min || (double)mine >= (double)st.least * (double)(1ull << kOneBits);
+    kept = rank == 0 || (big && (double)before < lo);
+    maybe = rank == 0 || (big && (double)before < hi);
+    // top-p must end within the candidates, unless min_p does
+    if (st.use_p && !st.use_k && !all_min && kept && rank == n - 1 && (double)(before + mine) < hi) maybe = false;
+  }
+  if (t < n) wk[t] = kept ? mine : 0;
+  if (__syncthreads_or(kept != maybe)) return false;
+  if (kept) {
+    uint64_t below = 0, all = 0;
+    const uint32_t nid = (uint32_t)me;  // ~id
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const uint64_t v = wk[i];
+      all += v;
+      below += (uint32_t)sh.cand[i] > nid ? v : 0;
+    }
+    uint64_t at = (uint64_t)((double)u * (double)all);
+    if (!(u < 1.0f) || at >= all) at = all - 1;
+    if (below <= at && at < below + mine) {
+      *token = (int)~nid;
+      if (logprob) *logprob = (float)log((double)mine / (double)all);
+    }
+  }
+  return true;
+}
+
+// The first CTA, with the candidates (every token from the first in order to
+// some later one) in sh.cand: the filters and the draw.  approx_total: the
+// row's weight in units of the largest, where top-p is over the whole row.
+// all_min: every token that min_p keeps is among them.  false: the cut is too
+// close to a border for that total.
+__device__ bool finish(Row& R, const Settings& st, int n, double approx_total, bool all_min, float u,
+                       int32_t* token, float* logprob) {
+  Shared& sh = R.sh;
+  const int t = threadIdx.x;
+  if (n <= kFew) return finish_few(R, st, n, approx_total, all_min, u, token, logprob);
+  int m = pow2_from(n);
+  for (int i = n + t; i < m; i += kThreads) sh.cand[i] = 0;
+  sort_desc(sh.cand, m);
+  // two elements per thread, in order
+  unsigned long long w[2] = {0, 0}, inc[2], all;
+  const int i0 = 2 * t;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (i0 + e < n && (!st.use_k || i0 + e < st.k))
+      w[e] = R.weight(logit_of((uint32_t)(sh.cand[i0 + e] >> 32)));
+  inc[0] = w[0];
+  inc[1] = w[1];
+  block_scan2(sh, inc, &all);
+  double lo = INFINITY, hi = INFINITY;  // the weight before a kept token is below lo, if not unsure
+  if (st.use_p) {
+    if (st.use_k) {
+      lo = hi = (double)st.p * (double)all;
+    } else {
+      const double z = (double)st.p * approx_total * (double)(1ull << kOneBits);
+      lo = z * (1.0 - kSlack);
+      hi = z * (1.0 + kSlack);
+    }
+  }
+  const double min_w = st.use_min ? (double)st.least * (double)(1ull << kOneBits) : 0.0;
+  int kept = 0, maybe = 0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = i0 + e;
+    if (i >= n || (st.use_k && i >= st.k)) continue;
+    const double before = (double)(inc[e] - w[e]);
+    const bool big = (double)w[e] >= min_w;
+    kept += i == 0 || (big && before < lo);
+    maybe += i == 0 || (big && before < hi);
+  }
+  const unsigned long long sum = (unsigned long long)R.block_sum(((uint64_t)maybe << 32) | (uint32_t)kept);
+  const int c = (int)(uint32_t)sum;
+  if ((int)(sum >> 32) != c) return false;
+  // top-p must end within the candidates, unless min_p does
+  if (st.use_p && !st.use_k && !all_min && c == n && (double)all < hi) return false;
+  // the kept ones by id: descending ~id
+  uint64_t item[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    item[e] = i0 + e < c ? (sh.cand[i0 + e] << 32) | (sh.cand[i0 + e] >> 32) : 0;
+  m = pow2_from(c);
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (i0 + e < m) sh.cand[i0 + e] = item[e];
+  sort_desc(sh.cand, m);
+  w[0] = w[1] = 0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (i0 + e < c) w[e] = R.weight(logit_of((uint32_t)sh.cand[i0 + e]));
+  inc[0] = w[0];
+  inc[1] = w[1];
+  block_scan2(sh, inc, &all);
+  uint64_t at = (uint64_t)((double)u * (double)all);
+  if (!(u < 1.0f) || at >= all) at = all - 1;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (i0 + e < c && inc[e] - w[e] <= at && at < inc[e]) {
+      *token = (int)~(uint32_t)(sh.cand[i0 + e] >> 32);
+      if (logprob) *logprob = (float)log((double)w[e] / (double)all);
+    }
+  return true;
+}
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -472,26 +728,64 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       xs[i] = f;
     }
   }
+  for (int i = n + tid; i < (n + 3) / 4 * 4; i += kThreads) xs[i] = -INFINITY;
   const float t = a.temperature ? a.temperature[row] : 1.0f;
-  const int k = a.top_k ? a.top_k[row] : 0;
-  const float p = a.top_p ? a.top_p[row] : 1.0f;
-  const float least = a.min_p ? a.min_p[row] : 0.0f;
-  for (int j = tid; j < kBins; j += kThreads) sh.lo[j] = sh.hi[j] = 0;
+  Settings st;
+  st.k = a.top_k ? a.top_k[row] : 0;
+  st.p = a.top_p ? a.top_p[row] : 1.0f;
+  st.least = a.min_p ? a.min_p[row] : 0.0f;
+  const bool greedy = !(t > 0.0f) || st.k == 1 || st.p <= 0.0f || st.least > 1.0f;
+  st.use_k = st.k > 0 && st.k < a.vocab;
+  st.use_p = st.p < 1.0f;
+  st.use_min = st.least > 0.0f;
+  const bool filtered = !greedy && (st.use_k || st.use_p || st.use_min);
+  float u = a.u[row];
+  u = u > 0.0f ? u : 0.0f;
+  for (int j = tid; j < kBins / 2; j += kThreads) sh.count2[j] = 0;
   if (tid < 32) sh.exp_table[tid] = __longlong_as_double((long long)kExpTable[tid]);
+  if (tid == 0) {
+    sh.n_list = 0;
+    sh.bin_k = sh.bin_p = 0x7fffffff;
+  }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-  if (lane == 0) sh.warp_sum[warp] = __float_as_uint(top);
+  if (lane == 0) sh.warp_sum_f[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, __uint_as_float((uint32_t)sh.warp_sum[w]));
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.warp_sum_f[w]);
   Row R{cl, sh, xs, n, base, rank, ranks, 0, 0.0f, 0.0, 0.0f, 0u, 0x7fffffff};
-  int par = R.exchange(0, __float_as_uint(top));
+
+  // The short way's histogram, from the slice's own largest logit down, and
+  // its weight in f32 where top-p is over the whole row.
+  const float grid = kGrid / t;
+  const int my_top = grid_of(top, grid);
+  const bool whole_p = filtered && st.use_p && !st.use_k;
+  float z_sum = 0.0f;
+  if (filtered) {
+    const float c = 1.4426950408889634f / t;
+    float part = 0.0f;
+    R.each([&](float v, int) {
+      const int b = my_top - grid_of(v, grid);
+      if (b < kBins) atomicAdd(&sh.count2[b >> 1], 1u << ((b & 1) * 16));
+      if (whole_p) part += exp2f((v - top) * c);
+    });
+    if (whole_p) {
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) part += __shfl_xor_sync(kFullMask, part, o);
+      __syncthreads();
+      if (lane == 0) sh.warp_sum_f[warp] = part;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) z_sum += sh.warp_sum_f[w];
+    }
+  }
+  int par = R.exchange(__float_as_uint(z_sum), __float_as_uint(top));
   for (int r = 0; r < ranks; ++r) top = fmaxf(top, __uint_as_float(sh.ex32[par][r]));
   R.top = top;
 
   // no token can be drawn, or the first in order is the answer
   const bool none = top == -INFINITY;
-  if (none || !(t > 0.0f) || k == 1 || p <= 0.0f || least > 1.0f) {
+  if (none || greedy) {
     uint32_t first = 0x7fffffff;
     if (!none)
       for (int i = tid; i < n; i += kThreads)
@@ -515,30 +809,133 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   R.inv_t = 1.0 / (double)t;
   R.bin_scale = 32.0f / t;
 
-  if (k > 0 && k < a.vocab) {
-    for (int i = tid; i < n; i += kThreads) atomicAdd(&sh.lo[R.bin_of(xs[i])], 1u);
-    R.select<false>((uint64_t)k);
-    R.clear_bins();
-  }
-  if (p < 1.0f) {
-    // Tokens that even together weigh less than (1 - p) of the largest cannot
-    // hold the crossing: they count into the total alone.
-    const double skip = 0.999 * (1.0 - (double)p) * (double)(1ull << kOneBits) / a.vocab;
-    const uint64_t floor_w = (uint64_t)skip;
-    uint64_t sum = 0;
-    for (int i = tid; i < n; i += kThreads) {
-      const float v = xs[i];
-      if (R.kept(key_of(v), base + i)) {
-        const uint64_t w = R.weight(v);
-        sum += w;
-        if (w > floor_w) R.add_bin(R.bin_of(v), w);
+  if (filtered && top < INFINITY) {
+    const int top_bin = grid_of(top, grid);
+    // the cluster's counts, two bins per thread, every load before the first is used
+    const int j0 = 2 * tid;
+    uint32_t got[2 * kMaxCluster];
+    double total = 0.0;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      got[2 * r] = got[2 * r + 1] = 0;
+      if (r < ranks) {
+        const float rt = __uint_as_float(sh.ex32[par][r]);
+        const int j = j0 - (top_bin - grid_of(rt, grid));
+        const Shared* o = cl.map_shared_rank(&sh, r);
+        // bins j and j + 1: one word, or the halves of two
+        if (j + 1 >= 0) {
+          const int q = (j + 1) >> 1;
+          got[2 * r + 1] = o->count2[q];
+          if (j >= 0 && (j & 1)) got[2 * r] = o->count2[q - 1];
+        }
+        if (whole_p && rt > -INFINITY)
+          total += (double)__uint_as_float((uint32_t)sh.ex64[par][r]) *
+                   (double)exp2f((rt - top) * (1.4426950408889634f / t));
       }
     }
+    uint32_t cnt[2] = {0, 0}, inc[2], all;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      if (r < ranks) {
+        const float rt = __uint_as_float(sh.ex32[par][r]);
+        const int j = j0 - (top_bin - grid_of(rt, grid));
+        const bool odd = j & 1;
+        cnt[0] += odd ? got[2 * r] >> 16 : j >= 0 ? got[2 * r + 1] & 0xffffu : 0u;
+        cnt[1] += odd ? got[2 * r + 1] & 0xffffu : got[2 * r + 1] >> 16;
+      }
+    }
+    inc[0] = cnt[0];
+    inc[1] = cnt[1];
+    block_scan2(sh, inc, &all);
+    if (st.use_k) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (inc[e] - cnt[e] < (uint32_t)st.k && (uint32_t)st.k <= inc[e]) sh.bin_k = j0 + e;
+    }
+    if (whole_p) {
+      // each bin's weight from below, in units of 2^-30: where it reaches top_p, the cut lies before
+      unsigned long long low[2], lows[2], low_all;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        low[e] = lows[e] = cnt[e] * (uint64_t)(exp2f(-(float)(j0 + e + 1) * (1.4426950408889634f / kGrid)) * 1073741824.0f);
+      block_scan2(sh, lows, &low_all);
+      const double want = (double)st.p * total * (1.0 + kSlack) * 1073741824.0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if ((double)(lows[e] - low[e]) < want && want <= (double)lows[e]) sh.bin_p = j0 + e;
+    }
+    __syncthreads();
+    // the last bin that min_p keeps a token of, with room for the roundings
+    int bin_min = 0x7fffffff;
+    if (st.use_min) {
+      float v = top + t * logf(st.least);
+      v -= 1e-6f * (fabsf(top) + fabsf(v));
+      bin_min = max(0, min(1 << 28, top_bin - grid_of(v, grid) + 1));
+    }
+    int j = st.use_k ? sh.bin_k : whole_p ? sh.bin_p : 0x7fffffff;
+    const bool all_min = st.use_min && bin_min <= j;
+    if (all_min && !(st.use_k && st.use_p)) j = bin_min;
+    if (j < kBins) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (j0 + e == j) sh.n_cand = (int)inc[e];
+      __syncthreads();
+      const int n_cand = sh.n_cand;
+      if (n_cand <= kCand) {
+        const int from = top_bin - j;
+        // floor(y) >= from <=> y >= from, where `from` is a float
+        const bool plain = abs(from) < (1 << 24);
+        const float from_f = (float)from;
+        R.each([&](float v, int id) {
+          if ((plain ? v * grid >= from_f : grid_of(v, grid) >= from) && v > -INFINITY) {
+            const int s = atomicAdd(&sh.n_list, 1);
+            if (s < kCand) sh.cand[s] = ((uint64_t)key_of(v) << 32) | (uint32_t)~id;
+          }
+        });
+        __syncthreads();
+        if (rank != 0) {  // to the first CTA
+          const int mine = min(sh.n_list, kCand);
+          Shared* o = cl.map_shared_rank(&sh, 0);
+          if (tid == 0) sh.answer = mine ? atomicAdd(&o->n_list, mine) : 0;
+          __syncthreads();
+          const int at = sh.answer;
+          for (int i = tid; i < mine && at + i < kCand; i += kThreads) o->cand[at + i] = sh.cand[i];
+        }
+        cl.sync();
+        bool done = true;
+        if (rank == 0)
+          done = finish(R, st, min(sh.n_list, kCand), total, all_min, u, a.token + row,
+                        a.logprob ? a.logprob + row : nullptr);
+        if (!whole_p) return;  // nothing of another CTA is read any more
+        par = R.exchange(0, done);
+        if (sh.ex32[par][0]) return;
+      }
+    }
+    R.exchange(0, 0);  // the counts are read no more
+  }
+
+  if (st.use_k) {
+    R.clear_bins();
+    R.each([&](float v, int) { atomicAdd(&sh.lo[R.bin_of(v)], 1u); });
+    R.select<false>((uint64_t)st.k);
+  }
+  if (st.use_p) {
+    R.clear_bins();
+    // Tokens that even together weigh less than (1 - p) of the largest cannot
+    // hold the crossing: they count into the total alone.
+    const double skip = 0.999 * (1.0 - (double)st.p) * (double)(1ull << kOneBits) / a.vocab;
+    const uint64_t floor_w = (uint64_t)skip;
+    uint64_t sum = 0;
+    R.each([&](float v, int id) {
+      const uint64_t w = R.kept(key_of(v), id) ? R.weight(v) : 0;
+      sum += w;
+      if (w > floor_w) R.add_bin(R.bin_of(v), w);
+    });
     sum = R.block_sum(sum);
     par = R.exchange(sum, 0);
     uint64_t total = 0;
     for (int r = 0; r < ranks; ++r) total += sh.ex64[par][r];
-    const double want = ceil((double)p * (double)total);
+    const double want = ceil((double)st.p * (double)total);
     uint64_t target = (uint64_t)want;
     target = target < 1 ? 1 : target > total ? total : target;
     R.select<true>(target);
@@ -548,18 +945,25 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   // elements: no bank conflicts), so the parts are in order of id.
   const int part = ((n + kThreads - 1) / kThreads) | 1;
   const int i0 = min(tid * part, n), i1 = min(i0 + part, n);
-  const double min_w = (double)least * (double)(1ull << kOneBits);
+  const double min_w = (double)st.least * (double)(1ull << kOneBits);
   // the scaled logit below which min_p surely drops a token
-  const double z_min = least > 0.0f ? log((double)least) - 1e-6 : -INFINITY;
+  const double z_min = st.use_min ? log((double)st.least) - 1e-6 : -INFINITY;
   auto final_weight = [&](int i) -> uint64_t {
     const float v = xs[i];
+    if (!filtered) return R.weight(v);
     if (!R.kept(key_of(v), base + i)) return 0;
     if (v != top && ((double)v - (double)top) * R.inv_t < z_min) return 0;
     const uint64_t w = R.weight(v);
     return (double)w >= min_w ? w : 0;
   };
   uint64_t mine = 0;
-  for (int i = i0; i < i1; ++i) mine += final_weight(i);
+  if (filtered) {
+#pragma unroll 2
+    for (int i = i0; i < i1; ++i) mine += final_weight(i);
+  } else {
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) mine += R.weight(xs[i]);
+  }
   uint64_t inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -580,8 +984,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     if (r < rank) before += sh.ex64[par][r];
     total += sh.ex64[par][r];
   }
-  float u = a.u[row];
-  u = u > 0.0f ? u : 0.0f;
   uint64_t at = (uint64_t)((double)u * (double)total);  // cumulative > u total <=> cumulative > at
   if (!(u < 1.0f) || at >= total) at = total - 1;
   const bool owner = before <= at && at < before + mine;
