@@ -340,53 +340,55 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
   }
 }
 
-// Joins the split tiles: a warp per row, its splits in order.  CTAs 0 ..
-// kRowsPlan.target - 1 take the 16-row tiles, the others 16 rows each of the
-// larger ones.
+// Joins the split tiles: a warp per row, its splits in order.  Both kinds of
+// tiles in pieces of kRows rows, a CTA per piece in turn.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kRows * 32)
-    attn_join_kernel(const __grid_constant__ AttnArgs a, int small_ctas) {
+__global__ void __launch_bounds__(kRows * 32) attn_join_kernel(const __grid_constant__ AttnArgs a) {
   pdl_wait();
   constexpr int kTileRows = tile_plan<HD>().tile_rows, kParts = kTileRows / kRows;
-  const bool small = (int)blockIdx.x < small_ctas;
-  const Partials& part = small ? a.rows : a.tiles;
-  const int cta = small ? blockIdx.x : blockIdx.x - small_ctas;
-  const int group = small ? cta : cta / kParts, rows = small ? kRows : kTileRows;
-  if (group >= __ldcg(part.n_groups)) return;
-  const Group g = part.groups[group];
-  const int r = (small ? 0 : cta % kParts * kRows) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (r >= g.rows) return;
-  const int tok = r / a.group, h = g.g * a.group + r - tok * a.group;
-  // A large tile's rows are in sub-tiles of 128, each of whole tokens.
-  const int per = small ? kRows : 128 / a.group * a.group;
-  const int at_row = r / per * 128 + r % per;
-  const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-  float M = sink;
-  for (int s = lane; s < g.splits; s += 32)
-    M = fmaxf(M, part.ml[(int64_t)(g.slot0 + s) * rows + at_row].x);
+  const int n_small = a.all_tiles ? 0 : __ldcg(a.rows.n_groups);
+  const int n_tiles = a.tiles.n_groups ? __ldcg(a.tiles.n_groups) : 0;
+  const int lane = threadIdx.x & 31;
+  for (int i = blockIdx.x; i < n_small + n_tiles * kParts; i += gridDim.x) {
+    const bool small = i < n_small;
+    const Partials& part = small ? a.rows : a.tiles;
+    const int rows = small ? kRows : kTileRows;
+    const Group g = part.groups[small ? i : (i - n_small) / kParts];
+    const int r = (small ? 0 : (i - n_small) % kParts * kRows) + (threadIdx.x >> 5);
+    if (r >= g.rows) continue;
+    const int tok = r / a.group, h = g.g * a.group + r - tok * a.group;
+    // A large tile's rows are in sub-tiles of 128, each of whole tokens.
+    const int per = small ? kRows : 128 / a.group * a.group;
+    const int at_row = r / per * 128 + r % per;
+    const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
+    float M = sink;
+    for (int s = lane; s < g.splits; s += 32)
+      M = fmaxf(M, part.ml[(int64_t)(g.slot0 + s) * rows + at_row].x);
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFullMask, M, o));
-  float L = M == -INFINITY ? 0.0f : ex2(sink - M);
-  float acc[HD / 32];
+    for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFullMask, M, o));
+    float L = M == -INFINITY ? 0.0f : ex2(sink - M);
+    float acc[HD / 32];
 #pragma unroll
-  for (int i = 0; i < HD / 32; ++i) acc[i] = 0.0f;
-  for (int s = 0; s < g.splits; ++s) {
-    const int64_t at = (int64_t)(g.slot0 + s) * rows + at_row;
-    const float2 ml = part.ml[at];
-    if (ml.x == -INFINITY) continue;
-    const float f = ex2(ml.x - M);
-    L += ml.y * f;
+    for (int i = 0; i < HD / 32; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < g.splits; ++s) {
+      const int64_t at = (int64_t)(g.slot0 + s) * rows + at_row;
+      const float2 ml = part.ml[at];
+      // an empty split's sums are not written
+      const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+      L += f == 0.0f ? 0.0f : ml.y * f;
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i) {
-      const float2 o = *reinterpret_cast<const float2*>(part.o + at * HD + i * 64 + lane * 2);
-      acc[2 * i] += o.x * f;
-      acc[2 * i + 1] += o.y * f;
+      for (int i = 0; i < HD / 64; ++i) {
+        const float2 o = *reinterpret_cast<const float2*>(part.o + at * HD + i * 64 + lane * 2);
+        acc[2 * i] += ml.x == -INFINITY ? 0.0f : o.x * f;
+        acc[2 * i + 1] += ml.x == -INFINITY ? 0.0f : o.y * f;
+      }
     }
-  }
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-  for (int i = 0; i < HD / 64; ++i)
-    store_out<T>(a, g.row0 + tok, h, i * 64 + lane * 2, acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    for (int i = 0; i < HD / 64; ++i)
+      store_out<T>(a, g.row0 + tok, h, i * 64 + lane * 2, acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  }
 }
 
 size_t workspace_layout(int head_dim, char* base, AttnArgs* a) {
@@ -406,32 +408,36 @@ size_t workspace_layout(int head_dim, char* base, AttnArgs* a) {
                     reinterpret_cast<float2*>(ml), reinterpret_cast<float*>(o)};
   };
   part(kRowsPlan, a ? &a->rows : nullptr);
-  part(head_dim == 256 ? tile_plan<256>() : tile_plan<64>(), a ? &a->tiles : nullptr);
+  part(head_dim == 64 ? tile_plan<64>() : head_dim == 128 ? tile_plan<128>() : tile_plan<256>(),
+       a ? &a->tiles : nullptr);
   return at;
 }
 
 template <typename T, int HD>
-cudaError_t launch_attn(const AttnArgs& a, int dtype, cudaStream_t st) {
+cudaError_t launch_attn(AttnArgs a, int dtype, cudaStream_t st) {
   constexpr Plan tp = tile_plan<HD>();
-  // Decoding sequences: one tile per KV head each.  Nothing on the host says
-  // that there are none, so the kernel runs for every batch (its CTAs without
-  // an item leave at once).
-  const int64_t grid = grid_bound(a, kRowsPlan, (int64_t)std::min(a.b.n_seqs, a.b.total_q) * a.b.nkv);
-  if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  auto kern = attn_rows_kernel<T, HD>;
-  cudaError_t e = set_smem_limit(kern, smem_bytes<HD>());
-  if (e != cudaSuccess) return e;
-  kern<<<(unsigned)grid, kThreads, smem_bytes<HD>(), st>>>(a);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  // Chunks: some sequence may have more than kRows rows.  Decoding sequences:
+  // some may have fewer, since not all can be as long as the longest.
   const bool tiles = (int64_t)a.b.max_q * a.group > kRows;
-  if (tiles && (e = launch_attn_tiles(a, dtype, HD, true, st)) != cudaSuccess) return e;
-  const bool join_small = a.b.max_kv / kRowsPlan.unit + 1 > kRowsPlan.min_units;
-  const bool join_tiles = tiles && a.b.max_kv / tp.unit + 1 > tp.min_units;
-  const int small_ctas = join_small ? kRowsPlan.target : 0;
-  const int ctas = small_ctas + (join_tiles ? tp.target * (tp.tile_rows / kRows) : 0);
-  if (!ctas) return cudaSuccess;
-  return launch_pdl(attn_join_kernel<T, HD>, dim3(ctas), dim3(kRows * 32), 0, st, a, small_ctas);
+  const int64_t least = a.b.total_q - (int64_t)(a.b.n_seqs - 1) * a.b.max_q;
+  a.all_tiles = tiles && least * a.group > kRows;
+  if (!tiles) a.tiles.n_groups = nullptr;
+  cudaError_t e;
+  if (!a.all_tiles) {
+    const int64_t grid =
+        grid_bound(a, kRowsPlan, (int64_t)std::min(a.b.n_seqs, a.b.total_q) * a.b.nkv);
+    if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    auto kern = attn_rows_kernel<T, HD>;
+    if ((e = set_smem_limit(kern, smem_bytes<HD>())) != cudaSuccess) return e;
+    kern<<<(unsigned)grid, kThreads, smem_bytes<HD>(), st>>>(a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
+  if (tiles && (e = launch_attn_tiles(a, dtype, HD, !a.all_tiles, st)) != cudaSuccess) return e;
+  // No sequence is split when the longest has too few keys for two splits.
+  const bool join = (!a.all_tiles && a.b.max_kv / kRowsPlan.unit + 1 > kRowsPlan.min_units) ||
+                    (tiles && a.b.max_kv / tp.unit + 1 > tp.min_units);
+  if (!join) return cudaSuccess;
+  return launch_pdl(attn_join_kernel<T, HD>, dim3(296), dim3(kRows * 32), 0, st, a);
 }
 
 template <typename T>

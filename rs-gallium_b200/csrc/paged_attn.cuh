@@ -9,7 +9,10 @@
 // key is read once for all of them: a tile is (rows / group) tokens x group
 // heads.  A sequence with at most kRows such rows (a decoding one) is one
 // 16-row tile of attn_rows_kernel, any other goes to attn_tile_kernel's tiles
-// of 256 (or 128) rows.  A tile's keys are split over several CTAs when the
+// of 128 or 256 rows (where the host's bounds tell that no sequence of the
+// batch is a decoding one, attn_rows_kernel is not launched, and should the
+// device's lengths say otherwise, the tile kernel takes that sequence too).  A
+// tile's keys are split over several CTAs when the
 // batch has too few tiles to fill the GPU: each split writes its unnormalised
 // sum with its maximum and its sum of weights, and a last kernel joins them in
 // the order of the splits.  The lengths are on the device, so every CTA works
@@ -36,11 +39,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 16;      // rows of a decoding sequence's tile, and of a joining CTA
 constexpr int kMaxGroup = 16;  // query heads per KV head
 
-// Splitting.  n = the units (of `unit` keys) a sequence's rows see, t = ceil(W /
-// target) units per split (W: the units of all tiles), so a sequence has
-// ceil(n / t) splits.  Tiles with more than one split have n > t, hence there
-// are at most W / t <= target such tiles (Plan::target entries of `groups`)
-// with at most 2 W / t <= 2 target splits (`slots`).
+// Splitting.  n = the units (of `unit` keys) a sequence's rows see, t = ceil(5/4
+// W / target) units per split (W: the units of all tiles; a quarter more than
+// an even share, so that a batch of nearly `target` equal tiles stays whole),
+// so a sequence has ceil(n / t) splits.  Tiles with more than one split have n >
+// t, hence there are at most W / t <= target such tiles (Plan::target entries of
+// `groups`) with at most 2 W / t <= 2 target splits (`slots`).
 struct Plan {
   int tile_rows;  // rows per tile
   int unit;       // keys per unit
@@ -51,7 +55,9 @@ struct Plan {
 constexpr Plan kRowsPlan{kRows, 64, 296, 2};  // two CTAs on each of 148 SMs
 template <int HD>
 constexpr Plan tile_plan() {
-  return HD == 256 ? Plan{128, 64, 148, 8} : Plan{256, 128, 148, 4};  // one CTA per SM
+  return HD == 64    ? Plan{128, 128, 296, 4}  // two CTAs per SM
+         : HD == 128 ? Plan{256, 128, 148, 4}
+                     : Plan{128, 64, 148, 8};
 }
 
 struct Group {  // a split tile, for the joining kernel
@@ -68,6 +74,7 @@ struct Partials {
 struct AttnArgs {
   Batch b;
   int nh, group, window, out_f32;
+  int all_tiles;  // attn_tile_kernel takes the decoding sequences too
   float scale;  // scale * log2 e
   const void* q;
   int64_t q_row, q_head;
@@ -96,7 +103,7 @@ template <bool SMALL>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, const Plan& pl, const Seq& q,
                                             int tpt) {
   SeqWork w{0, 0};
-  if ((q.q_len * a.group <= kRows) != SMALL) return w;
+  if ((!a.all_tiles && q.q_len * a.group <= kRows) != SMALL) return w;
   w.tiles = (q.q_len + tpt - 1) / tpt;
   const int last = q.kv_len - 1;
   if (w.tiles && last >= 0)
@@ -144,7 +151,7 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
 #pragma unroll
   for (int i = 0; i < kW; ++i) w += red[i];
   w *= b.nkv;
-  const unsigned long long t64 = (w + pl.target - 1) / pl.target;
+  const unsigned long long t64 = (w * 5 / 4 + pl.target - 1) / pl.target;
   const int t = (int)(t64 < (unsigned)pl.min_units ? pl.min_units
                       : t64 > (1u << 30)           ? (1u << 30)
                                                    : t64);

@@ -7,12 +7,14 @@
 //   P_w = 2^(S_w scale - m)  a warpgroup per row tile, a thread per row: S from
 //                            TMEM into registers, P back over S as 16-bit pairs
 //   O_w += P_w V             tcgen05.mma, A in TMEM, V as stored (its keys are
-//                            the MMA's K: B is "MN-major")
-// The two row tiles alternate, so the tensor cores work on one while the other
-// is in its softmax.  K and V tiles come by TMA from the pages as stored: a
-// box per page and 64 columns (the 128-byte swizzle), the page number read by
-// a lane of the producer warp; a page that is not needed, or bad, is read as
-// out of range, which TMA fills with zeros.
+//                            the MMA's K: B is "MN-major"), half the keys as soon
+//                            as their P is there
+// The tensor cores work on one row tile while the other is in its softmax: two
+// tiles of one CTA at head_dim 128 (each K and V tile is read once for both),
+// two CTAs of an SM at 64, which also hide each other's start and end.  K and V
+// tiles come by TMA from the pages as stored: a box per page and 64 columns (the
+// 128-byte swizzle), the page number read by a lane of the producer warp; a page
+// that is not needed, or bad, is read as out of range, which TMA fills with zeros.
 //
 // The reference maximum of a row moves only when a score passes the maximum by
 // 2^6 (the weights stay below 2^(kTop + 6)); then the row's warpgroup scales O
@@ -24,7 +26,7 @@
 // are cleared (0 x NaN is NaN), and values that are not finite are cleared and
 // noted: the rows that do see them add them at the end.
 //
-// Warps: 0-3 row tile 0, 4-7 row tile 1 (NT = 2), then a warpgroup with the TMA
+// Warps: a warpgroup per row tile, then one with the TMA
 // producer and the MMA issuer (and two idle warps, so that registers can be
 // shifted to the softmax warpgroups, which hold a row of S).  Every wait is
 // bounded, as in the expert GEMMs.
@@ -37,18 +39,25 @@ namespace {
 
 template <int HD>
 struct Cfg {
-  static constexpr int NT = HD == 256 ? 1 : 2;
-  static constexpr int KT = HD == 256 ? 64 : 128;
+  static constexpr int NT = HD == 128 ? 2 : 1;              // row tiles
+  static constexpr int KT = HD == 256 ? 64 : 128;           // keys per tile
+  static constexpr int kCtas = HD == 64 ? 2 : 1;            // per SM
   static constexpr int kSub = HD / 64;                      // 64-column blocks
   static constexpr int kQBytes = NT * 128 * HD * 2;
   static constexpr int kTileBytes = KT * HD * 2;            // a K or V tile
-  static constexpr int kRing = HD == 64 ? 8 : 5;            // K and V tiles in flight
+  static constexpr int kRing = 5;                           // K and V tiles in flight
   static constexpr int kSoftmax = NT * 128;                 // softmax threads
   static constexpr int kThreads = kSoftmax + 128;
   static constexpr int kBarBytes = 256;
   static constexpr int kSmem = 1024 + kQBytes + kRing * kTileBytes + kBarBytes;
-  static constexpr int kOCol = 256;                         // TMEM: S_0, S_1 below, O_w above
-  static constexpr int kSCol = 128;                         // columns between S_0 and S_1
+  // TMEM columns: S of row tile w at w kSCol, O of row tile w at kOCol + w HD
+  static constexpr int kTmem = 512 / kCtas;
+  static constexpr int kSCol = 128;
+  static constexpr int kOCol = HD == 64 ? 128 : 256;
+  // Registers of the softmax warpgroups and of the other one (0: as launched); their
+  // sum over the CTA's warpgroups is what it is launched with (2 x 128 and 3 x 168).
+  static constexpr int kRegs = HD == 64 ? 200 : HD == 128 ? 216 : 0;
+  [[maybe_unused]] static constexpr int kOtherRegs = HD == 64 ? 56 : 72;
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
@@ -60,16 +69,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// Shared-memory descriptor of an MN-major B matrix (V): 64-element (128-byte
-// swizzled) rows along N, `lbo` bytes between blocks of 64, 8-row groups along
-// K 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lbo) {
-  uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)(lbo >> 4) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
+// Low words of shared-memory descriptors (128-byte swizzle, 8-row groups 1024
+// bytes apart).  K-major (Q, K): rows of 64 elements along the MMA's K.  MN-major
+// (V): rows of 64 elements along N, `lbo` bytes between blocks of 64; the groups
+// of 8 rows lie along the MMA's K.
+__device__ __forceinline__ uint32_t k_major_lo(uint32_t saddr) {
+  return ((saddr & 0x3FFFFu) >> 4) | (1u << 16);
+}
+__device__ __forceinline__ uint32_t mn_major_lo(uint32_t saddr, uint32_t lbo) {
+  return ((saddr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16);
 }
 
 // kind::f16, D = f32, A and B of type T, M = 128, N = n; mn: B is MN-major.
@@ -78,6 +86,22 @@ __device__ __forceinline__ constexpr uint32_t idesc(int n, bool mn) {
   const uint32_t t = Elem<T>::kType == GB_DTYPE_BF16 ? 1u : 0u;
   return (1u << 4) | (t << 7) | (t << 10) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(128 >> 4) << 24);
+}
+
+// The MMA warp runs converged, on values that are the same in every lane (so
+// that descriptors stay in uniform registers: a lone lane in a divergent branch
+// took 60 to 100 clocks per MMA to move them there), and one elected lane issues.
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(kFullMask, v, 0); }
+// A 128-byte-swizzle descriptor from its low word (address and LBO); see sw128_desc.
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
+  constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  return ((uint64_t)hi << 32) | lo;
 }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
@@ -120,6 +144,27 @@ __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// ---- pairs of f32 (one instruction for both) -----------------------------------
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // Element (row, column) of a K or V tile: blocks of 64 columns, 128-byte rows,
 // 16-byte pieces swizzled by the row.
 template <int HD>
@@ -128,14 +173,14 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int piece) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
+__global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
     attn_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a) {
   using C = Cfg<HD>;
   constexpr int KT = C::KT, NT = C::NT;
   constexpr Plan kPlan = tile_plan<HD>();
   extern __shared__ uint8_t smem_raw[];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
   const int tpt = 128 / a.group;  // tokens per row tile
   Item it;
   const bool have = find_item<false, C::kThreads>(a, kPlan, a.tiles, NT * tpt, &it);
@@ -152,8 +197,8 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
   uint64_t* kv_empty = bars + C::kRing;    // [kRing]
   uint64_t* q_full = bars + 2 * C::kRing;
   uint64_t* s_full = q_full + 1;           // [2]
-  uint64_t* p_full = s_full + 2;           // [2]
-  uint64_t* o_done = p_full + 2;           // [2]
+  uint64_t* p_full = s_full + 2;           // [2][2]: row tile, half of the keys
+  uint64_t* o_done = p_full + 4;           // [2]
   uint64_t* v_clean = o_done + 2;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word, err_word, poisoned;
@@ -173,13 +218,16 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
   // a tile with a key that some row does not see
   const int32_t* table = a.b.table + it.seq * a.b.table_stride;
   const int page_size = 1 << a.b.page_shift;
-  // keys of the tile on bad pages, a bit per page of the tile (lane = page)
-  auto bad_pages = [&](int j) -> unsigned {
-    bool bad = false;
+  // Page `lane` of key tile j (a good number where it is not needed), and the
+  // tile's bad pages, a bit each, from those.
+  auto page_of = [&](int j) -> int {
     const int key = j * KT + lane * page_size;
-    if (lane * page_size < KT && key <= last && key + page_size > key_lo)
-      bad = (unsigned)__ldg(table + (key >> a.b.page_shift)) >= (unsigned)a.b.n_pages;
-    return __ballot_sync(kFullMask, bad);
+    return lane * page_size < KT && key <= last && key + page_size > key_lo
+               ? __ldg(table + (key >> a.b.page_shift))
+               : 0;
+  };
+  auto bad_pages = [&](int page) -> unsigned {
+    return __ballot_sync(kFullMask, (unsigned)page >= (unsigned)a.b.n_pages);
   };
   auto edge = [&](int j) { return j * KT + KT - 1 > it.pos0 || j * KT < all_lo; };
 
@@ -191,14 +239,15 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[2 * i], 128);
+      mbar_init(&p_full[2 * i + 1], 128);
       mbar_init(&o_done[i], 1);
     }
     mbar_init(v_clean, C::kSoftmax);
     abort_word = err_word = poisoned = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 0) tmem_alloc(&tmem_slot, 512);
+  if (warp == 0) tmem_alloc(&tmem_slot, C::kTmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -207,9 +256,9 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
     return mbar_wait(bar, parity & 1, abort_flag, &err_word);
   };
 
-  // 384 threads are launched with 168 registers each: 216 + 216 + 72 is that sum.
   if (warp < C::kSoftmax / 32) {
-    if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (C::kRegs != 0)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegs ? C::kRegs : 24));
     // ---------------- softmax: thread = row ---------------------------------------
     const int w = warp >> 2;               // row tile
     const int r = tid & 127;               // row of the tile
@@ -225,8 +274,11 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
     float m = -INFINITY, l = 0.0f;  // reference maximum, sum of weights
     int steps = 0;
     bool ok = true;
+    int page_next = it.u0 < it.u1 ? page_of(it.u0) : 0;
     for (int j = it.u0; j < it.u1 && ok; ++j) {
       const bool at_edge = edge(j);
+      const unsigned bad = bad_pages(page_next);
+      if (j + 1 < it.u1) page_next = page_of(j + 1);  // a step ahead: the load is not waited for
       if (at_edge) {
         // look over this thread's share of the V tile
         const int t = 2 * (j - it.u0) + 1;
@@ -261,7 +313,6 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
         mbar_arrive(v_clean);
       }
       if (!active(w, j)) continue;
-      const unsigned bad = bad_pages(j);
       ok = wait(&s_full[w], steps & 1);
       if (!ok) break;
       tc_fence_after();
@@ -310,24 +361,33 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
         }
       }
       const float ref = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint64_t scale2 = pair(a.scale, a.scale), ref2 = pair(-ref, -ref);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < KT / 2; c += 16) {
-        uint32_t p[16];
+      for (int h = 0; h < 2; ++h) {  // the MMAs of the first half start while the second is computed
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = ex2(__fmaf_rn(s[2 * (c + i)], a.scale, -ref));
-          const float y = ex2(__fmaf_rn(s[2 * (c + i) + 1], a.scale, -ref));
-          sum[(2 * i) & 3] += x;
-          sum[(2 * i + 1) & 3] += y;
-          p[i] = Elem<T>::pack(x, y);
+        for (int c = 0; c < KT / 4; c += 16) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int e = h * (KT / 2) + 2 * (c + i);
+            const uint64_t x = fma2(pair(s[e], s[e + 1]), scale2, ref2);
+            float2 v = unpair(x);
+            v.x = ex2(v.x);
+            v.y = ex2(v.y);
+            sum[i & 1] = add2(sum[i & 1], pair(v.x, v.y));
+            p[i] = Elem<T>::pack(v.x, v.y);
+          }
+          tmem_st16(s_addr + h * (KT / 4) + c, p);
         }
-        tmem_st16(s_addr + c, p);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[2 * w + h]);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_full[w]);
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      {
+        const float2 v = unpair(add2(sum[0], sum[1]));
+        l += v.x + v.y;
+      }
       ++steps;
     }
     // ---- the row's result
@@ -409,7 +469,8 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
       }
     }
   } else {
-    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (C::kRegs != 0)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
     if (warp == C::kSoftmax / 32) {
       // ---------------- TMA producer: Q, then K and V tiles in turn ---------------
       bool ok = true;
@@ -466,79 +527,108 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
       }
     } else if (warp == C::kSoftmax / 32 + 1) {
       // ---------------- MMA issuer -------------------------------------------------
-      if (lane == 0) {
-        bool ok = wait(q_full, 0);
-        // tile t of the ring's order (K of j: 2 (j - u0), V: one more)
-        auto ring_at = [&](int t) { return t % C::kRing; };
-        auto full = [&](int t) { return wait(&kv_full[ring_at(t)], (t / C::kRing) & 1); };
-        uint32_t p_phase[2] = {0, 0}, clean_phase = 0;
-        bool o_any[2] = {false, false};
-        auto issue_s = [&](int w, int j) {
-          const uint32_t q = smem_u32(smem + w * C::kSub * 128 * 128);
-          const uint32_t k = smem_u32(ring + ring_at(2 * (j - it.u0)) * C::kTileBytes);
+      auto all_wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(kFullMask, wait(bar, parity)) != 0;
+      };
+      const int u0 = uniform(it.u0), n = uniform(it.u1) - u0;
+      const int act0 = uniform(hi0) - u0;                            // row tile 0: j < act0
+      const int act1 = uniform(n1 > 0 ? lo1 - it.u0 : 0x7fffffff);   // row tile 1: j >= act1
+      // edge tiles: those from edge_hi on, and those before edge_lo
+      const int edge_hi = uniform((it.pos0 + 1) / KT) - u0;
+      const int edge_lo = uniform((all_lo + KT - 1) / KT) - u0;
+      const uint32_t t_base = (uint32_t)uniform((int)tmem);
+      const uint32_t q_lo = k_major_lo(smem_u32(smem)), ring_base = smem_u32(ring);
+      auto on = [&](int w, int j) { return w == 0 ? j < act0 : j >= act1; };
+      auto at_edge = [&](int j) { return j >= edge_hi || j < edge_lo; };
+      bool ok = all_wait(q_full, 0);
+      // Ring tile t (K of key tile j: 2 j, V: 2 j + 1) is in slot t % kRing, of phase t / kRing:
+      // next_k / next_v are the slots of K of j + 1 and of V of j.
+      int k_slot = 0, v_slot = 1;
+      uint32_t k_phase = 0, v_phase = 0;
+      auto advance = [&](int& slot, uint32_t& phase) {
+        slot += 2;
+        if (slot >= C::kRing) {
+          slot -= C::kRing;
+          phase ^= 1;
+        }
+      };
+      uint32_t p_phase0 = 0, p_phase1 = 0, clean_phase = 0;
+      bool any0 = false, any1 = false;
+      auto issue_s = [&](int w, uint32_t k_lo) {
+        const uint32_t d = t_base + w * C::kSCol, q = q_lo + w * (C::kSub * 128 * 128 >> 4);
+        if (elect()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
-            mma_ss(tmem + w * C::kSCol, sw128_desc(q + (kk >> 2) * 128 * 128 + (kk & 3) * 32),
-                   sw128_desc(k + (kk >> 2) * KT * 128 + (kk & 3) * 32), idesc<T>(KT, false), kk != 0);
+            mma_ss(d, desc_of(q + (((kk >> 2) * 128 * 128 + (kk & 3) * 32) >> 4)),
+                   desc_of(k_lo + (((kk >> 2) * KT * 128 + (kk & 3) * 32) >> 4)), idesc<T>(KT, false),
+                   kk != 0);
           mma_commit(&s_full[w]);
-        };
-        if (ok && it.u0 < it.u1) {
-          ok = full(0);
-          tc_fence_after();
-          if (ok) {
-            for (int w = 0; w < NT; ++w)
-              if (active(w, it.u0)) issue_s(w, it.u0);
-            mma_commit(&kv_empty[ring_at(0)]);
-          }
         }
-        for (int j = it.u0; j < it.u1 && ok; ++j) {
-          const int tk = 2 * (j - it.u0);
-          bool v_ready = false, k_ready = false;
-          for (int w = 0; w < NT && ok; ++w) {
-            if (active(w, j)) {
-              if (!v_ready) {
-                ok = full(tk + 1);
-                if (ok && edge(j)) ok = wait(v_clean, clean_phase);
-                v_ready = true;
-              }
-              ok = ok && wait(&p_full[w], p_phase[w]);
-              if (!ok) break;
-              p_phase[w] ^= 1;
-              tc_fence_after();
-              const uint32_t v = smem_u32(ring + ring_at(tk + 1) * C::kTileBytes);
+        __syncwarp();
+      };
+      if (ok && n > 0) {
+        ok = all_wait(&kv_full[0], 0);
+        tc_fence_after();
+        if (ok) {
+          const uint32_t k_lo = k_major_lo(ring_base);
+          for (int w = 0; w < NT; ++w)
+            if (on(w, 0)) issue_s(w, k_lo);
+          if (elect()) mma_commit(&kv_empty[0]);
+          advance(k_slot, k_phase);
+        }
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        // K of j + 1 and V of j: both before the first MMA that needs either
+        const bool more = j + 1 < n;
+        ok = all_wait(&kv_full[v_slot], v_phase);
+        if (ok && at_edge(j)) {
+          ok = all_wait(v_clean, clean_phase);
+          clean_phase ^= 1;
+        }
+        if (ok && more) ok = all_wait(&kv_full[k_slot], k_phase);
+        if (!ok) break;
+        const uint32_t v_lo = mn_major_lo(ring_base + v_slot * C::kTileBytes, KT * 128);
+        const uint32_t k_lo = k_major_lo(ring_base + k_slot * C::kTileBytes);
 #pragma unroll
-              for (int kk = 0; kk < KT / 16; ++kk)
-                mma_ts(tmem + C::kOCol + w * HD, tmem + w * C::kSCol + kk * 8,
-                       sw128_mn_desc(v + kk * 2048, KT * 128), idesc<T>(HD, true),
-                       o_any[w] || kk != 0);
-              o_any[w] = true;
-              mma_commit(&o_done[w]);
-            }
-            if (j + 1 < it.u1 && active(w, j + 1)) {
-              if (!k_ready) {
-                ok = full(tk + 2);
-                tc_fence_after();
-                k_ready = true;
+        for (int w = 0; w < NT; ++w) {
+          if (on(w, j)) {
+            bool& any = w ? any1 : any0;
+            uint32_t& phase = w ? p_phase1 : p_phase0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              ok = ok && all_wait(&p_full[2 * w + h], phase);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t first = any ? 1u : 0u;
+              if (elect()) {
+#pragma unroll
+                for (int kk = 0; kk < KT / 32; ++kk) {
+                  const int k = h * (KT / 32) + kk;
+                  mma_ts(t_base + C::kOCol + w * HD, t_base + w * C::kSCol + k * 8,
+                         desc_of(v_lo + k * (2048 >> 4)), idesc<T>(HD, true), k != 0 ? 1u : first);
+                }
+                if (h == 1) mma_commit(&o_done[w]);
               }
-              if (ok) issue_s(w, j + 1);
+              __syncwarp();
             }
+            if (!ok) break;
+            phase ^= 1;
+            any = true;
           }
-          if (!ok) break;
-          if (!v_ready) {  // neither row tile sees it (the window between them): still in order
-            ok = full(tk + 1);
-            if (ok && edge(j)) ok = wait(v_clean, clean_phase);
-          }
-          if (edge(j)) clean_phase ^= 1;
-          if (ok) mma_commit(&kv_empty[ring_at(tk + 1)]);
-          if (j + 1 < it.u1) {
-            if (ok && !k_ready) ok = full(tk + 2);
-            if (ok) mma_commit(&kv_empty[ring_at(tk + 2)]);
-          }
+          if (more && on(w, j + 1)) issue_s(w, k_lo);
         }
-        if (!ok) {  // issued MMAs read shared memory and TMEM: let them finish
-          const uint64_t t0 = globaltimer();
-          while (globaltimer() - t0 < 2000000ull) {
-          }
+        if (!ok) break;
+        if (elect()) {
+          mma_commit(&kv_empty[v_slot]);
+          if (more) mma_commit(&kv_empty[k_slot]);
+        }
+        __syncwarp();
+        advance(v_slot, v_phase);
+        advance(k_slot, k_phase);
+      }
+      if (!ok) {  // issued MMAs read shared memory and TMEM: let them finish
+        const uint64_t t0 = globaltimer();
+        while (globaltimer() - t0 < 2000000ull) {
         }
       }
     }
@@ -546,7 +636,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) tmem_dealloc(tmem, 512);
+  if (warp == 0) tmem_dealloc(tmem, C::kTmem);
   if (tid == 0 && *abort_flag) flag(a.b, GB_PAGED_TIMEOUT);
   pdl_wait();
 }
