@@ -55,7 +55,7 @@ struct Plan {
 constexpr Plan kRowsPlan{kRows, 64, 296, 2};  // two CTAs on each of 148 SMs
 template <int HD>
 constexpr Plan tile_plan() {
-  return HD == 64    ? Plan{128, 128, 296, 4}  // two CTAs per SM
+  return HD == 64    ? Plan{128, 64, 296, 8}  // two CTAs per SM
          : HD == 128 ? Plan{256, 128, 148, 4}
                      : Plan{128, 64, 148, 8};
 }

@@ -7,11 +7,12 @@
 //   P_w = 2^(S_w scale - m)  a warpgroup per row tile, a thread per row: S from
 //                            TMEM into registers, P back over S as 16-bit pairs
 //   O_w += P_w V             tcgen05.mma, A in TMEM, V as stored (its keys are
-//                            the MMA's K: B is "MN-major"), half the keys as soon
-//                            as their P is there
-// The tensor cores work on one row tile while the other is in its softmax: two
-// tiles of one CTA at head_dim 128 (each K and V tile is read once for both),
-// two CTAs of an SM at 64, which also hide each other's start and end.  K and V
+//                            the MMA's K: B is "MN-major")
+// The tensor cores work on one row tile while another is in its softmax: two
+// tiles of one CTA at head_dim 128 (each K and V tile is read once for both), two
+// CTAs of an SM at 64, which also hide each other's start and end.  Where TMEM
+// has room (64 and 256), S has two buffers, so that the next tile's S is there
+// when a softmax ends.  K and V
 // tiles come by TMA from the pages as stored: a box per page and 64 columns (the
 // 128-byte swizzle), the page number read by a lane of the producer warp; a page
 // that is not needed, or bad, is read as out of range, which TMA fills with zeros.
@@ -26,10 +27,8 @@
 // are cleared (0 x NaN is NaN), and values that are not finite are cleared and
 // noted: the rows that do see them add them at the end.
 //
-// Warps: a warpgroup per row tile, then one with the TMA
-// producer and the MMA issuer (and two idle warps, so that registers can be
-// shifted to the softmax warpgroups, which hold a row of S).  Every wait is
-// bounded, as in the expert GEMMs.
+// Warps: four per row tile, then the TMA producer and the MMA issuer.  Every wait
+// is bounded, as in the expert GEMMs.
 #include "paged_attn.cuh"
 #include "umma.cuh"
 
@@ -39,25 +38,26 @@ namespace {
 
 template <int HD>
 struct Cfg {
-  static constexpr int NT = HD == 128 ? 2 : 1;              // row tiles
-  static constexpr int KT = HD == 256 ? 64 : 128;           // keys per tile
-  static constexpr int kCtas = HD == 64 ? 2 : 1;            // per SM
-  static constexpr int kSub = HD / 64;                      // 64-column blocks
+  static constexpr int NT = HD == 128 ? 2 : 1;            // row tiles
+  static constexpr int KT = HD == 128 ? 128 : 64;         // keys per tile
+  static constexpr int kBufs = HD == 128 ? 1 : 2;         // S buffers per row tile
+  static constexpr int kCtas = HD == 64 ? 2 : 1;          // per SM
+  static constexpr int kSub = HD / 64;                    // 64-column blocks
   static constexpr int kQBytes = NT * 128 * HD * 2;
-  static constexpr int kTileBytes = KT * HD * 2;            // a K or V tile
-  static constexpr int kRing = 5;                           // K and V tiles in flight
-  static constexpr int kSoftmax = NT * 128;                 // softmax threads
-  static constexpr int kThreads = kSoftmax + 128;
-  static constexpr int kBarBytes = 256;
+  static constexpr int kTileBytes = KT * HD * 2;          // a K or V tile
+  static constexpr int kRing = HD == 64 ? 9 : HD == 128 ? 4 : 5;  // K and V tiles in flight
+  static constexpr int kSoftmax = NT * 128;               // softmax threads
+  // head_dim 128 holds 128 scores per thread: its softmax warps take registers
+  // from the other warpgroup, which two idle warps fill (3 x 168 = 2 x 216 + 72).
+  static constexpr bool kShift = HD == 128;
+  static constexpr int kThreads = kSoftmax + (kShift ? 128 : 64);
+  static constexpr int kBarBytes = 512;
   static constexpr int kSmem = 1024 + kQBytes + kRing * kTileBytes + kBarBytes;
-  // TMEM columns: S of row tile w at w kSCol, O of row tile w at kOCol + w HD
+  // TMEM columns: S of row tile w, buffer b at (w kBufs + b) KT; O at kOCol + w HD
   static constexpr int kTmem = 512 / kCtas;
-  static constexpr int kSCol = 128;
-  static constexpr int kOCol = HD == 64 ? 128 : 256;
-  // Registers of the softmax warpgroups and of the other one (0: as launched); their
-  // sum over the CTA's warpgroups is what it is launched with (2 x 128 and 3 x 168).
-  static constexpr int kRegs = HD == 64 ? 200 : HD == 128 ? 216 : 0;
-  [[maybe_unused]] static constexpr int kOtherRegs = HD == 64 ? 56 : 72;
+  static constexpr int kOCol = NT * kBufs * KT;
+  static_assert(kOCol + NT * HD <= kTmem && kCtas * kTmem <= 512, "S and O in TMEM");
+  static_assert((2 * kRing + 1 + 8 * NT) * 8 <= kBarBytes, "barriers");
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
@@ -177,7 +177,10 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
     attn_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a) {
   using C = Cfg<HD>;
-  constexpr int KT = C::KT, NT = C::NT;
+  constexpr int NT = C::NT, KT = C::KT, kBufs = C::kBufs;
+  // the buffer of a row tile's step, and the phase of its barriers
+  auto buf_of = [](int w, int step) { return w * kBufs + (kBufs == 2 ? step & 1 : 0); };
+  auto phase_of = [](int step) { return kBufs == 2 ? step >> 1 : step; };
   constexpr Plan kPlan = tile_plan<HD>();
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
@@ -196,12 +199,12 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
   uint64_t* kv_full = bars;                // [kRing]
   uint64_t* kv_empty = bars + C::kRing;    // [kRing]
   uint64_t* q_full = bars + 2 * C::kRing;
-  uint64_t* s_full = q_full + 1;           // [2]
-  uint64_t* p_full = s_full + 2;           // [2][2]: row tile, half of the keys
-  uint64_t* o_done = p_full + 4;           // [2]
-  uint64_t* v_clean = o_done + 2;
+  uint64_t* s_full = q_full + 1;           // [2 NT]: row tile and buffer
+  uint64_t* p_full = s_full + 2 * NT;      // [2 NT]
+  uint64_t* o_done = p_full + 2 * NT;      // [2 NT]: the PVs of a row tile in turn
+  uint64_t* v_clean = o_done + 2 * NT;     // [2 NT]: a row tile's edge tiles in turn
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word, err_word, poisoned;
+  __shared__ int abort_word, err_word, poisoned, any_bad;
   volatile int* abort_flag = &abort_word;
 
   // The tiles: row tile w has tokens [w tpt, w tpt + n_w); key tiles [u0, u1).
@@ -218,16 +221,13 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
   // a tile with a key that some row does not see
   const int32_t* table = a.b.table + it.seq * a.b.table_stride;
   const int page_size = 1 << a.b.page_shift;
-  // Page `lane` of key tile j (a good number where it is not needed), and the
-  // tile's bad pages, a bit each, from those.
-  auto page_of = [&](int j) -> int {
+  // keys of the tile on bad pages, a bit per page of the tile (lane = page)
+  auto bad_pages = [&](int j) -> unsigned {
+    bool bad = false;
     const int key = j * KT + lane * page_size;
-    return lane * page_size < KT && key <= last && key + page_size > key_lo
-               ? __ldg(table + (key >> a.b.page_shift))
-               : 0;
-  };
-  auto bad_pages = [&](int page) -> unsigned {
-    return __ballot_sync(kFullMask, (unsigned)page >= (unsigned)a.b.n_pages);
+    if (lane * page_size < KT && key <= last && key + page_size > key_lo)
+      bad = (unsigned)__ldg(table + (key >> a.b.page_shift)) >= (unsigned)a.b.n_pages;
+    return __ballot_sync(kFullMask, bad);
   };
   auto edge = [&](int j) { return j * KT + KT - 1 > it.pos0 || j * KT < all_lo; };
 
@@ -237,14 +237,13 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
       mbar_init(&kv_empty[i], 1);
     }
     mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2 * NT; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[2 * i], 128);
-      mbar_init(&p_full[2 * i + 1], 128);
+      mbar_init(&p_full[i], 128);
       mbar_init(&o_done[i], 1);
+      mbar_init(&v_clean[i], 128);
     }
-    mbar_init(v_clean, C::kSoftmax);
-    abort_word = err_word = poisoned = 0;
+    abort_word = err_word = poisoned = any_bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tmem_alloc(&tmem_slot, C::kTmem);
@@ -257,8 +256,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
   };
 
   if (warp < C::kSoftmax / 32) {
-    if constexpr (C::kRegs != 0)
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegs ? C::kRegs : 24));
+    if constexpr (C::kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------- softmax: thread = row ---------------------------------------
     const int w = warp >> 2;               // row tile
     const int r = tid & 127;               // row of the tile
@@ -268,26 +266,33 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
     const int pos = live ? it.pos0 + w * tpt + tok : -1;
     const int first = live && a.window > 0 ? max(0, pos - a.window + 1) : 0;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + w * C::kSCol + lane_base;
     const uint32_t o_addr = tmem + C::kOCol + w * HD + lane_base;
     constexpr float kTop = Elem<T>::kTop;
+    // PV of the row tile's step n done.  A parity tells a phase only from its
+    // neighbours: S of a step comes after PV of the step two before, so with two
+    // barriers in turn the phase before n's is always complete.
+    auto wait_o = [&](int n) { return wait(&o_done[2 * w + (n & 1)], n >> 1); };
     float m = -INFINITY, l = 0.0f;  // reference maximum, sum of weights
-    int steps = 0;
+    int steps = 0, edges = 0;
     bool ok = true;
-    int page_next = it.u0 < it.u1 ? page_of(it.u0) : 0;
     for (int j = it.u0; j < it.u1 && ok; ++j) {
       const bool at_edge = edge(j);
-      const unsigned bad = bad_pages(page_next);
-      if (j + 1 < it.u1) page_next = page_of(j + 1);  // a step ahead: the load is not waited for
+      if (!active(w, j)) continue;
+      const int buf = buf_of(w, steps);
+      const uint32_t s_addr = tmem + buf * KT + lane_base;
+      ok = wait(&s_full[buf], phase_of(steps));
+      if (!ok) break;
       if (at_edge) {
-        // look over this thread's share of the V tile
+        // Look over this thread's share of the V tile (S of the tile is there, so the
+        // ring is at most at this V).
         const int t = 2 * (j - it.u0) + 1;
         ok = wait(&kv_full[t % C::kRing], (t / C::kRing) & 1);
         if (!ok) break;
         uint8_t* v = ring + (t % C::kRing) * C::kTileBytes;
         constexpr int kPieces = HD / 8;
         bool found = false;
-        for (int i = tid; i < KT * kPieces; i += C::kSoftmax) {
+        const bool both = NT == 2 && active(w ^ 1, j);
+        for (int i = both ? tid : r; i < KT * kPieces; i += both ? 256 : 128) {
           const int row = i / kPieces, key = j * KT + row;
           uint4* p = reinterpret_cast<uint4*>(v + tile_offset<HD>(row, i % kPieces));
           if (key > last || key < key_lo) {
@@ -310,12 +315,11 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
         }
         if (found) *(volatile int*)&poisoned = 1;
         fence_proxy_async_smem();
-        mbar_arrive(v_clean);
+        mbar_arrive(&v_clean[2 * w + (edges++ & 1)]);
       }
-      if (!active(w, j)) continue;
-      ok = wait(&s_full[w], steps & 1);
-      if (!ok) break;
       tc_fence_after();
+      // set by the producer before the tile that S is of was copied
+      const unsigned bad = *(volatile int*)&any_bad ? bad_pages(j) : 0;
       uint32_t sb[KT];
 #pragma unroll
       for (int c = 0; c < KT; c += 32) tmem_ld32(s_addr + c, sb + c);
@@ -344,8 +348,8 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
         const float f = nm == -INFINITY ? 1.0f : ex2(m - nm);
         m = nm;
         l *= f;
-        if (steps) {  // O is this row tile's, all its MMAs done
-          ok = wait(&o_done[w], (steps - 1) & 1);
+        if (steps) {  // after the last MMAs into this O
+          ok = wait_o(steps - 1);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
@@ -364,26 +368,22 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
       const uint64_t scale2 = pair(a.scale, a.scale), ref2 = pair(-ref, -ref);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {  // the MMAs of the first half start while the second is computed
+      for (int c = 0; c < KT / 2; c += 16) {
+        uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < KT / 4; c += 16) {
-          uint32_t p[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int e = h * (KT / 2) + 2 * (c + i);
-            const uint64_t x = fma2(pair(s[e], s[e + 1]), scale2, ref2);
-            float2 v = unpair(x);
-            v.x = ex2(v.x);
-            v.y = ex2(v.y);
-            sum[i & 1] = add2(sum[i & 1], pair(v.x, v.y));
-            p[i] = Elem<T>::pack(v.x, v.y);
-          }
-          tmem_st16(s_addr + h * (KT / 4) + c, p);
+        for (int i = 0; i < 16; ++i) {
+          const int e = 2 * (c + i);
+          float2 v = unpair(fma2(pair(s[e], s[e + 1]), scale2, ref2));
+          v.x = ex2(v.x);
+          v.y = ex2(v.y);
+          sum[i & 1] = add2(sum[i & 1], pair(v.x, v.y));
+          p[i] = Elem<T>::pack(v.x, v.y);
         }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&p_full[2 * w + h]);
+        tmem_st16(s_addr + c, p);
       }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[buf]);
       {
         const float2 v = unpair(add2(sum[0], sum[1]));
         l += v.x + v.y;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
     }
     // ---- the row's result
     if (ok && steps) {
-      ok = wait(&o_done[w], (steps - 1) & 1);
+      ok = wait_o(steps - 1);
       tc_fence_after();
     }
     if (!*abort_flag && ok && (w == 0 || n1 > 0)) {
@@ -469,8 +469,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
       }
     }
   } else {
-    if constexpr (C::kRegs != 0)
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+    if constexpr (C::kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == C::kSoftmax / 32) {
       // ---------------- TMA producer: Q, then K and V tiles in turn ---------------
       bool ok = true;
@@ -495,10 +494,12 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
           in_page = key & (page_size - 1);
           if (lane < boxes && key <= last && key + box > key_lo) {
             const int p = __ldg(table + (key >> a.b.page_shift));
-            if ((unsigned)p < (unsigned)a.b.n_pages)
+            if ((unsigned)p < (unsigned)a.b.n_pages) {
               page = p;
-            else
+            } else {
+              *(volatile int*)&any_bad = 1;
               flag(a.b, GB_PAGED_BAD_PAGE);
+            }
           }
         }
         for (int kv = 0; kv < 2 && ok; ++kv) {
@@ -541,8 +542,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
       auto on = [&](int w, int j) { return w == 0 ? j < act0 : j >= act1; };
       auto at_edge = [&](int j) { return j >= edge_hi || j < edge_lo; };
       bool ok = all_wait(q_full, 0);
-      // Ring tile t (K of key tile j: 2 j, V: 2 j + 1) is in slot t % kRing, of phase t / kRing:
-      // next_k / next_v are the slots of K of j + 1 and of V of j.
+      // Ring tile t (K of key tile j: 2 j, V: 2 j + 1) is in slot t % kRing, of phase t / kRing.
       int k_slot = 0, v_slot = 1;
       uint32_t k_phase = 0, v_phase = 0;
       auto advance = [&](int& slot, uint32_t& phase) {
@@ -552,79 +552,85 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
           phase ^= 1;
         }
       };
-      uint32_t p_phase0 = 0, p_phase1 = 0, clean_phase = 0;
-      bool any0 = false, any1 = false;
+      int edges[2] = {0, 0};
+      int s_steps[2] = {0, 0}, p_steps[2] = {0, 0};  // S issued, P taken, per row tile
       auto issue_s = [&](int w, uint32_t k_lo) {
-        const uint32_t d = t_base + w * C::kSCol, q = q_lo + w * (C::kSub * 128 * 128 >> 4);
+        const int buf = buf_of(w, s_steps[w]++);
+        const uint32_t d = t_base + buf * KT, q = q_lo + w * (C::kSub * 128 * 128 >> 4);
         if (elect()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
             mma_ss(d, desc_of(q + (((kk >> 2) * 128 * 128 + (kk & 3) * 32) >> 4)),
                    desc_of(k_lo + (((kk >> 2) * KT * 128 + (kk & 3) * 32) >> 4)), idesc<T>(KT, false),
                    kk != 0);
-          mma_commit(&s_full[w]);
+          mma_commit(&s_full[buf]);
         }
         __syncwarp();
       };
-      if (ok && n > 0) {
-        ok = all_wait(&kv_full[0], 0);
+      auto issue_pv = [&](int w, uint32_t v_lo) -> bool {
+        const int step = p_steps[w]++, buf = buf_of(w, step);
+        if (!all_wait(&p_full[buf], phase_of(step))) return false;
         tc_fence_after();
-        if (ok) {
-          const uint32_t k_lo = k_major_lo(ring_base);
-          for (int w = 0; w < NT; ++w)
-            if (on(w, 0)) issue_s(w, k_lo);
-          if (elect()) mma_commit(&kv_empty[0]);
-          advance(k_slot, k_phase);
-        }
-      }
-      for (int j = 0; j < n && ok; ++j) {
-        // K of j + 1 and V of j: both before the first MMA that needs either
-        const bool more = j + 1 < n;
-        ok = all_wait(&kv_full[v_slot], v_phase);
-        if (ok && at_edge(j)) {
-          ok = all_wait(v_clean, clean_phase);
-          clean_phase ^= 1;
-        }
-        if (ok && more) ok = all_wait(&kv_full[k_slot], k_phase);
-        if (!ok) break;
-        const uint32_t v_lo = mn_major_lo(ring_base + v_slot * C::kTileBytes, KT * 128);
-        const uint32_t k_lo = k_major_lo(ring_base + k_slot * C::kTileBytes);
-#pragma unroll
-        for (int w = 0; w < NT; ++w) {
-          if (on(w, j)) {
-            bool& any = w ? any1 : any0;
-            uint32_t& phase = w ? p_phase1 : p_phase0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              ok = ok && all_wait(&p_full[2 * w + h], phase);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t first = any ? 1u : 0u;
-              if (elect()) {
-#pragma unroll
-                for (int kk = 0; kk < KT / 32; ++kk) {
-                  const int k = h * (KT / 32) + kk;
-                  mma_ts(t_base + C::kOCol + w * HD, t_base + w * C::kSCol + k * 8,
-                         desc_of(v_lo + k * (2048 >> 4)), idesc<T>(HD, true), k != 0 ? 1u : first);
-                }
-                if (h == 1) mma_commit(&o_done[w]);
-              }
-              __syncwarp();
-            }
-            if (!ok) break;
-            phase ^= 1;
-            any = true;
-          }
-          if (more && on(w, j + 1)) issue_s(w, k_lo);
-        }
-        if (!ok) break;
+        const uint32_t first = step ? 1u : 0u;
         if (elect()) {
-          mma_commit(&kv_empty[v_slot]);
-          if (more) mma_commit(&kv_empty[k_slot]);
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; ++kk)
+            mma_ts(t_base + C::kOCol + w * HD, t_base + buf * KT + kk * 8,
+                   desc_of(v_lo + kk * (2048 >> 4)), idesc<T>(HD, true), kk != 0 ? 1u : first);
+          mma_commit(&o_done[2 * w + (step & 1)]);
         }
         __syncwarp();
-        advance(v_slot, v_phase);
-        advance(k_slot, k_phase);
+        return true;
+      };
+      auto free_slot = [&](int& slot, uint32_t& phase) {  // once the MMAs issued so far are done
+        if (elect()) mma_commit(&kv_empty[slot]);
+        __syncwarp();
+        advance(slot, phase);
+      };
+      auto k_tile = [&](uint32_t* k_lo) -> bool {
+        if (!all_wait(&kv_full[k_slot], k_phase)) return false;
+        tc_fence_after();
+        *k_lo = k_major_lo(ring_base + k_slot * C::kTileBytes);
+        return true;
+      };
+      uint32_t k_lo = 0;
+      if (ok && n > 0 && (ok = k_tile(&k_lo))) {
+#pragma unroll
+        for (int w = 0; w < NT; ++w)
+          if (on(w, 0)) issue_s(w, k_lo);
+        free_slot(k_slot, k_phase);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const bool more = j + 1 < n;
+        ok = all_wait(&kv_full[v_slot], v_phase);
+        if (at_edge(j)) {
+#pragma unroll
+          for (int w = 0; w < NT; ++w)
+            if (on(w, j)) {
+              ok = ok && all_wait(&v_clean[2 * w + (edges[w] & 1)], edges[w] >> 1);
+              ++edges[w];
+            }
+        }
+        ok = ok && (!more || k_tile(&k_lo));
+        if (!ok) break;
+        const uint32_t v_lo = mn_major_lo(ring_base + v_slot * C::kTileBytes, KT * 128);
+        // With two buffers the next S goes before this P V: its buffer's last reader, PV
+        // of j - 1, is issued.  (Never before v_clean of j: a row tile's softmax cannot
+        // then reach edge tile j + 2 before that phase is seen.)  With one buffer, after.
+        if (kBufs == 2 && more) {
+#pragma unroll
+          for (int w = 0; w < NT; ++w)
+            if (on(w, j + 1)) issue_s(w, k_lo);
+          free_slot(k_slot, k_phase);
+        }
+#pragma unroll
+        for (int w = 0; w < NT; ++w) {
+          if (on(w, j)) ok = ok && issue_pv(w, v_lo);
+          if (kBufs == 1 && more && on(w, j + 1) && ok) issue_s(w, k_lo);
+        }
+        if (!ok) break;
+        free_slot(v_slot, v_phase);
+        if (kBufs == 1 && more) free_slot(k_slot, k_phase);
       }
       if (!ok) {  // issued MMAs read shared memory and TMEM: let them finish
         const uint64_t t0 = globaltimer();
