@@ -121,19 +121,122 @@ __device__ __forceinline__ V warp_inclusive(V v) {
   return v;
 }
 
+// Units per split (see Plan): the same in every CTA.
+__device__ __forceinline__ int split_units(const AttnArgs& a, const Plan& pl, unsigned long long w) {
+  const double t = ceil((double)w * a.b.nkv * (1.25 / pl.target));
+  return max(pl.min_units, (int)fmin(t, 1073741824.0));
+}
+
+// Item `j` (of its sequence) of sequence s with `splits` splits per tile; first_group,
+// first_slot: the split tiles and their splits of the sequences before.
+__device__ __forceinline__ Item make_item(const AttnArgs& a, const Plan& pl, const Partials& part,
+                                          int tpt, int s, const Seq& q, const SeqWork& x, int splits,
+                                          uint32_t j, uint32_t first_group, uint32_t first_slot,
+                                          bool write_group) {
+  Item it;
+  it.seq = s;
+  const uint32_t js = j / (uint32_t)a.b.nkv;
+  it.g = (int)(j - js * (uint32_t)a.b.nkv);
+  // the last tile, which sees most keys, first
+  const uint32_t back = js / (uint32_t)splits;
+  const int split = (int)(js - back * (uint32_t)splits), tile = x.tiles - 1 - (int)back;
+  it.row0 = q.row0 + tile * tpt;
+  it.tokens = min(tpt, q.q_len - tile * tpt);
+  it.pos0 = q.kv_len - q.q_len + tile * tpt;
+  const int last = it.pos0 + it.tokens - 1;
+  const int lo = first_unit(it.pos0, a.window, pl.unit);
+  const int n = last < 0 ? 0 : last / pl.unit - lo + 1;
+  const int per = (n + splits - 1) / splits;
+  it.u0 = lo + min(split * per, n);
+  it.u1 = lo + min((split + 1) * per, n);
+  it.slot = -1;
+  if (splits > 1) {
+    const int nth = tile * a.b.nkv + it.g;
+    const int slot0 = (int)first_slot + nth * splits;
+    it.slot = slot0 + split;
+    if (split == 0 && write_group)
+      part.groups[first_group + nth] = Group{it.row0, it.tokens * a.group, it.g, slot0, splits};
+  }
+  return it;
+}
+
 // Finds the CTA's item among the sequences of one kind (SMALL: at most kRows
-// rows); false: there is none.  Called by the first THREADS threads of the CTA
-// with `bar` a barrier over them.  tpt: tokens per tile.
+// rows); false: there is none.  Called by the whole CTA of THREADS threads; tpt:
+// tokens per tile.  Up to 128 sequences every warp works it out for itself, four
+// sequences a lane, without a barrier; more take the whole CTA.
 template <bool SMALL, int THREADS>
 __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& part, int tpt,
                           Item* out) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Batch& b = a.b;
+  if (b.n_seqs <= 128) {
+    Seq q[4];
+    SeqWork x[4];
+    unsigned long long w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q[i] = Seq{0, 0, 0};
+      const int s = 4 * lane + i;
+      if (s < b.n_seqs) q[i] = load_seq(b, s, blockIdx.x == 0 && warp == 0);
+      x[i] = seq_work<SMALL>(a, pl, q[i], tpt);
+      w += (unsigned long long)x[i].tiles * x[i].units;
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) w += __shfl_xor_sync(kFullMask, w, o);
+    const int t = split_units(a, pl, w);
+    uint32_t items[4], mine = 0, mine_groups = 0, mine_slots = 0;
+    int splits[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      splits[i] = x[i].units > t ? (x[i].units + t - 1) / t : 1;
+      items[i] = (uint32_t)x[i].tiles * b.nkv * splits[i];
+      mine += items[i];
+      if (splits[i] > 1) {
+        mine_groups += (uint32_t)x[i].tiles * b.nkv;
+        mine_slots += items[i];
+      }
+    }
+    uint32_t before = warp_inclusive(mine) - mine, groups = 0, slots = 0, all_groups = 0;
+    if (__any_sync(kFullMask, mine_slots)) {  // the same in every warp
+      groups = warp_inclusive(mine_groups);
+      all_groups = __shfl_sync(kFullMask, groups, 31);
+      groups -= mine_groups;
+      slots = warp_inclusive(mine_slots) - mine_slots;
+    }
+    if (blockIdx.x == 0 && tid == 0) *part.n_groups = (int)all_groups;
+    Item it{};
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (blockIdx.x >= before && blockIdx.x - before < items[i]) {
+        it = make_item(a, pl, part, tpt, 4 * lane + i, q[i], x[i], splits[i], blockIdx.x - before,
+                       groups, slots, warp == 0);
+        found = true;
+      }
+      before += items[i];
+      if (splits[i] > 1) {
+        groups += (uint32_t)x[i].tiles * b.nkv;
+        slots += items[i];
+      }
+    }
+    const unsigned m = __ballot_sync(kFullMask, found);
+    if (!m) return false;
+    const int src = __ffs(m) - 1;
+    out->seq = __shfl_sync(kFullMask, it.seq, src);
+    out->row0 = __shfl_sync(kFullMask, it.row0, src);
+    out->tokens = __shfl_sync(kFullMask, it.tokens, src);
+    out->pos0 = __shfl_sync(kFullMask, it.pos0, src);
+    out->g = __shfl_sync(kFullMask, it.g, src);
+    out->u0 = __shfl_sync(kFullMask, it.u0, src);
+    out->u1 = __shfl_sync(kFullMask, it.u1, src);
+    out->slot = __shfl_sync(kFullMask, it.slot, src);
+    return true;
+  }
   constexpr int kW = THREADS / 32;
   __shared__ unsigned long long red[kW];
   __shared__ unsigned long long run[kW][2];
   __shared__ Item found;
   __shared__ int have;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Batch& b = a.b;
   Seq mine{0, 0, 0};  // of the first THREADS sequences
   unsigned long long w = 0;
   for (int s = tid; s < b.n_seqs; s += THREADS) {
@@ -150,11 +253,7 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
   w = 0;
 #pragma unroll
   for (int i = 0; i < kW; ++i) w += red[i];
-  w *= b.nkv;
-  const unsigned long long t64 = (w * 5 / 4 + pl.target - 1) / pl.target;
-  const int t = (int)(t64 < (unsigned)pl.min_units ? pl.min_units
-                      : t64 > (1u << 30)           ? (1u << 30)
-                                                   : t64);
+  const int t = split_units(a, pl, w);
   // prefixes over the sequences: items; splits (high half) and tiles of split sequences
   unsigned long long base_items = 0, base_groups = 0;
   for (int s0 = 0; s0 < b.n_seqs; s0 += THREADS) {
@@ -162,7 +261,7 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
     Seq q{0, 0, 0};
     if (s < b.n_seqs) q = s0 ? load_seq(b, s, false) : mine;
     const SeqWork x = seq_work<SMALL>(a, pl, q, tpt);
-    const int splits = max(1, (x.units + t - 1) / t);
+    const int splits = x.units > t ? (x.units + t - 1) / t : 1;
     const unsigned long long tiles = (unsigned long long)x.tiles * b.nkv;
     const unsigned long long items = tiles * splits;
     const unsigned long long groups = splits > 1 ? (items << 32) | tiles : 0;
@@ -184,33 +283,9 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
     }
     const unsigned long long before = bi + ii - items;
     if (blockIdx.x >= before && blockIdx.x < before + items) {
-      const unsigned long long j = blockIdx.x - before;
       const unsigned long long first = bg + gg - groups;
-      Item it;
-      it.seq = s;
-      it.g = (int)(j % b.nkv);
-      const unsigned long long js = j / b.nkv;
-      // the last tile, which sees most keys, first
-      const int split = (int)(js % splits), tile = x.tiles - 1 - (int)(js / splits);
-      it.row0 = q.row0 + tile * tpt;
-      it.tokens = min(tpt, q.q_len - tile * tpt);
-      it.pos0 = q.kv_len - q.q_len + tile * tpt;
-      const int last = it.pos0 + it.tokens - 1;
-      const int lo = first_unit(it.pos0, a.window, pl.unit);
-      const int n = last < 0 ? 0 : last / pl.unit - lo + 1;
-      const int per = (n + splits - 1) / splits;
-      it.u0 = lo + min(split * per, n);
-      it.u1 = lo + min((split + 1) * per, n);
-      it.slot = -1;
-      if (splits > 1) {
-        const int nth = tile * b.nkv + it.g;
-        const int slot0 = (int)(first >> 32) + nth * splits;
-        it.slot = slot0 + split;
-        if (split == 0)
-          part.groups[(int)(uint32_t)first + nth] =
-              Group{it.row0, it.tokens * a.group, it.g, slot0, splits};
-      }
-      found = it;
+      found = make_item(a, pl, part, tpt, s, q, x, splits, (uint32_t)(blockIdx.x - before),
+                        (uint32_t)first, (uint32_t)(first >> 32), true);
       have = 1;
     }
   }

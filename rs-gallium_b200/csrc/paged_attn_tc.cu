@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a) {
   using C = Cfg<HD>;
   constexpr int NT = C::NT, KT = C::KT, kBufs = C::kBufs;
+  constexpr int kHalves = kBufs == 1 ? 2 : 1;  // P handed over in parts
   // the buffer of a row tile's step, and the phase of its barriers
   auto buf_of = [](int w, int step) { return w * kBufs + (kBufs == 2 ? step & 1 : 0); };
   auto phase_of = [](int step) { return kBufs == 2 ? step >> 1 : step; };
@@ -185,13 +186,6 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
   const int tpt = 128 / a.group;  // tokens per row tile
-  Item it;
-  const bool have = find_item<false, C::kThreads>(a, kPlan, a.tiles, NT * tpt, &it);
-  pdl_trigger();
-  if (!have) {
-    pdl_wait();  // this grid ends after the kernel it was launched beside
-    return;
-  }
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* ring = smem + C::kQBytes;
@@ -200,12 +194,41 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
   uint64_t* kv_empty = bars + C::kRing;    // [kRing]
   uint64_t* q_full = bars + 2 * C::kRing;
   uint64_t* s_full = q_full + 1;           // [2 NT]: row tile and buffer
-  uint64_t* p_full = s_full + 2 * NT;      // [2 NT]
+  uint64_t* p_full = s_full + 2 * NT;      // [2 NT]: row tile, and buffer or half
   uint64_t* o_done = p_full + 2 * NT;      // [2 NT]: the PVs of a row tile in turn
   uint64_t* v_clean = o_done + 2 * NT;     // [2 NT]: a row tile's edge tiles in turn
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word, err_word, poisoned, any_bad;
   volatile int* abort_flag = &abort_word;
+
+  if (tid == 0) {
+    for (int i = 0; i < C::kRing; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 2 * NT; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_done[i], 1);
+      mbar_init(&v_clean[i], 128);
+    }
+    abort_word = err_word = poisoned = any_bad = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) tmem_alloc(&tmem_slot, C::kTmem);
+  // the item, while the barriers are set up and TMEM is allocated
+  Item it;
+  const bool have = find_item<false, C::kThreads>(a, kPlan, a.tiles, NT * tpt, &it);
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (!have) {
+    if (warp == 0) tmem_dealloc(tmem_slot, C::kTmem);
+    pdl_wait();  // this grid ends after the kernel it was launched beside
+    return;
+  }
 
   // The tiles: row tile w has tokens [w tpt, w tpt + n_w); key tiles [u0, u1).
   const int n0 = min(it.tokens, tpt), n1 = it.tokens - n0;
@@ -231,25 +254,6 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
   };
   auto edge = [&](int j) { return j * KT + KT - 1 > it.pos0 || j * KT < all_lo; };
 
-  if (tid == 0) {
-    for (int i = 0; i < C::kRing; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
-    }
-    mbar_init(q_full, 1);
-    for (int i = 0; i < 2 * NT; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
-      mbar_init(&o_done[i], 1);
-      mbar_init(&v_clean[i], 128);
-    }
-    abort_word = err_word = poisoned = any_bad = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 0) tmem_alloc(&tmem_slot, C::kTmem);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
   const uint32_t tmem = tmem_slot;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait(bar, parity & 1, abort_flag, &err_word);
@@ -368,22 +372,25 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
       const uint64_t scale2 = pair(a.scale, a.scale), ref2 = pair(-ref, -ref);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < KT / 2; c += 16) {
-        uint32_t p[16];
+      for (int h = 0; h < kHalves; ++h) {  // the MMAs of a half start while the next is computed
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int e = 2 * (c + i);
-          float2 v = unpair(fma2(pair(s[e], s[e + 1]), scale2, ref2));
-          v.x = ex2(v.x);
-          v.y = ex2(v.y);
-          sum[i & 1] = add2(sum[i & 1], pair(v.x, v.y));
-          p[i] = Elem<T>::pack(v.x, v.y);
+        for (int c = h * (KT / 2 / kHalves); c < (h + 1) * (KT / 2 / kHalves); c += 16) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int e = 2 * (c + i);
+            float2 v = unpair(fma2(pair(s[e], s[e + 1]), scale2, ref2));
+            v.x = ex2(v.x);
+            v.y = ex2(v.y);
+            sum[i & 1] = add2(sum[i & 1], pair(v.x, v.y));
+            p[i] = Elem<T>::pack(v.x, v.y);
+          }
+          tmem_st16(s_addr + c, p);
         }
-        tmem_st16(s_addr + c, p);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[kHalves == 2 ? 2 * w + h : buf]);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_full[buf]);
       {
         const float2 v = unpair(add2(sum[0], sum[1]));
         l += v.x + v.y;
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
       const int64_t part_row = split ? (int64_t)it.slot * kPlan.tile_rows + w * 128 + r : 0;
       if (split && live) a.tiles.ml[part_row] = make_float2(m, l);
       const bool poison = *(volatile int*)&poisoned != 0;
-#pragma unroll 1
+#pragma unroll(HD == 64 ? 2 : 1)
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
         if (steps) {
@@ -569,17 +576,22 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
       };
       auto issue_pv = [&](int w, uint32_t v_lo) -> bool {
         const int step = p_steps[w]++, buf = buf_of(w, step);
-        if (!all_wait(&p_full[buf], phase_of(step))) return false;
-        tc_fence_after();
         const uint32_t first = step ? 1u : 0u;
-        if (elect()) {
 #pragma unroll
-          for (int kk = 0; kk < KT / 16; ++kk)
-            mma_ts(t_base + C::kOCol + w * HD, t_base + buf * KT + kk * 8,
-                   desc_of(v_lo + kk * (2048 >> 4)), idesc<T>(HD, true), kk != 0 ? 1u : first);
-          mma_commit(&o_done[2 * w + (step & 1)]);
+        for (int h = 0; h < kHalves; ++h) {
+          if (!all_wait(&p_full[kHalves == 2 ? 2 * w + h : buf], phase_of(step))) return false;
+          tc_fence_after();
+          if (elect()) {
+#pragma unroll
+            for (int i = 0; i < KT / 16 / kHalves; ++i) {
+              const int kk = h * (KT / 16 / kHalves) + i;
+              mma_ts(t_base + C::kOCol + w * HD, t_base + buf * KT + kk * 8,
+                     desc_of(v_lo + kk * (2048 >> 4)), idesc<T>(HD, true), kk != 0 ? 1u : first);
+            }
+            if (h == kHalves - 1) mma_commit(&o_done[2 * w + (step & 1)]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
         return true;
       };
       auto free_slot = [&](int& slot, uint32_t& phase) {  // once the MMAs issued so far are done
