@@ -54,95 +54,214 @@ __device__ __forceinline__ void cp_wait() {
 
 // Keys per warp and step; a CTA's four warps take a unit of 64.
 constexpr int kStep = 16;
+constexpr int kWarps = kThreads / 32;
 
 template <int HD>
-constexpr int stages() { return HD == 64 ? 6 : HD == 128 ? 5 : 3; }
+constexpr int stages() { return HD == 64 ? 6 : 3; }
 template <int HD>
 constexpr int warp_bytes() { return stages<HD>() * 2 * kStep * HD * 2; }
+// the stages, Q, and the join of the warps' sums
 template <int HD>
-constexpr int q_bytes() { return kRows * HD * 2; }
-template <int HD>
-constexpr int smem_bytes() { return 4 * warp_bytes<HD>() + q_bytes<HD>(); }
+constexpr int smem_bytes() { return kWarps * warp_bytes<HD>() + kRows * HD * 2 + kRows * HD * 4; }
 
-// A CTA per item: four warps, each with keys of its own (16 of every unit) and
-// its own pipeline of cp.async stages, so no barrier stands in the loop; their
-// results are joined in shared memory at the end.
+// Where a CTA's share begins: the units of the decoding sequences' (sequence, KV
+// head) pairs in a row, cut into equal shares of `share` units.
+struct Share {
+  int64_t begin, units;  // begin < 0: none
+  int64_t share, total;
+  int seq;               // of the first unit
+  int64_t offset;        // of the first unit from the sequence's first
+};
+
+// The units of one of the sequence's pairs; a sequence with rows that see nothing
+// has one, in which its zeros are written.
+__device__ __forceinline__ int pair_units(const AttnArgs& a, const Plan& pl, const Seq& q) {
+  const SeqWork x = seq_work<true>(a, pl, q, kRows / a.group);
+  return x.tiles ? max(x.units, 1) : 0;
+}
+
+__device__ __forceinline__ void set_share(const AttnArgs& a, const Plan& pl, unsigned long long total,
+                                          Share* sh) {
+  const int64_t t = (int64_t)((total + pl.target - 1) / (unsigned)pl.target);
+  sh->share = t < pl.min_units ? pl.min_units : t;
+  sh->total = (int64_t)total;
+  sh->begin = blockIdx.x * sh->share;
+  sh->units = min(sh->share, sh->total - sh->begin);
+  if (sh->units <= 0) sh->begin = -1;
+}
+
+// Up to 128 sequences each warp holds them all, four a lane (mine); else the CTA
+// works out its share together and sequences are read when they are needed.
+__device__ Share find_share(const AttnArgs& a, const Plan& pl, Seq (&mine)[4]) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Batch& b = a.b;
+  Share sh;
+  sh.seq = 0;
+  sh.offset = 0;
+  if (b.n_seqs <= 128) {
+    unsigned long long w[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      mine[i] = Seq{0, 0, 0};
+      if (4 * lane + i < b.n_seqs) mine[i] = load_seq(b, 4 * lane + i, blockIdx.x == 0 && warp == 0);
+      w[i] = (unsigned long long)pair_units(a, pl, mine[i]) * b.nkv;
+      sum += w[i];
+    }
+    const unsigned long long inc = warp_inclusive(sum);
+    set_share(a, pl, __shfl_sync(kFullMask, inc, 31), &sh);
+    unsigned long long before = inc - sum;
+    int seq = -1;
+    int64_t off = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (sh.begin >= (int64_t)before && sh.begin < (int64_t)(before + w[i])) {
+        seq = 4 * lane + i;
+        off = sh.begin - (int64_t)before;
+      }
+      before += w[i];
+    }
+    const unsigned m = __ballot_sync(kFullMask, seq >= 0);
+    if (m) {
+      sh.seq = __shfl_sync(kFullMask, seq, __ffs(m) - 1);
+      sh.offset = __shfl_sync(kFullMask, (long long)off, __ffs(m) - 1);
+    }
+    return sh;
+  }
+  __shared__ unsigned long long part[kWarps];
+  __shared__ int first;
+  __shared__ long long first_off;
+  unsigned long long sum = 0;
+  for (int s = tid; s < b.n_seqs; s += kThreads)
+    sum += pair_units(a, pl, load_seq(b, s, blockIdx.x == 0));
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+  if (lane == 0) part[warp] = sum;
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) sum += part[i];
+  set_share(a, pl, sum * b.nkv, &sh);
+  if (sh.begin < 0) return sh;
+  unsigned long long base = 0;
+  for (int s0 = 0; s0 < b.n_seqs; s0 += kThreads) {
+    const int s = s0 + tid;
+    const unsigned long long w =
+        s < b.n_seqs ? (unsigned long long)pair_units(a, pl, load_seq(b, s, false)) * b.nkv : 0;
+    const unsigned long long inc = warp_inclusive(w);
+    __syncthreads();
+    if (lane == 31) part[warp] = inc;
+    __syncthreads();
+    unsigned long long before = base + inc - w;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) before += part[i];
+      base += part[i];
+    }
+    if (sh.begin >= (int64_t)before && sh.begin < (int64_t)(before + w)) {
+      first = s;
+      first_off = sh.begin - (int64_t)before;
+    }
+    if ((int64_t)base > sh.begin) break;  // the same in every thread
+  }
+  __syncthreads();
+  sh.seq = first;
+  sh.offset = first_off;
+  return sh;
+}
+
+// A place in the row of units.
+struct Cursor {
+  int seq, g, u, units, lo;  // KV head, unit of the pair, the pair's units, its first key unit
+  Seq q;
+};
+
+// Every CTA takes an equal share of the units of all decoding sequences, whatever
+// their lengths; where it cuts a pair, both sides leave partial sums for the
+// joining kernel.  Four warps, each with keys of its own (16 of every unit) and
+// its own pipeline of cp.async stages, which runs on across the pairs; their
+// results are joined in shared memory at the end of each.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_constant__ AttnArgs a) {
   extern __shared__ __align__(128) unsigned char sm[];
+  constexpr Plan kPlan = rows_plan<HD>();
   constexpr int kStages = stages<HD>();
   constexpr int C = HD / 8;                 // 16-byte pieces of a row
   constexpr int kStageBytes = 2 * kStep * HD * 2;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int tpt = kRows / a.group;
-  Item it;
-  constexpr Plan kPlan = kRowsPlan;
-  const bool have = find_item<true, kThreads>(a, kPlan, a.rows, tpt, &it);
+  Seq held[4];
+  const Share share = find_share(a, kPlan, held);
   pdl_trigger();
-  if (!have) return;
-  const int n_rows = it.tokens * a.group;
-  unsigned char* qs = sm + 4 * warp_bytes<HD>();
-  // Q rows, piece c of row r at c ^ (r & 7): ldmatrix reads 8 rows without bank conflicts
-  for (int i = tid; i < kRows * C; i += kThreads) {
-    const int r = i / C, c = i % C;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < n_rows) {
-      const int tok = r / a.group, h = it.g * a.group + r - tok * a.group;
-      v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
-                                          (it.row0 + tok) * a.q_row + h * a.q_head + c * 8);
-    }
-    *reinterpret_cast<uint4*>(qs + r * HD * 2 + ((c ^ (r & 7)) << 4)) = v;
-  }
-  __syncthreads();
+  // the pair that begins in this share and ends in a later one, if there is one
+  if (tid == 0) a.rows.groups[blockIdx.x].splits = 0;
+  if (share.begin < 0) return;
+  auto seq_at = [&](int s) -> Seq {  // the same in every lane
+    if (a.b.n_seqs > 128) return load_seq(a.b, s, false);
+    Seq q = held[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+      if ((s & 3) == i) q = held[i];
+    return Seq{__shfl_sync(kFullMask, q.row0, s >> 2), __shfl_sync(kFullMask, q.q_len, s >> 2),
+               __shfl_sync(kFullMask, q.kv_len, s >> 2)};
+  };
+  auto enter = [&](Cursor& c) {  // c.seq and c.q are set
+    c.units = pair_units(a, kPlan, c.q);
+    c.lo = first_unit(max(c.q.kv_len - c.q.q_len, 0), a.window, kPlan.unit);
+  };
+  auto next_pair = [&](Cursor& c) {
+    c.u = 0;
+    if (++c.g < a.b.nkv) return;
+    c.g = 0;
+    do {
+      if (++c.seq >= a.b.n_seqs) return;  // past the last unit: not used
+      c.q = seq_at(c.seq);
+      enter(c);
+    } while (!c.units);
+  };
+  Cursor at;
+  at.seq = share.seq;
+  at.q = seq_at(at.seq);
+  enter(at);
+  at.g = (int)(share.offset / at.units);
+  at.u = (int)(share.offset - (int64_t)at.g * at.units);
+  const int total = (int)share.units;
+
+  unsigned char* qs = sm + kWarps * warp_bytes<HD>();
+  float* os = reinterpret_cast<float*>(qs + kRows * HD * 2);  // [kRows][HD]
+  __shared__ unsigned bad_keys[kWarps][kStages];  // of each stage, a bit per key
+  __shared__ float wm[kWarps][kRows], wl[kWarps][kRows];
   const uint32_t qbase = smem_u32(qs);
   const uint32_t wbase = smem_u32(sm) + warp * warp_bytes<HD>();
-  constexpr bool kQInRegs = HD <= 128;
-  uint32_t qf[kQInRegs ? HD / 16 : 1][4];
-  auto load_q = [&](int ks, uint32_t(&f)[4]) {
-    const int r = lane & 15, c = ks * 2 + (lane >> 4);
-    ldsm4(f, qbase + r * HD * 2 + ((c ^ (r & 7)) << 4));
-  };
-  if constexpr (kQInRegs) {
-#pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) load_q(ks, qf[ks]);
-  }
-  // this lane's two rows
-  const int r0 = lane >> 2, r1 = r0 + 8;
-  const int p0 = it.pos0 + r0 / a.group, p1 = it.pos0 + r1 / a.group;
-  const int window = a.window > 0 ? a.window : 0x7fffffff;
-  const int last = it.pos0 + it.tokens - 1;
-  const int key_lo = max(0, a.window > 0 ? it.pos0 - a.window + 1 : 0);
-  // keys that every row sees lie in [all_lo, it.pos0]
-  const int all_lo = max(0, a.window > 0 ? last - a.window + 1 : 0);
-  float acc[HD / 8][4];
-#pragma unroll
-  for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-
-  const int n = it.u1 - it.u0;
-  const T* kp = static_cast<const T*>(a.k_pool) + it.g * a.b.head_stride;
-  const T* vp = static_cast<const T*>(a.v_pool) + it.g * a.b.head_stride;
-  const int32_t* table = a.b.table + it.seq * a.b.table_stride;
+  const T* kp = static_cast<const T*>(a.k_pool);
+  const T* vp = static_cast<const T*>(a.v_pool);
   const int page_mask = (1 << a.b.page_shift) - 1;
-  // the element offset of key lane & 15 of step u; -1: not to be read, -2: its page is bad
-  auto key_offset = [&](int u) -> int64_t {
-    const int key = (it.u0 + u) * kPlan.unit + warp * kStep + (lane & 15);
-    if (u >= n || key < key_lo || key > last) return -1;
-    const int page = __ldg(table + (key >> a.b.page_shift));
-    if ((unsigned)page >= (unsigned)a.b.n_pages) {
-      flag(a.b, GB_PAGED_BAD_PAGE);
-      return -2;
+
+  // The loads run kStages - 1 steps ahead, their page numbers one more.
+  Cursor ld = at;
+  int looked = 0;  // steps whose pages were looked up
+  // the element offset of key lane & 15 of the next step; -1: not to be read, -2: its page is bad
+  auto look_up = [&]() -> int64_t {
+    if (looked >= total) return -1;
+    ++looked;
+    const int key = (ld.lo + ld.u) * kPlan.unit + warp * kStep + (lane & 15);
+    const int first = a.window > 0 ? max(0, ld.q.kv_len - ld.q.q_len - a.window + 1) : 0;
+    int64_t off = -1;
+    if (key >= first && key < ld.q.kv_len) {
+      const int page = __ldg(a.b.table + ld.seq * a.b.table_stride + (key >> a.b.page_shift));
+      if ((unsigned)page < (unsigned)a.b.n_pages) {
+        off = page * a.b.page_stride + (key & page_mask) * a.b.slot_stride + ld.g * a.b.head_stride;
+      } else {
+        flag(a.b, GB_PAGED_BAD_PAGE);
+        off = -2;
+      }
     }
-    return page * a.b.page_stride + (key & page_mask) * a.b.slot_stride;
+    if (++ld.u == ld.units && looked < total) next_pair(ld);
+    return off;
   };
-  __shared__ unsigned bad_keys[4][kStages];  // of each stage, a bit per key
-  auto issue = [&](int u, int64_t off) {
-    const uint32_t dst = wbase + (u % kStages) * kStageBytes;
-    constexpr int kRowsPer = 32 / C > 0 ? 32 / C : 1;
+  auto issue = [&](int slot, int64_t off) {
+    const uint32_t dst = wbase + slot * kStageBytes;
+    constexpr int kRowsPer = 32 / C;
     const unsigned bad = __ballot_sync(kFullMask, off == -2) & 0xffffu;
-    if (lane == 0) bad_keys[warp][u % kStages] = bad;
+    if (lane == 0) bad_keys[warp][slot] = bad;
 #pragma unroll
     for (int i = 0; i < kStep / kRowsPer; ++i) {
       const int r = i * kRowsPer + lane / C, c = lane % C;
@@ -156,188 +275,267 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
   };
 #pragma unroll
   for (int u = 0; u < kStages - 1; ++u) {
-    if (u < n) issue(u, key_offset(u));
+    const int64_t off = look_up();
+    if (u < total) issue(u, off);
     cp_commit();
   }
-  int64_t next_off = key_offset(kStages - 1);
-  for (int u = 0; u < n; ++u) {
-    if (u + kStages - 1 < n) issue(u + kStages - 1, next_off);
-    cp_commit();
-    next_off = key_offset(u + kStages);
-    cp_wait<kStages - 1>();
-    __syncwarp();
-    const uint32_t ks_ = wbase + (u % kStages) * kStageBytes, vs_ = ks_ + kStep * HD * 2;
-    const int key0 = (it.u0 + u) * kPlan.unit + warp * kStep;
-    if (key0 <= last && key0 + kStep > key_lo) {  // the same on the whole warp
-      float s[2][4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        uint32_t kf[4], qt[4];
-        // keys 0-7 / 8-15, dims 0-7 / 8-15 of the step
-        const int r = (lane & 7) + ((lane >> 4) << 3), c = ks * 2 + ((lane >> 3) & 1);
-        ldsm4(kf, ks_ + r * HD * 2 + ((c ^ (r & 7)) << 4));
-        if constexpr (kQInRegs) {
-          mma16816<T>(s[0], qf[ks], kf[0], kf[1]);
-          mma16816<T>(s[1], qf[ks], kf[2], kf[3]);
-        } else {
-          load_q(ks, qt);
-          mma16816<T>(s[0], qt, kf[0], kf[1]);
-          mma16816<T>(s[1], qt, kf[2], kf[3]);
-        }
+  int64_t next_off = look_up();
+
+  int done = 0, slot = 0, fill = kStages - 1;  // steps computed; stages of the next step and load
+  while (done < total) {
+    // ---- a pair, or what of it is in this share
+    const int len = min(at.units - at.u, total - done);
+    const int n_rows = at.q.q_len * a.group, pos0 = at.q.kv_len - at.q.q_len;
+    const int last = at.q.kv_len - 1;
+    __syncthreads();  // the pair before is done with Q
+    // Q rows, piece c of row r at c ^ (r & 7): ldmatrix reads 8 rows without bank conflicts
+    for (int i = tid; i < kRows * C; i += kThreads) {
+      const int r = i / C, c = i % C;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < n_rows) {
+        const int tok = r / a.group, h = at.g * a.group + r - tok * a.group;
+        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
+                                            (at.q.row0 + tok) * a.q_row + h * a.q_head + c * 8);
       }
-      const unsigned bad = bad_keys[warp][u % kStages];
-      const bool masked = key0 + kStep - 1 > it.pos0 || key0 < all_lo || bad;
-      uint32_t seen = 0xffu;  // bit nt * 4 + j: score s[nt][j] is visible
+      *reinterpret_cast<uint4*>(qs + r * HD * 2 + ((c ^ (r & 7)) << 4)) = v;
+    }
+    __syncthreads();
+    constexpr bool kQInRegs = HD <= 128;
+    uint32_t qf[kQInRegs ? HD / 16 : 1][4];
+    auto load_q = [&](int ks, uint32_t(&f)[4]) {
+      const int r = lane & 15, c = ks * 2 + (lane >> 4);
+      ldsm4(f, qbase + r * HD * 2 + ((c ^ (r & 7)) << 4));
+    };
+    if constexpr (kQInRegs) {
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+      for (int ks = 0; ks < HD / 16; ++ks) load_q(ks, qf[ks]);
+    }
+    // this lane's two rows
+    const int r0 = lane >> 2, r1 = r0 + 8;
+    const int p0 = pos0 + r0 / a.group, p1 = pos0 + r1 / a.group;
+    const int window = a.window > 0 ? a.window : 0x7fffffff;
+    const int key_lo = max(0, a.window > 0 ? pos0 - a.window + 1 : 0);
+    // keys that every row sees lie in [all_lo, pos0]
+    const int all_lo = max(0, a.window > 0 ? last - a.window + 1 : 0);
+    float acc[HD / 8][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[nt][j] *= a.scale;
-      if (masked) {
-        seen = 0;
+    for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+
+    for (int k = 0; k < len; ++k) {
+      if (done + k + kStages - 1 < total) issue(fill, next_off);
+      cp_commit();
+      next_off = look_up();
+      cp_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t ks_ = wbase + slot * kStageBytes, vs_ = ks_ + kStep * HD * 2;
+      const int key0 = (at.lo + at.u + k) * kPlan.unit + warp * kStep;
+      if (key0 <= last && key0 + kStep > key_lo) {  // the same on the whole warp
+        float s[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          uint32_t kf[4], qt[4];
+          // keys 0-7 / 8-15, dims 0-7 / 8-15 of the step
+          const int r = (lane & 7) + ((lane >> 4) << 3), c = ks * 2 + ((lane >> 3) & 1);
+          ldsm4(kf, ks_ + r * HD * 2 + ((c ^ (r & 7)) << 4));
+          if constexpr (kQInRegs) {
+            mma16816<T>(s[0], qf[ks], kf[0], kf[1]);
+            mma16816<T>(s[1], qf[ks], kf[2], kf[3]);
+          } else {
+            load_q(ks, qt);
+            mma16816<T>(s[0], qt, kf[0], kf[1]);
+            mma16816<T>(s[1], qt, kf[2], kf[3]);
+          }
+        }
+        const unsigned bad = bad_keys[warp][slot];
+        const bool masked = key0 + kStep - 1 > pos0 || key0 < all_lo || bad;
+        uint32_t seen = 0xffu;  // bit nt * 4 + j: score s[nt][j] is visible
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int kk = nt * 8 + (lane & 3) * 2 + (j & 1), key = key0 + kk;
-            const int p = j < 2 ? p0 : p1;
-            if (key <= p && p - key < window && !((bad >> kk) & 1))
-              seen |= 1u << (nt * 4 + j);
-            else
-              s[nt][j] = -INFINITY;
-          }
-      }
-      float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-      float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-      x0 = fmaxf(x0, __shfl_xor_sync(kFullMask, x0, 1));
-      x1 = fmaxf(x1, __shfl_xor_sync(kFullMask, x1, 1));
-      x0 = fmaxf(x0, __shfl_xor_sync(kFullMask, x0, 2));
-      x1 = fmaxf(x1, __shfl_xor_sync(kFullMask, x1, 2));
-      // The reference (a maximum less kTop) moves only when a score passes the
-      // maximum by 2^6: the weights then stay below 2^(kTop + 6), which the
-      // 16-bit types hold as exactly as 1.
-      constexpr float kTop = Elem<T>::kTop;
-      if (__any_sync(kFullMask, x0 > m0 + (kTop + 6.0f) || x1 > m1 + (kTop + 6.0f))) {
-        const float n0 = fmaxf(m0, x0 - kTop), n1 = fmaxf(m1, x1 - kTop);
-        const float c0 = n0 == -INFINITY ? 1.0f : ex2(m0 - n0);
-        const float c1 = n1 == -INFINITY ? 1.0f : ex2(m1 - n1);
-        m0 = n0;
-        m1 = n1;
-        l0 *= c0;
-        l1 *= c1;
+          for (int j = 0; j < 4; ++j) s[nt][j] *= a.scale;
+        if (masked) {
+          seen = 0;
 #pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-          acc[i][0] *= c0;
-          acc[i][1] *= c0;
-          acc[i][2] *= c1;
-          acc[i][3] *= c1;
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int kk = nt * 8 + (lane & 3) * 2 + (j & 1), key = key0 + kk;
+              const int p = j < 2 ? p0 : p1;
+              if (key <= p && p - key < window && !((bad >> kk) & 1))
+                seen |= 1u << (nt * 4 + j);
+              else
+                s[nt][j] = -INFINITY;
+            }
         }
-      }
-      const float u0 = m0 == -INFINITY ? 0.0f : m0, u1 = m1 == -INFINITY ? 0.0f : m1;
+        float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+        float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+        x0 = fmaxf(x0, __shfl_xor_sync(kFullMask, x0, 1));
+        x1 = fmaxf(x1, __shfl_xor_sync(kFullMask, x1, 1));
+        x0 = fmaxf(x0, __shfl_xor_sync(kFullMask, x0, 2));
+        x1 = fmaxf(x1, __shfl_xor_sync(kFullMask, x1, 2));
+        // The reference (a maximum less kTop) moves only when a score passes the
+        // maximum by 2^6: the weights then stay below 2^(kTop + 6), which the
+        // 16-bit types hold as exactly as 1.
+        constexpr float kTop = Elem<T>::kTop;
+        if (__any_sync(kFullMask, x0 > m0 + (kTop + 6.0f) || x1 > m1 + (kTop + 6.0f))) {
+          const float n0 = fmaxf(m0, x0 - kTop), n1 = fmaxf(m1, x1 - kTop);
+          const float c0 = n0 == -INFINITY ? 1.0f : ex2(m0 - n0);
+          const float c1 = n1 == -INFINITY ? 1.0f : ex2(m1 - n1);
+          m0 = n0;
+          m1 = n1;
+          l0 *= c0;
+          l1 *= c1;
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        s[nt][0] = ex2(s[nt][0] - u0);
-        s[nt][1] = ex2(s[nt][1] - u0);
-        s[nt][2] = ex2(s[nt][2] - u1);
-        s[nt][3] = ex2(s[nt][3] - u1);
-        l0 += s[nt][0] + s[nt][1];
-        l1 += s[nt][2] + s[nt][3];
-      }
-      const uint32_t pf[4] = {Elem<T>::pack(s[0][0], s[0][1]), Elem<T>::pack(s[0][2], s[0][3]),
-                              Elem<T>::pack(s[1][0], s[1][1]), Elem<T>::pack(s[1][2], s[1][3])};
+          for (int i = 0; i < HD / 8; ++i) {
+            acc[i][0] *= c0;
+            acc[i][1] *= c0;
+            acc[i][2] *= c1;
+            acc[i][3] *= c1;
+          }
+        }
+        const float u0 = m0 == -INFINITY ? 0.0f : m0, u1 = m1 == -INFINITY ? 0.0f : m1;
 #pragma unroll
-      for (int dt = 0; dt < HD / 16; ++dt) {
-        uint32_t vf[4];
-        const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = dt * 2 + (lane >> 4);
-        ldsm4_t(vf, vs_ + r * HD * 2 + ((c ^ (r & 7)) << 4));
-        if (masked && __any_sync(kFullMask, any_nonfinite<T>(vf[0]) || any_nonfinite<T>(vf[1]) ||
-                                                any_nonfinite<T>(vf[2]) || any_nonfinite<T>(vf[3]))) {
-          // 0 x inf is NaN: add the visible products alone, key by key
-          for (int kk = 0; kk < kStep; ++kk) {
-            const int own = (lane & ~3) | ((kk & 7) >> 1), nt = kk >> 3;
-            const uint32_t sb = __shfl_sync(kFullMask, seen, own) >> (nt * 4 + (kk & 1));
-            const uint32_t a0 = __shfl_sync(kFullMask, pf[nt * 2], own);
-            const uint32_t a1 = __shfl_sync(kFullMask, pf[nt * 2 + 1], own);
-            const float2 f0 = Elem<T>::unpack(a0), f1 = Elem<T>::unpack(a1);
-            const float w0 = kk & 1 ? f0.y : f0.x, w1 = kk & 1 ? f1.y : f1.x;
+        for (int nt = 0; nt < 2; ++nt) {
+          s[nt][0] = ex2(s[nt][0] - u0);
+          s[nt][1] = ex2(s[nt][1] - u0);
+          s[nt][2] = ex2(s[nt][2] - u1);
+          s[nt][3] = ex2(s[nt][3] - u1);
+          l0 += s[nt][0] + s[nt][1];
+          l1 += s[nt][2] + s[nt][3];
+        }
+        const uint32_t pf[4] = {Elem<T>::pack(s[0][0], s[0][1]), Elem<T>::pack(s[0][2], s[0][3]),
+                                Elem<T>::pack(s[1][0], s[1][1]), Elem<T>::pack(s[1][2], s[1][3])};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int col = dt * 16 + h * 8 + (lane & 3) * 2;
-              const uint32_t vw = *reinterpret_cast<const uint32_t*>(
-                  sm + (vs_ - smem_u32(sm)) + kk * HD * 2 + (((col >> 3) ^ (kk & 7)) << 4) +
-                  (col & 7) * 2);
-              const float2 v = Elem<T>::unpack(vw);
-              if (sb & 1) {
-                acc[dt * 2 + h][0] += w0 * v.x;
-                acc[dt * 2 + h][1] += w0 * v.y;
-              }
-              if (sb & 4) {
-                acc[dt * 2 + h][2] += w1 * v.x;
-                acc[dt * 2 + h][3] += w1 * v.y;
+        for (int dt = 0; dt < HD / 16; ++dt) {
+          uint32_t vf[4];
+          const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = dt * 2 + (lane >> 4);
+          ldsm4_t(vf, vs_ + r * HD * 2 + ((c ^ (r & 7)) << 4));
+          if (masked && __any_sync(kFullMask, any_nonfinite<T>(vf[0]) || any_nonfinite<T>(vf[1]) ||
+                                                  any_nonfinite<T>(vf[2]) || any_nonfinite<T>(vf[3]))) {
+            // 0 x inf is NaN: add the visible products alone, key by key
+            for (int kk = 0; kk < kStep; ++kk) {
+              const int own = (lane & ~3) | ((kk & 7) >> 1), nt = kk >> 3;
+              const uint32_t sb = __shfl_sync(kFullMask, seen, own) >> (nt * 4 + (kk & 1));
+              const uint32_t a0 = __shfl_sync(kFullMask, pf[nt * 2], own);
+              const uint32_t a1 = __shfl_sync(kFullMask, pf[nt * 2 + 1], own);
+              const float2 f0 = Elem<T>::unpack(a0), f1 = Elem<T>::unpack(a1);
+              const float w0 = kk & 1 ? f0.y : f0.x, w1 = kk & 1 ? f1.y : f1.x;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int col = dt * 16 + h * 8 + (lane & 3) * 2;
+                const uint32_t vw = *reinterpret_cast<const uint32_t*>(
+                    sm + (vs_ - smem_u32(sm)) + kk * HD * 2 + (((col >> 3) ^ (kk & 7)) << 4) +
+                    (col & 7) * 2);
+                const float2 v = Elem<T>::unpack(vw);
+                if (sb & 1) {
+                  acc[dt * 2 + h][0] += w0 * v.x;
+                  acc[dt * 2 + h][1] += w0 * v.y;
+                }
+                if (sb & 4) {
+                  acc[dt * 2 + h][2] += w1 * v.x;
+                  acc[dt * 2 + h][3] += w1 * v.y;
+                }
               }
             }
+          } else {
+            mma16816<T>(acc[dt * 2], pf, vf[0], vf[1]);
+            mma16816<T>(acc[dt * 2 + 1], pf, vf[2], vf[3]);
           }
-        } else {
-          mma16816<T>(acc[dt * 2], pf, vf[0], vf[1]);
-          mma16816<T>(acc[dt * 2 + 1], pf, vf[2], vf[3]);
         }
       }
+      __syncwarp();  // the stage is read before a later issue overwrites it
+      fill = slot;
+      slot = slot + 1 == kStages ? 0 : slot + 1;
     }
-    __syncwarp();  // the stage is read before the next issue overwrites it
+    l0 += __shfl_xor_sync(kFullMask, l0, 1);
+    l1 += __shfl_xor_sync(kFullMask, l1, 1);
+    l0 += __shfl_xor_sync(kFullMask, l0, 2);
+    l1 += __shfl_xor_sync(kFullMask, l1, 2);
+    // ---- the warps' sums, added in their order
+    if ((lane & 3) == 0) {
+      wm[warp][r0] = m0;
+      wm[warp][r1] = m1;
+      wl[warp][r0] = l0;
+      wl[warp][r1] = l1;
+    }
+    __syncthreads();
+    float M0 = -INFINITY, M1 = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      M0 = fmaxf(M0, wm[w][r0]);
+      M1 = fmaxf(M1, wm[w][r1]);
+    }
+    const float f0 = m0 == -INFINITY ? 0.0f : ex2(m0 - M0), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - M1);
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) {
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          const int d = i * 8 + (lane & 3) * 2;
+          float2* o0 = reinterpret_cast<float2*>(os + r0 * HD + d);
+          float2* o1 = reinterpret_cast<float2*>(os + r1 * HD + d);
+          // a warp that saw nothing of a row adds nothing to it, not 0 x its sums
+          float2 x = w ? *o0 : make_float2(0.0f, 0.0f), y = w ? *o1 : make_float2(0.0f, 0.0f);
+          if (f0 != 0.0f) {
+            x.x += acc[i][0] * f0;
+            x.y += acc[i][1] * f0;
+          }
+          if (f1 != 0.0f) {
+            y.x += acc[i][2] * f1;
+            y.y += acc[i][3] * f1;
+          }
+          *o0 = x;
+          *o1 = y;
+        }
+      }
+      __syncthreads();
+    }
+    const bool whole = len == at.units;
+    // A partial result's slot: a share has at most two, in its first pair and its last.
+    const int part = 2 * blockIdx.x + (done ? 1 : 0);
+    for (int i = tid; i < n_rows * (HD / 2); i += kThreads) {
+      const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, wm[w][r]);
+      const int tok = r / a.group, h = at.g * a.group + r - tok * a.group;
+      const float top = M;
+      float L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        if (wm[w][r] != -INFINITY) L += wl[w][r] * ex2(wm[w][r] - M);
+      const float2 o = *reinterpret_cast<const float2*>(os + r * HD + d);
+      if (!whole) {
+        *reinterpret_cast<float2*>(a.rows.o + ((int64_t)part * kRows + r) * HD + d) = o;
+        if (d == 0) a.rows.ml[part * kRows + r] = make_float2(top, L);
+      } else {
+        float f = 1.0f;
+        if (a.sinks) {
+          const float sink = a.sinks[h] * kLog2e;
+          M = fmaxf(M, sink);
+          f = top == -INFINITY ? 0.0f : ex2(top - M);
+          L = L * f + (M == -INFINITY ? 0.0f : ex2(sink - M));
+        }
+        const float inv = L == 0.0f ? 0.0f : f / L;
+        store_out<T>(a, at.q.row0 + tok, h, d, o.x * inv, o.y * inv);
+      }
+    }
+    if (!whole && at.u == 0 && tid == 0) {
+      const int64_t end = share.begin + done + at.units - 1;  // the pair's last unit
+      a.rows.groups[blockIdx.x] =
+          Group{at.q.row0, n_rows, at.g, part, 2 * (int)blockIdx.x, 2,
+                (int)(end / share.share) - (int)blockIdx.x + 1};
+    }
+    done += len;
+    if (done < total) next_pair(at);
   }
   cp_wait<0>();
-  l0 += __shfl_xor_sync(kFullMask, l0, 1);
-  l1 += __shfl_xor_sync(kFullMask, l1, 1);
-  l0 += __shfl_xor_sync(kFullMask, l0, 2);
-  l1 += __shfl_xor_sync(kFullMask, l1, 2);
-  // join the four warps
-  __shared__ float wm[4][kRows], wl[4][kRows];
-  __syncthreads();  // the stages are free
-  float* os = reinterpret_cast<float*>(sm);  // [4][kRows][HD]
-  if ((lane & 3) == 0) {
-    wm[warp][r0] = m0;
-    wm[warp][r1] = m1;
-    wl[warp][r0] = l0;
-    wl[warp][r1] = l1;
-  }
-#pragma unroll
-  for (int i = 0; i < HD / 8; ++i) {
-    const int d = i * 8 + (lane & 3) * 2;
-    *reinterpret_cast<float2*>(os + (warp * kRows + r0) * HD + d) = make_float2(acc[i][0], acc[i][1]);
-    *reinterpret_cast<float2*>(os + (warp * kRows + r1) * HD + d) = make_float2(acc[i][2], acc[i][3]);
-  }
-  __syncthreads();
-  for (int i = tid; i < n_rows * (HD / 2); i += kThreads) {
-    const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, wm[w][r]);
-    const int tok = r / a.group, h = it.g * a.group + r - tok * a.group;
-    float sink = -INFINITY;
-    if (it.slot < 0 && a.sinks) sink = a.sinks[h] * kLog2e;
-    M = fmaxf(M, sink);
-    float L = M == -INFINITY ? 0.0f : ex2(sink - M), x = 0.0f, y = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (wm[w][r] == -INFINITY) continue;
-      const float f = ex2(wm[w][r] - M);
-      const float2 o = *reinterpret_cast<const float2*>(os + (w * kRows + r) * HD + d);
-      L += wl[w][r] * f;
-      x += o.x * f;
-      y += o.y * f;
-    }
-    if (it.slot >= 0) {
-      *reinterpret_cast<float2*>(a.rows.o + ((int64_t)it.slot * kRows + r) * HD + d) =
-          make_float2(x, y);
-      if (d == 0) a.rows.ml[it.slot * kRows + r] = make_float2(M, L);
-    } else {
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-      store_out<T>(a, it.row0 + tok, h, d, x * inv, y * inv);
-    }
-  }
 }
 
 // Joins the split tiles: a warp per row, its splits in order.  Both kinds of
@@ -346,7 +544,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kRows * 32) attn_join_kernel(const __grid_constant__ AttnArgs a) {
   pdl_wait();
   constexpr int kTileRows = tile_plan<HD>().tile_rows, kParts = kTileRows / kRows;
-  const int n_small = a.all_tiles ? 0 : __ldcg(a.rows.n_groups);
+  const int n_small = a.all_tiles ? 0 : a.rows_grid;
   const int n_tiles = a.tiles.n_groups ? __ldcg(a.tiles.n_groups) : 0;
   const int lane = threadIdx.x & 31;
   for (int i = blockIdx.x; i < n_small + n_tiles * kParts; i += gridDim.x) {
@@ -355,33 +553,56 @@ __global__ void __launch_bounds__(kRows * 32) attn_join_kernel(const __grid_cons
     const int rows = small ? kRows : kTileRows;
     const Group g = part.groups[small ? i : (i - n_small) / kParts];
     const int r = (small ? 0 : (i - n_small) % kParts * kRows) + (threadIdx.x >> 5);
-    if (r >= g.rows) continue;
+    if (!g.splits || r >= g.rows) continue;  // nothing else of g is written without splits
     const int tok = r / a.group, h = g.g * a.group + r - tok * a.group;
     // A large tile's rows are in sub-tiles of 128, each of whole tokens.
     const int per = small ? kRows : 128 / a.group * a.group;
     const int at_row = r / per * 128 + r % per;
     const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
     float M = sink;
-    for (int s = lane; s < g.splits; s += 32)
-      M = fmaxf(M, part.ml[(int64_t)(g.slot0 + s) * rows + at_row].x);
+    // row of partial result s
+    auto at_part = [&](int s) -> int64_t {
+      return (int64_t)(s ? g.slot1 + s * g.step : g.slot0) * rows + at_row;
+    };
+    float2 ml = make_float2(-INFINITY, 0.0f);  // of split `lane`, later of the chunk's
+    if (lane < g.splits) ml = part.ml[at_part(lane)];
+    M = fmaxf(M, ml.x);
+    for (int s = lane + 32; s < g.splits; s += 32) M = fmaxf(M, part.ml[at_part(s)].x);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFullMask, M, o));
     float L = M == -INFINITY ? 0.0f : ex2(sink - M);
     float acc[HD / 32];
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < g.splits; ++s) {
-      const int64_t at = (int64_t)(g.slot0 + s) * rows + at_row;
-      const float2 ml = part.ml[at];
-      // an empty split's sums are not written
-      const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-      L += f == 0.0f ? 0.0f : ml.y * f;
+    for (int s0 = 0; s0 < g.splits; s0 += 32) {
+      if (s0) {
+        ml = make_float2(-INFINITY, 0.0f);
+        if (s0 + lane < g.splits) ml = part.ml[at_part(s0 + lane)];
+      }
+      // an empty split's sums were written as well, but its weight is 0
+      const float fl = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M), ll = ml.y * fl;
+      constexpr int kU = HD == 64 ? 16 : HD == 128 ? 8 : 4;  // splits whose loads are in flight
+      const int n = min(32, g.splits - s0);
+      for (int s = 0; s < n; s += kU) {
+        float2 o[kU][HD / 64];
 #pragma unroll
-      for (int i = 0; i < HD / 64; ++i) {
-        const float2 o = *reinterpret_cast<const float2*>(part.o + at * HD + i * 64 + lane * 2);
-        acc[2 * i] += ml.x == -INFINITY ? 0.0f : o.x * f;
-        acc[2 * i + 1] += ml.x == -INFINITY ? 0.0f : o.y * f;
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int i = 0; i < HD / 64; ++i)
+            o[u][i] = s + u < n ? *reinterpret_cast<const float2*>(
+                                      part.o + at_part(s0 + s + u) * HD + i * 64 + lane * 2)
+                                : make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const float f = __shfl_sync(kFullMask, fl, (s + u) & 31), lu = __shfl_sync(kFullMask, ll, (s + u) & 31);
+          if (s + u >= n || f == 0.0f) continue;
+          L += lu;
+#pragma unroll
+          for (int i = 0; i < HD / 64; ++i) {
+            acc[2 * i] += o[u][i].x * f;
+            acc[2 * i + 1] += o[u][i].y * f;
+          }
+        }
       }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -407,7 +628,7 @@ size_t workspace_layout(int head_dim, char* base, AttnArgs* a) {
       *p = Partials{reinterpret_cast<int*>(n), reinterpret_cast<Group*>(g),
                     reinterpret_cast<float2*>(ml), reinterpret_cast<float*>(o)};
   };
-  part(kRowsPlan, a ? &a->rows : nullptr);
+  part(head_dim == 256 ? rows_plan<256>() : rows_plan<64>(), a ? &a->rows : nullptr);
   part(head_dim == 64 ? tile_plan<64>() : head_dim == 128 ? tile_plan<128>() : tile_plan<256>(),
        a ? &a->tiles : nullptr);
   return at;
@@ -424,18 +645,18 @@ cudaError_t launch_attn(AttnArgs a, int dtype, cudaStream_t st) {
   if (!tiles) a.tiles.n_groups = nullptr;
   cudaError_t e;
   if (!a.all_tiles) {
-    const int64_t grid =
-        grid_bound(a, kRowsPlan, (int64_t)std::min(a.b.n_seqs, a.b.total_q) * a.b.nkv);
-    if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    // shares, but no more than min_units each would make
+    constexpr Plan pl = rows_plan<HD>();
+    const int64_t most = (int64_t)std::min(a.b.n_seqs, a.b.total_q) * a.b.nkv * (a.b.max_kv / pl.unit + 1);
+    a.rows_grid = (int)std::min<int64_t>(pl.target, (most + pl.min_units - 1) / pl.min_units);
     auto kern = attn_rows_kernel<T, HD>;
     if ((e = set_smem_limit(kern, smem_bytes<HD>())) != cudaSuccess) return e;
-    kern<<<(unsigned)grid, kThreads, smem_bytes<HD>(), st>>>(a);
+    kern<<<(unsigned)a.rows_grid, kThreads, smem_bytes<HD>(), st>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   if (tiles && (e = launch_attn_tiles(a, dtype, HD, !a.all_tiles, st)) != cudaSuccess) return e;
-  // No sequence is split when the longest has too few keys for two splits.
-  const bool join = (!a.all_tiles && a.b.max_kv / kRowsPlan.unit + 1 > kRowsPlan.min_units) ||
-                    (tiles && a.b.max_kv / tp.unit + 1 > tp.min_units);
+  // One share cuts no pair; no tile is split when the longest sequence has too few keys.
+  const bool join = (!a.all_tiles && a.rows_grid > 1) || (tiles && a.b.max_kv / tp.unit + 1 > tp.min_units);
   if (!join) return cudaSuccess;
   return launch_pdl(attn_join_kernel<T, HD>, dim3(296), dim3(kRows * 32), 0, st, a);
 }

@@ -7,16 +7,15 @@
 //
 // Work.  The query heads that share a KV head are rows of one tile, so each
 // key is read once for all of them: a tile is (rows / group) tokens x group
-// heads.  A sequence with at most kRows such rows (a decoding one) is one
-// 16-row tile of attn_rows_kernel, any other goes to attn_tile_kernel's tiles
-// of 128 or 256 rows (where the host's bounds tell that no sequence of the
-// batch is a decoding one, attn_rows_kernel is not launched, and should the
-// device's lengths say otherwise, the tile kernel takes that sequence too).  A
-// tile's keys are split over several CTAs when the
-// batch has too few tiles to fill the GPU: each split writes its unnormalised
-// sum with its maximum and its sum of weights, and a last kernel joins them in
-// the order of the splits.  The lengths are on the device, so every CTA works
-// out its own item from them (a scan over the sequences), and the grids are
+// heads.  A sequence with at most kRows such rows (a decoding one) is one 16-row
+// tile of attn_rows_kernel, any other goes to attn_tile_kernel's tiles of 128 or
+// 256 rows (where the host's bounds tell that no sequence of the batch is a
+// decoding one, attn_rows_kernel is not launched, and should the device's lengths
+// say otherwise, the tile kernel takes that sequence too).  A tile's keys are cut
+// over several CTAs when the batch has too few tiles to fill the GPU: each part
+// writes its unnormalised sum with its maximum and its sum of weights, and a last
+// kernel joins them in their order.  The lengths are on the device, so every CTA
+// works out its own part from them (a scan over the sequences), and the grids are
 // sized from the host's bounds.
 #pragma once
 
@@ -52,7 +51,11 @@ struct Plan {
   int min_units;  // units per split, at least
   __host__ __device__ constexpr int slots() const { return 2 * target; }
 };
-constexpr Plan kRowsPlan{kRows, 64, 296, 2};  // two CTAs on each of 148 SMs
+// Shares of attn_rows_kernel: two CTAs on each of 148 SMs, one at head_dim 256.
+template <int HD>
+constexpr Plan rows_plan() {
+  return Plan{kRows, 64, HD == 256 ? 148 : 296, 2};
+}
 template <int HD>
 constexpr Plan tile_plan() {
   return HD == 64    ? Plan{128, 64, 296, 8}  // two CTAs per SM
@@ -61,7 +64,9 @@ constexpr Plan tile_plan() {
 }
 
 struct Group {  // a split tile, for the joining kernel
-  int row0, rows, g, slot0, splits;
+  int row0, rows, g;
+  int slot0, slot1, step;  // partial result s > 0 is in slot1 + s step, the first in slot0
+  int splits;
 };
 
 struct Partials {
@@ -74,6 +79,7 @@ struct Partials {
 struct AttnArgs {
   Batch b;
   int nh, group, window, out_f32;
+  int rows_grid;  // CTAs of attn_rows_kernel
   int all_tiles;  // attn_tile_kernel takes the decoding sequences too
   float scale;  // scale * log2 e
   const void* q;
@@ -155,7 +161,7 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, const Plan& pl, con
     const int slot0 = (int)first_slot + nth * splits;
     it.slot = slot0 + split;
     if (split == 0 && write_group)
-      part.groups[first_group + nth] = Group{it.row0, it.tokens * a.group, it.g, slot0, splits};
+      part.groups[first_group + nth] = Group{it.row0, it.tokens * a.group, it.g, slot0, slot0, 1, splits};
   }
   return it;
 }

@@ -114,6 +114,38 @@ class Case:
         return out, tol
 
 
+def _check_large(c, window=0, sinks=None, batch=None):
+    """The same check as _check_attention with the float64 reference on the GPU,
+    for batches that the row by row one is too slow for."""
+    torch = _torch()
+    s = None if sinks is None else torch.tensor(sinks, dtype=torch.float32).cuda()
+    batch = batch or c.batch()
+    out = paged.attention(batch, c.q, c.k, c.v, sinks=s, window=window)
+    batch.check()
+    for b, (n, kv) in enumerate(c.lens):
+        if not n:
+            continue
+        pages = torch.from_numpy(c.table_np[b, :-(-kv // c.page)]).long().cuda()
+        K, V = (x[pages].reshape(-1, c.kvh, c.dim)[:kv].double() for x in (c.k, c.v))
+        q = c.q[c.starts[b]:c.starts[b] + n].double()
+        pos = torch.arange(kv - n, kv, device="cuda")[:, None]
+        key = torch.arange(kv, device="cuda")[None]
+        hidden = (key > pos) | ((pos - key >= window) if window else False)
+        for h in range(c.heads):
+            k, v = K[:, h * c.kvh // c.heads], V[:, h * c.kvh // c.heads]
+            a = (q[:, h] @ k.T * c.dim ** -0.5).masked_fill(hidden, -math.inf)
+            e = (q[:, h].abs() @ k.abs().T).masked_fill(hidden, 0).amax(1, keepdim=True) * c.dim ** -0.5
+            if s is not None:
+                a = torch.cat([a, s[h].double().expand(n, 1)], 1)
+            w = torch.softmax(a, 1)[:, :kv]
+            want, A = w @ v, w @ v.abs()
+            tol = A * (U[c.dtype] + 2 * (e * (c.dim + 4) * U["f32"] + 2.0 ** -20) + kv * U["f32"]) + U[c.dtype] * want.abs()
+            got = out[c.starts[b]:c.starts[b] + n, h].double()
+            bad = (got - want).abs() - tol - SMALL[U[c.dtype]]
+            assert torch.isfinite(got).all() and bad.max() <= 0, (b, h, float(bad.max()))
+    return out
+
+
 def _close(got, want, tol, u):
     got = got.double().cpu().numpy()
     assert np.isfinite(got).all()
@@ -151,6 +183,34 @@ LENS = {
 @pytest.mark.parametrize("lens", list(LENS))
 def test_attention_lengths(lens, dtype):
     _check_attention(Case(LENS[lens], dtype=dtype, seed=1, spare_rows=3))
+
+
+@pytest.mark.parametrize("dim,heads,kvh", [(64, 16, 2), (128, 8, 2), (256, 4, 2)])
+@pytest.mark.parametrize("window", [0, 200])
+def test_attention_long_chunks(dim, heads, kvh, window):
+    """Prompts of many tiles (every key tile count, several waves of CTAs), with
+    and without cached keys, beside decoding sequences."""
+    lens = [(2048, 2048), (1, 3000), (777, 1500), (601, 601), (1, 5), (64, 4000)]
+    _check_large(Case(lens, heads=heads, kvh=kvh, dim=dim, seed=21, page=64), window=window,
+                 sinks=np.linspace(-2, 2, heads))
+
+
+@pytest.mark.parametrize("dim,heads,kvh,dtype", [(64, 8, 1, "bf16"), (128, 12, 4, "f16"), (256, 2, 2, "bf16")])
+def test_attention_many_sequences(dim, heads, kvh, dtype):
+    """More sequences than a warp holds, of very different lengths; some idle."""
+    r = np.random.default_rng(22)
+    lens = [(1, int(n)) for n in np.exp(r.uniform(0, np.log(3000), 300))]
+    lens[7] = lens[150] = lens[299] = (0, 40)
+    lens[40] = (2, 2)
+    for extra in ([], [(300, 900), (40, 40)]):
+        _check_large(Case(lens + extra, heads=heads, kvh=kvh, dim=dim, dtype=dtype, seed=23))
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 127, 128, 129, 256])
+def test_attention_equal_sequences(n):
+    """Shares that end with a pair, and shares that cut every pair."""
+    for kv in (64, 129, 1000):
+        _check_large(Case([(1, kv)] * n, heads=8, kvh=4, seed=24 + n), sinks=[0.5] * 8)
 
 
 @pytest.mark.parametrize("heads,kvh,dim", [(1, 1, 64), (3, 1, 128), (16, 1, 64), (10, 2, 64), (7, 7, 128), (12, 4, 256),
