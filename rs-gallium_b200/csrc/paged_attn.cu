@@ -56,8 +56,11 @@ __device__ __forceinline__ void cp_wait() {
 constexpr int kStep = 16;
 constexpr int kWarps = kThreads / 32;
 
+// Few stages for many warps: a step is a chain of some 370 instructions, and with two
+// warps on each scheduler (six stages of 4 KB at head_dim 64) the chains, not the
+// memory, were the bound (3.9 TB/s).
 template <int HD>
-constexpr int stages() { return HD == 64 ? 6 : 3; }
+constexpr int stages() { return HD == 128 ? 2 : 3; }
 template <int HD>
 constexpr int warp_bytes() { return stages<HD>() * 2 * kStep * HD * 2; }
 // the stages, Q, and the join of the warps' sums
@@ -92,7 +95,7 @@ __device__ __forceinline__ void set_share(const AttnArgs& a, const Plan& pl, uns
 
 // Up to 128 sequences each warp holds them all, four a lane (mine); else the CTA
 // works out its share together and sequences are read when they are needed.
-__device__ Share find_share(const AttnArgs& a, const Plan& pl, Seq (&mine)[4]) {
+__device__ __forceinline__ Share find_share(const AttnArgs& a, const Plan& pl, Seq (&mine)[4]) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Batch& b = a.b;
   Share sh;
@@ -181,7 +184,8 @@ struct Cursor {
 // its own pipeline of cp.async stages, which runs on across the pairs; their
 // results are joined in shared memory at the end of each.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
+    attn_rows_kernel(const __grid_constant__ AttnArgs a) {
   extern __shared__ __align__(128) unsigned char sm[];
   constexpr Plan kPlan = rows_plan<HD>();
   constexpr int kStages = stages<HD>();
@@ -628,7 +632,8 @@ size_t workspace_layout(int head_dim, char* base, AttnArgs* a) {
       *p = Partials{reinterpret_cast<int*>(n), reinterpret_cast<Group*>(g),
                     reinterpret_cast<float2*>(ml), reinterpret_cast<float*>(o)};
   };
-  part(head_dim == 256 ? rows_plan<256>() : rows_plan<64>(), a ? &a->rows : nullptr);
+  part(head_dim == 64 ? rows_plan<64>() : head_dim == 128 ? rows_plan<128>() : rows_plan<256>(),
+       a ? &a->rows : nullptr);
   part(head_dim == 64 ? tile_plan<64>() : head_dim == 128 ? tile_plan<128>() : tile_plan<256>(),
        a ? &a->tiles : nullptr);
   return at;
@@ -658,7 +663,7 @@ cudaError_t launch_attn(AttnArgs a, int dtype, cudaStream_t st) {
   // One share cuts no pair; no tile is split when the longest sequence has too few keys.
   const bool join = (!a.all_tiles && a.rows_grid > 1) || (tiles && a.b.max_kv / tp.unit + 1 > tp.min_units);
   if (!join) return cudaSuccess;
-  return launch_pdl(attn_join_kernel<T, HD>, dim3(296), dim3(kRows * 32), 0, st, a);
+  return launch_pdl(attn_join_kernel<T, HD>, dim3(592), dim3(kRows * 32), 0, st, a);
 }
 
 template <typename T>

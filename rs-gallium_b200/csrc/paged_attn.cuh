@@ -51,10 +51,10 @@ struct Plan {
   int min_units;  // units per split, at least
   __host__ __device__ constexpr int slots() const { return 2 * target; }
 };
-// Shares of attn_rows_kernel: two CTAs on each of 148 SMs, one at head_dim 256.
+// Shares of attn_rows_kernel: four, three or one CTA on each of 148 SMs.
 template <int HD>
-constexpr Plan rows_plan() {
-  return Plan{kRows, 64, HD == 256 ? 148 : 296, 2};
+__host__ __device__ constexpr Plan rows_plan() {
+  return Plan{kRows, 64, 148 * (HD == 64 ? 4 : HD == 128 ? 3 : 1), 2};
 }
 template <int HD>
 constexpr Plan tile_plan() {

@@ -59,18 +59,15 @@ namespace {
 
 // ---- norm + rotation + page append -----------------------------------------
 // One pass over q, k and v: y = x / sqrt(mean(x^2) + eps) * w over a head, then
-// the halves-layout rotation, q to q_out, k and v to their pages.  The work is
-// a list of (row, head) units, rows of nh + 2 nkv heads; a group of
-// head_dim / 8 lanes takes one unit, 8 elements (16 bytes of a 2-byte type) a
-// lane, so a warp's loads and stores are whole 128-byte lines.  The rotation
+// the halves-layout rotation, q to q_out, k and v to their pages.  A group of
+// head_dim / 8 lanes takes a head of a row, 8 elements (16 bytes of a 2-byte type)
+// a lane, so a warp's loads and stores are whole 128-byte lines.  The rotation
 // pairs element j with j + rot / 2, which another lane of the group holds at a
-// fixed lane distance (rot / 16), so one shuffle per element exchanges them.
-// Bound by memory: each element is read once and written once.  The rows'
-// sequences and slots are looked up by one warp per row (32-way search of
-// q_start) while the first loads of q, k and v, which need neither, are in
-// flight.
+// fixed lane distance (rot / 16), so one shuffle per element exchanges them.  Each
+// element is read once and written once; memory is the floor.
 
 constexpr int kRopeThreads = 256;
+constexpr int kRopeRows = 64;  // rows per CTA, at most
 
 struct RopeArgs {
   Batch b;
@@ -162,105 +159,178 @@ struct Load8<float> {
   }
 };
 
-// U units of each lane group in flight.
-template <typename In, typename Out, int HD, int U>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int L = HD / 8;                // lanes per unit
-  constexpr int G = kRopeThreads / L;      // units per pass of the CTA
-  constexpr int kMaxRows = G * U;          // rows a CTA's units can touch
-  __shared__ RowInfo rows[kMaxRows];
-  const int heads = a.nh + 2 * a.b.nkv;
-  const int64_t unit0 = (int64_t)blockIdx.x * (G * U);
-  const int64_t last = min(unit0 + G * U, a.units) - 1;
-  const int row0 = (int)(unit0 / heads), n_rows = (int)(last / heads) - row0 + 1;
-  const int grp = threadIdx.x / L, gl = threadIdx.x % L, d = gl * 8;
-  Load8<In> x[U];
-  int row[U], head[U];
+// Norm and rotation of a head, 8 elements a lane.  w: norm weights or null (norms:
+// some head of the call has them, so the sums are taken by every lane); cs, sn: the
+// lane's cosines and sines, sn negative in the first half of the rotated elements;
+// rotates: this lane's elements are rotated.
+template <int HD>
+__device__ __forceinline__ void norm_rotate(float (&y)[8], bool norms, const float* w, int d, float eps,
+                                            bool rotation, bool rotates, int partner,
+                                            const float (&cs)[8], const float (&sn)[8]) {
+  if (norms) {
+    float ss = 0.0f;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t unit = unit0 + u * G + grp;
-    row[u] = -1;
-    head[u] = 0;
-    if (unit <= last) {
-      row[u] = (int)(unit / heads);
-      head[u] = (int)(unit - (int64_t)row[u] * heads);
-      const int h = head[u];
-      if (h < a.nh)
-        x[u].load(a.q, row[u] * a.q_row + h * a.q_head + d);
-      else if (h < a.nh + a.b.nkv)
-        x[u].load(a.k, row[u] * a.k_row + (h - a.nh) * a.k_head + d);
-      else
-        x[u].load(a.v, row[u] * a.v_row + (h - a.nh - a.b.nkv) * a.v_head + d);
+    for (int i = 0; i < 8; ++i) ss = __fmaf_rn(y[i], y[i], ss);
+#pragma unroll
+    for (int o = HD / 16; o >= 1; o >>= 1) ss += __shfl_xor_sync(kFullMask, ss, o);
+    if (w) {
+      const float inv = rsqrtf(__fmaf_rn(ss, 1.0f / HD, eps));
+      const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + d));
+      const float4 w1 = __ldg(reinterpret_cast<const float4*>(w + d + 4));
+      const float ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * ws[i];
     }
+  }
+  if (rotation) {
+    float other[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(kFullMask, y[i], partner);
+    if (rotates) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fmaf_rn(y[i], cs[i], other[i] * sn[i]);
+    }
+  }
+}
+
+// cs and sn of a lane whose elements start at d, for a row at `pos`.
+__device__ __forceinline__ void load_turn(const RopeArgs& a, int pos, int half, int d, float (&cs)[8],
+                                          float (&sn)[8]) {
+  const bool first = d < half;
+  const int64_t at = (int64_t)pos * half + (first ? d : d - half);
+  const float4* c4 = reinterpret_cast<const float4*>(a.cos_t + at);
+  const float4* s4 = reinterpret_cast<const float4*>(a.sin_t + at);
+  const float4 c0 = __ldg(c4), c1 = __ldg(c4 + 1), s0 = __ldg(s4), s1 = __ldg(s4 + 1);
+  cs[0] = c0.x, cs[1] = c0.y, cs[2] = c0.z, cs[3] = c0.w;
+  cs[4] = c1.x, cs[5] = c1.y, cs[6] = c1.z, cs[7] = c1.w;
+  sn[0] = s0.x, sn[1] = s0.y, sn[2] = s0.z, sn[3] = s0.w;
+  sn[4] = s1.x, sn[5] = s1.y, sn[6] = s1.z, sn[7] = s1.w;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sn[i] = first ? -sn[i] : sn[i];
+}
+
+template <typename Out>
+__device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
+  return make_uint4(Elem<Out>::pack(y[0], y[1]), Elem<Out>::pack(y[2], y[3]),
+                    Elem<Out>::pack(y[4], y[5]), Elem<Out>::pack(y[6], y[7]));
+}
+
+// Few (row, head) units: one per lane group, over as many CTAs as that takes.  The
+// rows' sequences and slots are looked up while the units' loads are in flight.
+template <typename In, typename Out, int HD>
+__global__ void __launch_bounds__(kRopeThreads) rope_units_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int L = HD / 8;                // lanes per unit
+  constexpr int G = kRopeThreads / L;      // units of the CTA
+  __shared__ RowInfo rows[G];
+  const int heads = a.nh + 2 * a.b.nkv;
+  const int64_t unit0 = (int64_t)blockIdx.x * G, last = min(unit0 + G, a.units) - 1;
+  const int row0 = (int)(unit0 / heads), n_rows = (int)(last / heads) - row0 + 1;
+  const int d = threadIdx.x % L * 8, lane = threadIdx.x & 31;
+  const int64_t unit = unit0 + threadIdx.x / L;
+  const bool live = unit <= last;
+  const int row = live ? (int)(unit / heads) : row0;
+  const int h = live ? (int)(unit - (int64_t)row * heads) : 0;
+  const bool is_q = h < a.nh, is_v = h >= a.nh + a.b.nkv;
+  Load8<In> x;
+  if (live) {
+    if (is_q)
+      x.load(a.q, row * a.q_row + h * a.q_head + d);
+    else if (!is_v)
+      x.load(a.k, row * a.k_row + (h - a.nh) * a.k_head + d);
+    else
+      x.load(a.v, row * a.v_row + (h - a.nh - a.b.nkv) * a.v_head + d);
   }
   for (int i = threadIdx.x >> 5; i < n_rows; i += kRopeThreads / 32) {
-    const RowInfo r = find_row(a.b, row0 + i, a.rot ? a.table_rows : INT64_MAX, threadIdx.x & 31);
-    if ((threadIdx.x & 31) == 0) rows[i] = r;
+    const RowInfo r = find_row(a.b, row0 + i, a.rot ? a.table_rows : INT64_MAX, lane);
+    if (lane == 0) rows[i] = r;
   }
   __syncthreads();
-  const int half = a.rot / 2;
+  const RowInfo info = live ? rows[row - row0] : RowInfo{-1, 0, -1};
+  const int half = a.rot / 2, gap = half / 8;  // lanes to the rotation's partner
+  const int partner = d < half ? lane + gap : d < a.rot ? lane - gap : lane;
+  const bool rotates = !is_v && d < a.rot && info.pos >= 0;
+  float y[8] = {}, cs[8] = {}, sn[8] = {};
+  if (live) x.get(y);
+  if (rotates) load_turn(a, info.pos, half, d, cs, sn);
+  norm_rotate<HD>(y, a.q_norm || a.k_norm, is_v ? nullptr : is_q ? a.q_norm : a.k_norm, d, a.eps, half,
+                  rotates, partner, cs, sn);
+  if (!live || info.pos < 0) return;
+  const uint4 o = pack8<Out>(y);
+  if (is_q) {
+    *reinterpret_cast<uint4*>(static_cast<Out*>(a.q_out) + row * a.o_row + h * a.o_head + d) = o;
+  } else if (info.page >= 0) {
+    const int g = is_v ? h - a.nh - a.b.nkv : h - a.nh;
+    Out* pool = static_cast<Out*>(is_v ? a.v_pool : a.k_pool);
+    *reinterpret_cast<uint4*>(pool + info.page + info.slot * a.b.slot_stride + g * a.b.head_stride + d) = o;
+  }
+}
+
+// Many rows: a CTA takes `per` of them (at most kRopeRows).  `across` lane groups
+// share a row, each with its heads in turn, so that a row's cosines, sines, page
+// and addresses are worked out once for them; the groups' other rows run beside.
+template <typename In, typename Out, int HD>
+__global__ void __launch_bounds__(kRopeThreads, 4)
+    rope_rows_kernel(const __grid_constant__ RopeArgs a, int per, int across) {
+  constexpr int L = HD / 8;
+  constexpr int G = kRopeThreads / L;
+  constexpr int U = 3;  // heads whose loads are in flight
+  __shared__ RowInfo rows[kRopeRows];
+  const int heads = a.nh + 2 * a.b.nkv;
+  const int row0 = blockIdx.x * per, n_rows = min(per, a.b.total_q - row0);
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < n_rows; i += kRopeThreads / 32) {
+    const RowInfo r = find_row(a.b, row0 + i, a.rot ? a.table_rows : INT64_MAX, lane);
+    if (lane == 0) rows[i] = r;
+  }
+  __syncthreads();
+  const int d = threadIdx.x % L * 8;
+  const int grp = threadIdx.x / L, beside = G / across;  // rows at a time
+  const int sub = grp / across, h0 = grp - sub * across;
+  const int half = a.rot / 2, gap = half / 8;
+  const int partner = d < half ? lane + gap : d < a.rot ? lane - gap : lane;
+  const bool norms = a.q_norm || a.k_norm;
+  for (int i0 = 0; i0 < n_rows; i0 += beside) {  // the same passes in every lane
+    const int i = i0 + sub;
+    const RowInfo info = sub < beside && i < n_rows ? rows[i] : RowInfo{-1, 0, -1};
+    const bool on = info.pos >= 0;
+    float cs[8] = {}, sn[8] = {};
+    if (on && d < a.rot) load_turn(a, info.pos, half, d, cs, sn);
+    const int64_t r = row0 + i;
+    const int64_t q_at = r * a.q_row + d, k_at = r * a.k_row + d, v_at = r * a.v_row + d;
+    const int64_t o_at = r * a.o_row + d;
+    const int64_t p_at = info.page < 0 ? -1 : info.page + info.slot * a.b.slot_stride + d;
+    for (int hb = 0; hb < heads; hb += across * U) {
+      Load8<In> x[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int h = head[u];
-    const bool live = row[u] >= 0;
-    const RowInfo info = live ? rows[row[u] - row0] : RowInfo{-1, 0, -1};
-    const bool is_q = h < a.nh, is_v = h >= a.nh + a.b.nkv;
-    float y[8];
-    if (live) {
-      x[u].get(y);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = 0.0f;
-    }
-    const float* w = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
-    if (a.q_norm || a.k_norm) {  // the same on every lane: the shuffles meet
-      float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = __fmaf_rn(y[i], y[i], ss);
-#pragma unroll
-      for (int o = L / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(kFullMask, ss, o);
-      if (w) {
-        const float m = sqrtf(__fadd_rn(__fmul_rn(ss, 1.0f / HD), a.eps));
-        const float4 w0 = *reinterpret_cast<const float4*>(w + d);
-        const float4 w1 = *reinterpret_cast<const float4*>(w + d + 4);
-        const float ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(__fdiv_rn(y[i], m), ws[i]);
+      for (int u = 0; u < U; ++u) {
+        const int h = hb + u * across + h0;
+        if (!on || h >= heads) continue;
+        if (h < a.nh)
+          x[u].load(a.q, q_at + h * a.q_head);
+        else if (h < a.nh + a.b.nkv)
+          x[u].load(a.k, k_at + (h - a.nh) * a.k_head);
+        else
+          x[u].load(a.v, v_at + (h - a.nh - a.b.nkv) * a.v_head);
       }
-    }
-    if (half) {
-      const int lane = threadIdx.x & 31, gap = half / 8;  // lanes to the partner
-      const bool first = gl < gap;
-      const int partner = first ? lane + gap : gl < 2 * gap ? lane - gap : lane;
-      float other[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(kFullMask, y[i], partner);
-      if (!is_v && gl < 2 * gap && info.pos >= 0) {
-        const int64_t at = (int64_t)info.pos * half + (first ? d : d - half);
-        const float4* c4 = reinterpret_cast<const float4*>(a.cos_t + at);
-        const float4* s4 = reinterpret_cast<const float4*>(a.sin_t + at);
-        const float4 c0 = c4[0], c1 = c4[1], s0 = s4[0], s1 = s4[1];
-        const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-        const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          y[i] = first ? __fsub_rn(__fmul_rn(y[i], cs[i]), __fmul_rn(other[i], sn[i]))
-                       : __fadd_rn(__fmul_rn(other[i], sn[i]), __fmul_rn(y[i], cs[i]));
+      for (int u = 0; u < U; ++u) {
+        if (hb + u * across >= heads) break;  // for every group
+        const int h = hb + u * across + h0;
+        const bool live = on && h < heads, is_q = h < a.nh, is_v = h >= a.nh + a.b.nkv;
+        float y[8] = {};
+        if (live) x[u].get(y);
+        norm_rotate<HD>(y, norms, is_v ? nullptr : is_q ? a.q_norm : a.k_norm, d, a.eps, half,
+                        live && !is_v && d < a.rot, partner, cs, sn);
+        if (!live) continue;
+        const uint4 o = pack8<Out>(y);
+        if (is_q) {
+          *reinterpret_cast<uint4*>(static_cast<Out*>(a.q_out) + o_at + h * a.o_head) = o;
+        } else if (p_at >= 0) {
+          const int g = is_v ? h - a.nh - a.b.nkv : h - a.nh;
+          *reinterpret_cast<uint4*>(static_cast<Out*>(is_v ? a.v_pool : a.k_pool) + p_at +
+                                    g * a.b.head_stride) = o;
+        }
       }
-    }
-    if (!live || info.pos < 0) continue;
-    uint4 o;
-    o.x = Elem<Out>::pack(y[0], y[1]);
-    o.y = Elem<Out>::pack(y[2], y[3]);
-    o.z = Elem<Out>::pack(y[4], y[5]);
-    o.w = Elem<Out>::pack(y[6], y[7]);
-    if (is_q) {
-      *reinterpret_cast<uint4*>(static_cast<Out*>(a.q_out) + row[u] * a.o_row + h * a.o_head + d) = o;
-    } else if (info.page >= 0) {
-      const int g = is_v ? h - a.nh - a.b.nkv : h - a.nh;
-      Out* pool = static_cast<Out*>(is_v ? a.v_pool : a.k_pool);
-      *reinterpret_cast<uint4*>(pool + info.page + info.slot * a.b.slot_stride +
-                                g * a.b.head_stride + d) = o;
     }
   }
 }
@@ -268,12 +338,16 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_
 template <typename In, typename Out, int HD>
 cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st) {
   constexpr int G = kRopeThreads / (HD / 8);
-  // Few units: one per lane group, so that they spread over the SMs.
+  const int heads = a.nh + 2 * a.b.nkv;
   if (a.units <= (int64_t)G * 148 * 4) {
-    rope_append_kernel<In, Out, HD, 1><<<(unsigned)((a.units + G - 1) / G), kRopeThreads, 0, st>>>(a);
+    rope_units_kernel<In, Out, HD><<<(unsigned)((a.units + G - 1) / G), kRopeThreads, 0, st>>>(a);
   } else {
-    rope_append_kernel<In, Out, HD, 4>
-        <<<(unsigned)((a.units + 4 * G - 1) / (4 * G)), kRopeThreads, 0, st>>>(a);
+    // Four CTAs an SM, a few rows each: the look-ups of a row are some 1.5 us of
+    // dependent loads, which other CTAs' rows hide.
+    const int64_t rows = a.units / heads;
+    const int per = (int)std::max<int64_t>(1, std::min<int64_t>(kRopeRows, rows / (148 * 4 * 4)));
+    rope_rows_kernel<In, Out, HD>
+        <<<(unsigned)((rows + per - 1) / per), kRopeThreads, 0, st>>>(a, per, std::min(heads, G));
   }
   return cudaGetLastError();
 }
