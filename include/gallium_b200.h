@@ -579,6 +579,30 @@ int gb_paged_copy(void* const* pools_dev, int32_t n_pools, int64_t n_pages, int6
                   int64_t page_stride, const int32_t* src, const int32_t* dst, int32_t n,
                   void* stream);
 
+/* One forward of the GPT-OSS decode stack over a paged cache: n_seqs sequences,
+ * each with its own number of new tokens at its own positions (the batch), where
+ * gb_decoder_forward runs B sequences in lockstep on the decoder's own cache.
+ * tokens_dev [total_q] i32; k_pools / v_pools: host arrays of n_layers device
+ * pointers, a K and a V pool per layer, laid out as the batch says (head_dim and
+ * n_kv_heads the model's; head_dim 64, 128 or 256).  Every layer stores its new
+ * keys and values into the pools (gb_paged_rope_append) and attends over the pages
+ * (gb_paged_attention); queries, keys and values are rounded to the pools' type,
+ * all else is f32 as in gb_decoder_forward.  total_q <= max_batch * max_tokens,
+ * n_seqs <= max_batch, positions below max_seq_len.  logits_dev (nullable, 16-byte
+ * aligned): f32 [n_seqs][vocab] of each sequence's last new token; next_dev
+ * (nullable): i32 [n_seqs], its greedy token; a sequence without new tokens gets
+ * zero logits (and the last id, as of equal logits).  tokens_dev of rows of no
+ * sequence are token ids too.  The decoder keeps nothing of the sequences and its
+ * own cache and position are untouched; its activation buffers are shared with the
+ * other forwards, so calls on several streams must be ordered by the caller.
+ * Asynchronous on `stream` and capturable after a first call, which allocates the
+ * attention workspace.  What the batch's device arrays do wrong is flagged in its
+ * error word, a token id out of range in gb_decoder_device_status. */
+int gb_decoder_forward_paged(gb_decoder* d, const int32_t* tokens_dev,
+                             const gb_paged_batch* batch, void* const* k_pools,
+                             void* const* v_pools, float* logits_dev, int32_t* next_dev,
+                             void* stream);
+
 /* ---- Sampling --------------------------------------------------------------
  * One token per row of logits, drawn with a uniform number that the caller
  * gives (sampling.rs:7-173 draws from its own generator): beside the greedy

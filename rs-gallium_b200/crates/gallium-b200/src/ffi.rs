@@ -331,6 +331,10 @@ extern "C" {
     pub fn gb_paged_copy(pools_dev: *const *mut c_void, n_pools: i32, n_pages: i64,
                          page_bytes: i64, page_stride: i64, src: *const i32, dst: *const i32,
                          n: i32, stream: *mut c_void) -> c_int;
+    pub fn gb_decoder_forward_paged(d: *mut gb_decoder, tokens_dev: *const i32,
+                                    batch: *const gb_paged_batch, k_pools: *const *mut c_void,
+                                    v_pools: *const *mut c_void, logits_dev: *mut f32,
+                                    next_dev: *mut i32, stream: *mut c_void) -> c_int;
     pub fn gb_sample(args: *const gb_sample_args, stream: *mut c_void) -> c_int;
     pub fn gb_nccl_unique_id(out: *mut u8) -> c_int;
     pub fn gb_last_error() -> *const c_char;

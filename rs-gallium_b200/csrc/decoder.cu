@@ -78,10 +78,22 @@ __global__ void __launch_bounds__(kNormThreads)
     add_rmsnorm_kernel(float* __restrict__ h, const float* __restrict__ delta,
                        const float* __restrict__ w, int H, float eps, int src_stride, int src_off,
                        float* __restrict__ out, __nv_bfloat16* __restrict__ oh,
-                       __nv_bfloat16* __restrict__ ol) {
+                       __nv_bfloat16* __restrict__ ol, const int32_t* __restrict__ q_start,
+                       int n_rows) {
   __shared__ float red[32];
   const int r = blockIdx.x;
-  const int64_t src = (int64_t)(r * src_stride + src_off) * H;
+  int64_t src = (int64_t)(r * src_stride + src_off) * H;
+  if (q_start) {
+    const int first = max(q_start[r], 0), end = min(q_start[r + 1], n_rows);
+    if (end <= first) {
+      for (int i = threadIdx.x; i < H; i += blockDim.x) {
+        out[(int64_t)r * H + i] = 0.0f;
+        if (oh) split_store(oh, ol, (int64_t)r * H + i, 0.0f);
+      }
+      return;
+    }
+    src = (int64_t)(end - 1) * H;
+  }
   float4* x4 = reinterpret_cast<float4*>(h + src);
   const float4* d4 = delta ? reinterpret_cast<const float4*>(delta + src) : nullptr;
   const int n4 = H / 4;
@@ -702,6 +714,9 @@ struct Decoder {
   float* rope_sin = nullptr;
   float* kcache = nullptr;      // [L][max_batch][nkv][S][hd]
   float* vcache = nullptr;
+  void* q16 = nullptr;          // paged forwards: [rows_cap][nh hd] rotated queries, the pools' type
+  void* attn_ws = nullptr;      // and the attention workspace
+  int64_t attn_ws_bytes = 0;
   void* act_base = nullptr;     // one allocation for the buffers below
   float *h = nullptr, *xn = nullptr, *qkv = nullptr, *att = nullptr, *moe_out = nullptr;
   float *last = nullptr, *logits = nullptr, *part = nullptr;
@@ -860,7 +875,7 @@ void release(Decoder* D) {
   }
   if (D->lm_head != D->embed) cudaFree(D->lm_head);
   for (void* p : {(void*)D->embed, (void*)D->final_norm, (void*)D->rope_cos, (void*)D->rope_sin,
-                  (void*)D->kcache, (void*)D->vcache, D->act_base})
+                  (void*)D->kcache, (void*)D->vcache, D->act_base, D->q16, D->attn_ws})
     cudaFree(p);
   for (cudaEvent_t e : D->ev) cudaEventDestroy(e);
   if (D->cap) cudaStreamDestroy(D->cap);
@@ -1036,7 +1051,7 @@ int run_step(Decoder& D, const int32_t* tokens, int B, int T, float* logits, int
     const bool split = linear_tc(D, rows);  // producers write the hi / lo copies
     dec::add_rmsnorm_kernel<<<rows, dec::kNormThreads, 0, st>>>(
         D.h, l ? D.moe_out : nullptr, L.attn_norm, H, d.rms_eps, 1, 0, D.xn,
-        split ? D.xh : nullptr, split ? D.xl : nullptr);
+        split ? D.xh : nullptr, split ? D.xl : nullptr, nullptr, 0);
     DEC_CUDA(cudaGetLastError(), "norm launch");
     float* kc = D.kcache + (size_t)l * layer_kv;
     float* vc = D.vcache + (size_t)l * layer_kv;
@@ -1079,7 +1094,7 @@ int run_step(Decoder& D, const int32_t* tokens, int B, int T, float* logits, int
                      true, st, split)))
       return rc;
     dec::add_rmsnorm_kernel<<<rows, dec::kNormThreads, 0, st>>>(
-        D.h, nullptr, L.post_norm, H, d.rms_eps, 1, 0, D.xn, nullptr, nullptr);
+        D.h, nullptr, L.post_norm, H, d.rms_eps, 1, 0, D.xn, nullptr, nullptr, nullptr, 0);
     DEC_CUDA(cudaGetLastError(), "norm launch");
     if ((rc = record(D, 2 * l + 1, st))) return rc;
     if ((rc = gb_moe_forward(L.moe, D.xn, rows, D.moe_out, st))) return rc;
@@ -1090,7 +1105,7 @@ int run_step(Decoder& D, const int32_t* tokens, int B, int T, float* logits, int
   const bool split_head = linear_tc(D, B);
   dec::add_rmsnorm_kernel<<<B, dec::kNormThreads, 0, st>>>(
       D.h, D.moe_out, D.final_norm, H, d.rms_eps, T, T - 1, D.last,
-      split_head ? D.xh : nullptr, split_head ? D.xl : nullptr);
+      split_head ? D.xh : nullptr, split_head ? D.xl : nullptr, nullptr, 0);
   DEC_CUDA(cudaGetLastError(), "final norm launch");
   if ((rc = linear(D, D.last, B, H, D.lm_head, D.tc ? D.map_lm : nullptr, d.vocab, nullptr,
                    logits, d.vocab, false, st, split_head)))
@@ -1102,6 +1117,101 @@ int run_step(Decoder& D, const int32_t* tokens, int B, int T, float* logits, int
   }
   DEC_CUDA(cudaGetLastError(), "greedy token launch");
   return record(D, head_ev + 1, st);
+}
+
+// The buffers of paged forwards, on the first of them; the workspace's size is the
+// same for every batch of one head_dim, so a captured graph keeps its pointers.  Rows
+// of no sequence are never written, so the buffers start as zeros.
+int ensure_paged(Decoder& D, int64_t need, cudaStream_t st) {
+  int rc;
+  const size_t q_bytes = (size_t)D.rows_cap * D.att_w * 2;
+  if (!D.q16) {
+    if ((rc = dalloc((char**)&D.q16, q_bytes, "rotated queries"))) return rc;
+    DEC_CUDA(cudaMemsetAsync(D.q16, 0, q_bytes, st), "rotated queries");
+    DEC_CUDA(cudaMemsetAsync(D.att, 0, (size_t)D.rows_cap * D.att_w * 4, st), "attention rows");
+  }
+  if (!D.attn_ws) {
+    if ((rc = dalloc((char**)&D.attn_ws, (size_t)need, "attention workspace"))) return rc;
+    D.attn_ws_bytes = need;
+  }
+  return GB_OK;
+}
+
+// Enqueues one ragged forward over the batch's pages.
+int run_paged(Decoder& D, const int32_t* tokens, const gb_paged_batch* batch, void* const* k_pools,
+              void* const* v_pools, float* logits, int32_t* next, cudaStream_t st) {
+  const gb_decoder_desc& d = D.d;
+  const int H = d.hidden, nh = d.n_heads, nkv = d.n_kv_heads, hd = d.head_dim;
+  const int rows = batch->total_q, B = batch->n_seqs;
+  int rc;
+  dec::embed_kernel<<<rows, 256, 0, st>>>(tokens, D.embed, H, d.vocab, D.h, D.err);
+  DEC_CUDA(cudaGetLastError(), "embedding launch");
+  gb_rope_args ra{};
+  ra.struct_size = sizeof(ra);
+  ra.in_dtype = GB_DTYPE_F32;
+  ra.n_heads = nh;
+  ra.rot_dim = hd;
+  ra.q_dev = D.qkv;
+  ra.k_dev = D.qkv + (size_t)nh * hd;
+  ra.v_dev = D.qkv + (size_t)(nh + nkv) * hd;
+  ra.q_row_stride = ra.k_row_stride = ra.v_row_stride = D.qkv_w;
+  ra.q_head_stride = ra.k_head_stride = ra.v_head_stride = hd;
+  ra.q_out_dev = D.q16;
+  ra.out_row_stride = D.att_w;
+  ra.out_head_stride = hd;
+  ra.cos_dev = D.rope_cos;
+  ra.sin_dev = D.rope_sin;
+  ra.table_rows = d.max_seq_len;
+  gb_attn_args aa{};
+  aa.struct_size = sizeof(aa);
+  aa.n_heads = nh;
+  aa.out_dtype = GB_DTYPE_F32;
+  aa.scale = (float)(1.0 / sqrt((double)hd));
+  aa.q_dev = D.q16;
+  aa.out_dev = D.att;
+  aa.q_row_stride = aa.out_row_stride = D.att_w;
+  aa.q_head_stride = aa.out_head_stride = hd;
+  aa.workspace_dev = D.attn_ws;
+  aa.workspace_bytes = D.attn_ws_bytes;
+  const bool split = linear_tc(D, rows);
+  for (int l = 0; l < d.n_layers; ++l) {
+    DecLayer& L = D.layers[l];
+    dec::add_rmsnorm_kernel<<<rows, dec::kNormThreads, 0, st>>>(
+        D.h, l ? D.moe_out : nullptr, L.attn_norm, H, d.rms_eps, 1, 0, D.xn,
+        split ? D.xh : nullptr, split ? D.xl : nullptr, nullptr, 0);
+    DEC_CUDA(cudaGetLastError(), "norm launch");
+    if ((rc = linear(D, D.xn, rows, H, L.wqkv, D.tc ? L.map_qkv : nullptr, D.qkv_w, L.bqkv, D.qkv,
+                     D.qkv_w, false, st, split)))
+      return rc;
+    ra.k_pool_dev = k_pools[l];
+    ra.v_pool_dev = v_pools[l];
+    if ((rc = gb_paged_rope_append(batch, &ra, st))) return rc;
+    aa.k_pool_dev = k_pools[l];
+    aa.v_pool_dev = v_pools[l];
+    aa.sinks_dev = L.sinks;
+    aa.window = L.sliding ? d.sliding_window : 0;
+    if ((rc = gb_paged_attention(batch, &aa, st))) return rc;
+    if ((rc = linear(D, D.att, rows, D.att_w, L.wo, D.tc ? L.map_o : nullptr, H, L.bo, D.h, H, true,
+                     st)))
+      return rc;
+    dec::add_rmsnorm_kernel<<<rows, dec::kNormThreads, 0, st>>>(
+        D.h, nullptr, L.post_norm, H, d.rms_eps, 1, 0, D.xn, nullptr, nullptr, nullptr, 0);
+    DEC_CUDA(cudaGetLastError(), "norm launch");
+    if ((rc = gb_moe_forward(L.moe, D.xn, rows, D.moe_out, st))) return rc;
+  }
+  const bool split_head = linear_tc(D, B);
+  dec::add_rmsnorm_kernel<<<B, dec::kNormThreads, 0, st>>>(
+      D.h, D.moe_out, D.final_norm, H, d.rms_eps, 1, 0, D.last, split_head ? D.xh : nullptr,
+      split_head ? D.xl : nullptr, batch->q_start_dev, rows);
+  DEC_CUDA(cudaGetLastError(), "final norm launch");
+  if ((rc = linear(D, D.last, B, H, D.lm_head, D.tc ? D.map_lm : nullptr, d.vocab, nullptr, logits,
+                   d.vocab, false, st, split_head)))
+    return rc;
+  const int per_cta = dec::kArgmaxThreads * dec::kArgmaxPerThread;
+  dec::argmax_kernel<<<dim3((d.vocab + per_cta - 1) / per_cta, B), dec::kArgmaxThreads, 0, st>>>(
+      logits, d.vocab, D.am_slot, D.am_ticket, next, nullptr);
+  DEC_CUDA(cudaGetLastError(), "greedy token launch");
+  return GB_OK;
 }
 
 int check_positions(Decoder& D, int B, int T, int64_t pos) {
@@ -1211,6 +1321,36 @@ int gb_decoder_forward(gb_decoder* h, const int32_t* tokens_dev, int32_t B, int3
   D.pos = pos + T;
   D.batch = B;
   return GB_OK;
+}
+
+int gb_decoder_forward_paged(gb_decoder* h, const int32_t* tokens_dev, const gb_paged_batch* batch,
+                             void* const* k_pools, void* const* v_pools, float* logits_dev,
+                             int32_t* next_dev, void* stream) {
+  using namespace gb;
+  if (!h) return set_error(GB_ERR_INVALID_ARG, "handle is null");
+  Decoder& D = *h->D;
+  if (!tokens_dev || !k_pools || !v_pools)
+    return set_error(GB_ERR_INVALID_ARG, "tokens_dev, k_pools and v_pools must not be null");
+  DevScope ds(D.device);
+  int64_t ws = 0;
+  int rc = gb_paged_attention_workspace(batch, D.d.n_heads, &ws);  // checks the batch
+  if (rc) return rc;
+  if (batch->head_dim != D.d.head_dim || batch->n_kv_heads != D.d.n_kv_heads)
+    return set_error(GB_ERR_INVALID_ARG, "the batch's head_dim %d and n_kv_heads %d are not the model's %d, %d",
+                     batch->head_dim, batch->n_kv_heads, D.d.head_dim, D.d.n_kv_heads);
+  if (batch->n_seqs > D.d.max_batch || batch->total_q > D.rows_cap)
+    return set_error(GB_ERR_INVALID_ARG, "%d sequences with %d rows: at most %d and %lld",
+                     batch->n_seqs, batch->total_q, D.d.max_batch, (long long)D.rows_cap);
+  for (int l = 0; l < D.d.n_layers; ++l)
+    if (!k_pools[l] || !v_pools[l])
+      return set_error(GB_ERR_INVALID_ARG, "layer %d: a pool is null", l);
+  if (logits_dev && (reinterpret_cast<uintptr_t>(logits_dev) & 15))
+    return set_error(GB_ERR_INVALID_ARG, "logits_dev must be 16-byte aligned");
+  if (batch->n_seqs == 0 || batch->total_q == 0) return GB_OK;
+  if ((rc = ensure_paged(D, ws, static_cast<cudaStream_t>(stream)))) return rc;
+  D.timed = false;
+  return run_paged(D, tokens_dev, batch, k_pools, v_pools, logits_dev ? logits_dev : D.logits,
+                   next_dev ? next_dev : D.next, static_cast<cudaStream_t>(stream));
 }
 
 int gb_decoder_generate(gb_decoder* h, const int32_t* tokens_dev, int32_t B, int64_t pos,

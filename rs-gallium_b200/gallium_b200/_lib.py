@@ -290,6 +290,8 @@ SIGNATURES = {
     "gb_paged_attention_workspace": (c_int, [POINTER(PagedBatchDesc), c_int32, POINTER(c_int64)]),
     "gb_paged_copy": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p,
                               c_int32, c_void_p]),
+    "gb_decoder_forward_paged": (c_int, [c_void_p, c_void_p, POINTER(PagedBatchDesc), POINTER(c_void_p),
+                                         POINTER(c_void_p), c_void_p, c_void_p, c_void_p]),
     "gb_sample": (c_int, [POINTER(SampleArgs), c_void_p]),
     "gb_nccl_unique_id": (c_int, [POINTER(c_uint8)]),
     "gb_last_error": (c_char_p, []),

@@ -165,6 +165,43 @@ class GptOssQ:
         self.pos = pos + n_steps
         return out
 
+    def forward_paged(self, token_ids, batch, k_pools, v_pools, check_status: bool = True):
+        """One forward of a ragged batch (paged.PagedBatch) over paged caches:
+        token_ids (total_q,) int32, k_pools / v_pools a tensor [n_layers, n_pages,
+        page_size, n_kv_heads, head_dim] each or a sequence of n_layers pools.
+        The new tokens' keys and values go into the pools; returns the (n_seqs,
+        vocab) f32 logits of each sequence's last new token and leaves the greedy
+        tokens in self.last_next."""
+        import torch
+
+        dev = torch.device("cuda", self.device)
+        if len(k_pools) != self.n_layers or len(v_pools) != self.n_layers:
+            raise _lib.GalliumError(_lib.GB_ERR_INVALID_ARG, f"{self.n_layers} K and V pools are needed")
+        if batch.device != dev:
+            raise _lib.GalliumError(_lib.GB_ERR_INVALID_ARG, f"the batch is on {batch.device}, the model on {dev}")
+        t = torch.as_tensor(np.asarray(token_ids) if not torch.is_tensor(token_ids) else token_ids)
+        t = t.to(device=dev, dtype=torch.int32).contiguous().reshape(-1)
+        if t.shape[0] != batch.total_q:
+            raise _lib.GalliumError(_lib.GB_ERR_INVALID_ARG,
+                                    f"{t.shape[0]} tokens, the batch has {batch.total_q} rows")
+        ptrs = [(ctypes.c_void_p * self.n_layers)() for _ in range(2)]
+        for l in range(self.n_layers):
+            batch._set_pool(k_pools[l], v_pools[l])
+            if l and batch._pool != first:
+                raise _lib.GalliumError(_lib.GB_ERR_INVALID_ARG, f"layer {l}'s pools differ from layer 0's")
+            first = batch._pool
+            ptrs[0][l], ptrs[1][l] = k_pools[l].data_ptr(), v_pools[l].data_ptr()
+        n = batch._desc.n_seqs
+        logits = torch.empty((n, self.vocab), dtype=torch.float32, device=dev)
+        nxt = torch.empty((n,), dtype=torch.int32, device=dev)
+        check(self._lib.gb_decoder_forward_paged(self._h, t.data_ptr(), batch._ref, ptrs[0], ptrs[1],
+                                                 logits.data_ptr(), nxt.data_ptr(), self._stream()))
+        if check_status:
+            check(self._lib.gb_decoder_device_status(self._h, self._stream()))
+            batch.check()
+        self.last_next = nxt
+        return logits
+
     def reset(self) -> None:
         check(self._lib.gb_decoder_reset(self._h))
         self.pos = 0
