@@ -8,20 +8,29 @@
 //
 // The kept set is a prefix of the tokens in order (falling logit, rising id).
 // The short way, for a filtered row:
-//   1. a histogram of counts, bins of 1/32 of a nat of the scaled logits on an
-//      absolute grid (so that it needs no common maximum), tells from which bin
-//      on no token can be kept;
-//   2. the candidates before it, when they are at most kCand, go to the
+//   1. a histogram, bins of 1/32 of a nat of the scaled logits on an absolute grid
+//      (so that it needs no common maximum), tells from which bin on no token can be
+//      kept: of counts, or, where top-p is over the whole row, of masses (a token's
+//      weight relative to its bin's largest in 16 bits), whose sums give the row's
+//      total weight to some 2^-15 as well;
+//   2. the candidates before that bin, when they are at most kCand, go to the
 //      cluster's first CTA, which sorts them, applies the filters exactly,
-//      sorts the kept ones by id and draws.
-// Where top-p is over the whole row, its total weight is summed in f32: that
-// decides the cut unless the cut lies within kSlack of a border.
+//      sorts the kept ones by id and draws (unless top-p's cut lies so near a border
+//      that the total does not decide it).
+// The middle way, for top-p over many tokens: the mass histogram gives a window of a
+// bin or less for the cut, one pass sums the exact weights (for the cut and for the
+// draw), and the first CTA looks for the cut among the window's tokens.
 // The long way, for what remains: each filter is the search for the element at
 // which a running sum -- of ones for top-k, of weights for top-p -- reaches a
 // target, by histograms of 1024 bins (the second and later ones over the bits
 // of the logits, down to a single value, where equal logits go by id); then all
 // kept weights are summed in order of id.  An unfiltered row takes that last
 // step alone.
+//
+// Measured, f32 rows of 201088: 15 us for one row with all filters, 35 where top-p
+// keeps thousands; 128 rows 82 and 205 us, without filters 85, greedy 49 (2.1 TB/s).
+// The rows are bound by instructions between some ten cluster barriers, not by memory:
+// two CTAs of 113 KB on an SM take turns at loading and computing.
 //
 // Weights are e^z 2^45, z = (x - max) / T <= 0, rounded to integers: their sums
 // are exact, so neither the order of the sums nor that of the atomics matters.
@@ -47,11 +56,11 @@ constexpr int kBins = 1024;
 constexpr int kList = 512;          // elements of a bin resolved in one step
 constexpr int kCand = 1024;         // candidates sorted by one CTA: two per thread
 constexpr float kGrid = 32.0f;      // bins per nat
-// Bound of the relative error of an f32 sum of weights: three roundings of an
-// argument of up to 46 (2^z) move a weight by 46 ln 2 x 3 x 2^-24 = 5.7e-6, ex2
-// itself by 2^-22, and sums in parts of at most 98, 21 and 8 terms by 127 x
-// 2^-24 = 7.6e-6; together below 1.4e-5.
-constexpr double kSlack = 1.0 / 32768;
+constexpr float kStep = 1.4426950408889634f / kGrid;  // a bin in powers of two
+// Masses: a token's weight relative to its bin's largest, in units of 2^-16, so that a
+// slice of at most 50000 tokens stays below 2^32.
+constexpr float kUnit = 65536.0f;
+constexpr unsigned kLeastMass = 63500;  // no mass is below: e^-1/32 2^16 = 63520, less the roundings
 constexpr int kMaxVocab = 400000;   // 8 x 200 KB of shared memory
 constexpr int kOneBits = 45;        // the largest weight is 2^45: 400000 of them stay below 2^64
 constexpr double kNoWeight = -32.0; // e^z 2^45 rounds to 0 below -46 ln 2 = -31.9
@@ -80,6 +89,7 @@ struct alignas(16) Shared {
     uint16_t count[kBins];  // the short way's histogram (a slice is below 2^16)
     uint32_t count2[kBins / 2];
     uint32_t lo[kBins];     // a bin's sum, low words (shared memory adds 32 bits natively)
+    unsigned long long part[kThreads];  // weights added to the threads' parts of the slice
     Item all[kList];        // the cluster's elements of the crossing bin, once the bins are read
   };
   union {
@@ -96,11 +106,13 @@ struct alignas(16) Shared {
   uint64_t warp_sum[kWarps];
   float warp_sum_f[kWarps];
   uint64_t ex64[2][kMaxCluster];  // exchange slots, by parity of the exchange
+  uint64_t ex64b[2][kMaxCluster];
   uint32_t ex32[2][kMaxCluster];
   uint64_t above;
   int bin, n_list, answer;
   int bin_k, bin_p, n_cand;  // the short way: bins that hold the cuts, candidates
   uint32_t key_lo, key_hi;
+  float win_lo, win_hi;      // the window of cut_window, in grid units
 };
 
 static_assert(sizeof(Shared) % 16 == 0, "the slice behind Shared is read as float4");
@@ -152,6 +164,77 @@ __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int o) {
   return __shfl_xor_sync(kFullMask, (unsigned long long)v, o);
 }
 
+// The inclusive sums of the CTA's values, two in a row per thread; total: all.
+template <typename V>
+__device__ __forceinline__ void block_scan2(Shared& sh, V (&v)[2], V* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v[1] += v[0];
+  V inc = v[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V t = __shfl_up_sync(kFullMask, inc, o);
+    if (lane >= o) inc += t;
+  }
+  __syncthreads();
+  if (lane == 31) sh.warp_sum[warp] = inc;
+  __syncthreads();
+  // the warps' sums, scanned by every warp for itself
+  V ws = lane < kWarps ? (V)sh.warp_sum[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const V t = __shfl_up_sync(kFullMask, ws, o);
+    if (lane >= o) ws += t;
+  }
+  const V all = __shfl_sync(kFullMask, ws, kWarps - 1);
+  const V upto = __shfl_sync(kFullMask, ws, (warp + 31) & 31);
+  const V before = inc - v[1] + (warp ? upto : 0);
+  v[0] += before;
+  v[1] += before;
+  *total = all;
+}
+
+// The grid bin of a logit: a non-decreasing function of v (each rounding is
+// monotone, 0 x inf converts to 0, between the ends).
+__device__ __forceinline__ int grid_of(float v, float scale) {
+  const int g = __float2int_rd(v * scale);
+  return max(-(1 << 28), min(1 << 28, g));
+}
+
+// The mass of a logit in its grid bin.
+__device__ __forceinline__ uint32_t mass_of(float v, float scale, int bin) {
+  const float frac = fminf(fmaxf(v * scale - (float)bin, 0.0f), 1.0f);
+  return (uint32_t)__float2int_rn(exp2f((frac - 1.0f) * kStep) * kUnit);
+}
+
+// The relative error of a weight of a mass histogram, and of their sums: half a unit,
+// and the roundings of v * scale and of scale itself, 2^-23 of it each for v and for
+// the largest logit, over 32 bins per nat.
+__device__ __forceinline__ float mass_slack(float top, float scale) {
+  return 1.0f / 65536.0f + (fabsf(top * scale) + (float)kBins) * (1.0f / (1 << 27));
+}
+
+// A bin's mass on the scale of all bins: 2^32 is the upper edge of bin 0.
+__device__ __forceinline__ unsigned long long scaled_mass(uint64_t m, int j) {
+  return (unsigned long long)((double)m * (double)(exp2f(-(float)j * kStep) * 65536.0f));
+}
+
+// The window around the cut at which the running mass reaches `want`, in grid units:
+// the bin with its slack, or of a bin of many the part where the cut is as a rule
+// (n tokens at random are off by half their root).  v: the bin's scaled mass, before:
+// that of the bins above, count: its tokens.
+__device__ __forceinline__ void set_window(Shared& sh, int bin, float count, double v, double before,
+                                           double want, double all) {
+  const float slack = (float)(1e-5 * all / v);
+  float hi = (float)(bin + 1), lo = (float)bin;
+  if (count > 900.0f) {
+    const float at = hi - (float)((want - before) / v), half = 2.5f * rsqrtf(count);
+    lo = at - half;
+    hi = at + half;
+  }
+  sh.win_lo = lo - slack;
+  sh.win_hi = hi + slack;
+}
+
 struct Row {
   cg::cluster_group cl;
   Shared& sh;
@@ -195,14 +278,15 @@ struct Row {
     }
   }
 
-  // Every CTA's value, to be read from ex64[parity] / ex32[parity] until the
+  // Every CTA's values, to be read from ex64 / ex32 / ex64b[parity] until the
   // exchange after the next one.
-  __device__ __forceinline__ int exchange(uint64_t a, uint32_t b) {
+  __device__ __forceinline__ int exchange(uint64_t a, uint32_t b, uint64_t c = 0) {
     const int par = exchanges++ & 1;
     if (threadIdx.x < ranks) {
       Shared* o = cl.map_shared_rank(&sh, threadIdx.x);
       o->ex64[par][rank] = a;
       o->ex32[par][rank] = b;
+      o->ex64b[par][rank] = c;
     }
     cl.sync();
     return par;
@@ -467,16 +551,197 @@ struct Row {
     }
     cut_tie(lo, need);
   }
+
+  // The window of top-p's cut over the tokens that top-k kept, by a mass histogram.
+  __device__ bool find_window(float p, float scale) {
+    const int tid = threadIdx.x, top_bin = grid_of(top, scale);
+    __syncthreads();
+    for (int j = tid; j < kBins; j += kThreads) sh.lo[j] = 0;
+    if (tid == 0) sh.win_hi = -INFINITY;
+    __syncthreads();
+    each([&](float v, int id) {
+      const int b = grid_of(v, scale), j = top_bin - b;
+      if (j < kBins && kept(key_of(v), id)) atomicAdd(&sh.lo[j], mass_of(v, scale, b));
+    });
+    cl.sync();
+    const int j0 = 2 * tid;
+    uint64_t m[2] = {0, 0};
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)
+      if (r < ranks) {
+        const uint2 got = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh, r)->lo + j0);
+        m[0] += got.x;
+        m[1] += got.y;
+      }
+    unsigned long long v[2], inc[2], all;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v[e] = inc[e] = scaled_mass(m[e], j0 + e);
+    block_scan2(sh, inc, &all);
+    const double want = (double)p * (double)all;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if ((double)(inc[e] - v[e]) < want && want <= (double)inc[e])
+        set_window(sh, top_bin - (j0 + e), (float)m[e] / kUnit, (double)v[e], (double)(inc[e] - v[e]), want,
+                   (double)all);
+    __syncthreads();
+    return sh.win_hi > -INFINITY;
+  }
+
+  // Top-p's cut over the kept tokens with one exact pass (the middle way): sums the
+  // exact weights of all and of those before the window, and lists the window's tokens
+  // for the first CTA, which finds the cut among them.  The exact sums show whether the
+  // cut lies in the window: when it does not (or the window's tokens are too many),
+  // false, and nothing has changed.  mine: the weight, of at least min_w each, of the
+  // tokens kept in the slice's part [i0, i1) that this thread sums for the draw.
+  __device__ bool cut_window(float p, float scale, int part, int i0, int i1, uint64_t min_w, uint64_t& mine) {
+    const int tid = threadIdx.x;
+    const float win_lo = sh.win_lo, win_hi = sh.win_hi;
+    if (tid == 0) sh.n_list = 0;
+    __syncthreads();
+    uint64_t sum = 0, above = 0, draw = 0;
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) {
+      const float v = x[i];
+      const uint32_t k = key_of(v);
+      const bool in = kept(k, base + i);
+      const uint64_t w = in ? weight(v) : 0;
+      const float y = v * scale;
+      sum += w;
+      above += y > win_hi ? w : 0;
+      draw += y > win_hi && w >= min_w ? w : 0;
+      if (in && y <= win_hi && y >= win_lo) {
+        const int s = atomicAdd(&sh.n_list, 1);
+        if (s < kCand) sh.cand[s] = ((uint64_t)k << 32) | (uint32_t)~(base + i);
+      }
+    }
+    sum = block_sum(sum);
+    above = block_sum(above);
+    int par = exchange(sum, (uint32_t)sh.n_list, above);
+    uint64_t total = 0;
+    above = 0;
+    int count = 0, before_me = 0;
+    for (int r = 0; r < ranks; ++r) {
+      total += sh.ex64[par][r];
+      above += sh.ex64b[par][r];
+      if (r < rank) before_me += (int)sh.ex32[par][r];
+      count += (int)sh.ex32[par][r];
+    }
+    const double ceiled = ceil((double)p * (double)total);
+    uint64_t target = (uint64_t)ceiled;
+    target = target < 1 ? 1 : target > total ? total : target;
+    if (above >= target || count > kCand) return false;
+    const int n_mine = sh.n_list;
+    if (rank != 0) {
+      Shared* o = cl.map_shared_rank(&sh, 0);
+      for (int i = tid; i < n_mine; i += kThreads) o->cand[before_me + i] = sh.cand[i];
+    }
+    cl.sync();
+    uint64_t answer = 0;
+    uint32_t found = 0;
+    if (rank == 0) found = find_cut(count, above, target, answer);
+    par = exchange(answer, found);
+    if (!sh.ex32[par][0]) return false;
+    cut_key = (uint32_t)(sh.ex64[par][0] >> 32);
+    cut_idx = (int)(uint32_t)sh.ex64[par][0];
+    // the window's kept tokens, to the threads whose parts they are of
+    sh.part[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n_mine; i += kThreads) {
+      const uint32_t k = (uint32_t)(sh.cand[i] >> 32);
+      const int id = (int)~(uint32_t)sh.cand[i];
+      if (kept(k, id)) {
+        const uint64_t w = weight(logit_of(k));
+        if (w >= min_w) atomicAdd(&sh.part[(id - base) / part], (unsigned long long)w);
+      }
+    }
+    __syncthreads();
+    mine = draw + sh.part[tid];
+    return true;
+  }
+
+  // Of the n tokens in sh.cand, the one at which above + the weights up to it (in
+  // order) reach target: its key and id in answer.  0: they do not.
+  __device__ uint32_t find_cut(int n, uint64_t above, uint64_t target, uint64_t& answer) {
+    uint32_t key[2] = {0, 0}, id[2] = {0, 0};
+    uint64_t w[2] = {0, 0};
+    uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = threadIdx.x + e * kThreads;
+      if (i < n) {
+        key[e] = (uint32_t)(sh.cand[i] >> 32);
+        id[e] = ~(uint32_t)sh.cand[i];
+        w[e] = weight(logit_of(key[e]));
+        lo = min(lo, key[e]);
+        hi = max(hi, key[e]);
+      }
+    }
+    if (above + block_sum(w[0] + w[1]) < target) return 0;
+    lo = __reduce_min_sync(kFullMask, lo);
+    hi = __reduce_max_sync(kFullMask, hi);
+    if (threadIdx.x == 0) {
+      sh.key_lo = 0xffffffffu;
+      sh.key_hi = 0;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) {
+      atomicMin(&sh.key_lo, lo);
+      atomicMax(&sh.key_hi, hi);
+    }
+    __syncthreads();
+    lo = sh.key_lo;
+    hi = sh.key_hi;
+    // The largest key from which on the weights reach the target, by histograms of
+    // kThreads bins over the keys' span, a bin per thread: low words, then high words.
+    while (lo < hi) {
+      int shift = 0;
+      while (((hi - lo) >> shift) >= (uint32_t)kThreads) ++shift;
+      sh.lo[threadIdx.x] = sh.lo[kThreads + threadIdx.x] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (w[e] && key[e] >= lo && key[e] <= hi) {
+          const int j = (hi - key[e]) >> shift;
+          const uint32_t l = (uint32_t)w[e], old = atomicAdd(&sh.lo[j], l);
+          const uint32_t h = (uint32_t)(w[e] >> 32) + (old + l < old ? 1u : 0u);
+          if (h) atomicAdd(&sh.lo[kThreads + j], h);
+        }
+      __syncthreads();
+      const uint64_t v = (uint64_t)sh.lo[threadIdx.x] | ((uint64_t)sh.lo[kThreads + threadIdx.x] << 32);
+      unsigned long long inc[2] = {v, 0}, all;
+      block_scan2(sh, inc, &all);
+      const uint64_t before = above + inc[0] - v;
+      if (before < target && target <= before + v) {  // one thread
+        sh.bin = threadIdx.x;
+        sh.above = before;
+      }
+      __syncthreads();
+      const uint32_t edge = hi - ((uint32_t)sh.bin << shift), width = (1u << shift) - 1;
+      above = sh.above;
+      lo = edge - lo > width ? edge - width : lo;
+      hi = edge;
+    }
+    // equal logits, by id: each weighs the same
+    const uint64_t one = weight(logit_of(lo));
+    const uint64_t need = (target - above + one - 1) / one;  // one > 0: they reach the target
+    const bool is0 = key[0] == lo && threadIdx.x < n, is1 = key[1] == lo && threadIdx.x + kThreads < n;
+    uint32_t first = 0, last = 0x7fffffffu;
+    const uint64_t same = block_sum(((uint64_t)is0 + is1) << 40 | (is0 ? id[0] : 0) + (is1 ? id[1] : 0));
+    if (same >> 40 == 1) {
+      first = (uint32_t)same;  // the only one
+    } else {
+      while (first < last) {
+        const uint32_t mid = first + (last - first) / 2;
+        if (block_sum((uint64_t)(is0 && id[0] <= mid) + (is1 && id[1] <= mid)) >= need) last = mid;
+        else first = mid + 1;
+      }
+    }
+    answer = ((uint64_t)lo << 32) | first;
+    return 1;
+  }
 };
 
 // ---- the short way -----------------------------------------------------------
-
-// The grid bin of a logit: a non-decreasing function of v (each rounding is
-// monotone, 0 x inf converts to 0, between the ends).
-__device__ __forceinline__ int grid_of(float v, float scale) {
-  const int g = __float2int_rd(v * scale);
-  return max(-(1 << 28), min(1 << 28, g));
-}
 
 struct Settings {
   bool use_k, use_p, use_min;
@@ -504,41 +769,12 @@ __device__ __forceinline__ void sort_desc(uint64_t* a, int m) {
   __syncthreads();
 }
 
-// The inclusive sums of the CTA's values, two in a row per thread; total: all.
-template <typename V>
-__device__ __forceinline__ void block_scan2(Shared& sh, V (&v)[2], V* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  v[1] += v[0];
-  V inc = v[1];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const V t = __shfl_up_sync(kFullMask, inc, o);
-    if (lane >= o) inc += t;
-  }
-  __syncthreads();
-  if (lane == 31) sh.warp_sum[warp] = inc;
-  __syncthreads();
-  // the warps' sums, scanned by every warp for itself
-  V ws = lane < kWarps ? (V)sh.warp_sum[lane] : 0;
-#pragma unroll
-  for (int o = 1; o < kWarps; o <<= 1) {
-    const V t = __shfl_up_sync(kFullMask, ws, o);
-    if (lane >= o) ws += t;
-  }
-  const V all = __shfl_sync(kFullMask, ws, kWarps - 1);
-  const V upto = __shfl_sync(kFullMask, ws, (warp + 31) & 31);
-  const V before = inc - v[1] + (warp ? upto : 0);
-  v[0] += before;
-  v[1] += before;
-  *total = all;
-}
-
 __device__ __forceinline__ int pow2_from(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
 
 // The same for few candidates (n <= kFew), a thread each: sums over the pairs
 // instead of sorts, three barriers in all.
 constexpr int kFew = 128;
-__device__ bool finish_few(Row& R, const Settings& st, int n, double approx_total, bool all_min, float u,
+__device__ bool finish_few(Row& R, const Settings& st, int n, double approx_total, double slack, bool all_min, float u,
                            int32_t* token, float* logprob) {
   Shared& sh = R.sh;
   const int t = threadIdx.x;
@@ -569,8 +805,8 @@ __device__ bool finish_few(Row& R, const Settings& st, int n, double approx_tota
     double lo = INFINITY, hi = INFINITY;
     if (st.use_p) {
       const double z = (double)st.p * (st.use_k ? (double)sh.above : approx_total * (double)(1ull << kOneBits));
-      lo = st.use_k ? z : z * (1.0 - kSlack);
-      hi = st.use_k ? z : z * (1.0 + kSlack);
+      lo = st.use_k ? z : z * (1.0 - slack);
+      hi = st.use_k ? z : z * (1.0 + slack);
     }
     const bool big = !st.use_min || (double)mine >= (double)st.least * (double)(1ull << kOneBits);
     kept = rank == 0 || (big && (double)before < lo);
@@ -604,11 +840,11 @@ __device__ bool finish_few(Row& R, const Settings& st, int n, double approx_tota
 // row's weight in units of the largest, where top-p is over the whole row.
 // all_min: every token that min_p keeps is among them.  false: the cut is too
 // close to a border for that total.
-__device__ bool finish(Row& R, const Settings& st, int n, double approx_total, bool all_min, float u,
+__device__ bool finish(Row& R, const Settings& st, int n, double approx_total, double slack, bool all_min, float u,
                        int32_t* token, float* logprob) {
   Shared& sh = R.sh;
   const int t = threadIdx.x;
-  if (n <= kFew) return finish_few(R, st, n, approx_total, all_min, u, token, logprob);
+  if (n <= kFew) return finish_few(R, st, n, approx_total, slack, all_min, u, token, logprob);
   int m = pow2_from(n);
   for (int i = n + t; i < m; i += kThreads) sh.cand[i] = 0;
   sort_desc(sh.cand, m);
@@ -628,8 +864,8 @@ __device__ bool finish(Row& R, const Settings& st, int n, double approx_total, b
       lo = hi = (double)st.p * (double)all;
     } else {
       const double z = (double)st.p * approx_total * (double)(1ull << kOneBits);
-      lo = z * (1.0 - kSlack);
-      hi = z * (1.0 + kSlack);
+      lo = z * (1.0 - slack);
+      hi = z * (1.0 + slack);
     }
   }
   const double min_w = st.use_min ? (double)st.least * (double)(1ull << kOneBits) : 0.0;
@@ -741,11 +977,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   const bool filtered = !greedy && (st.use_k || st.use_p || st.use_min);
   float u = a.u[row];
   u = u > 0.0f ? u : 0.0f;
-  for (int j = tid; j < kBins / 2; j += kThreads) sh.count2[j] = 0;
+  for (int j = tid; j < kBins; j += kThreads) sh.lo[j] = 0;
   if (tid < 32) sh.exp_table[tid] = __longlong_as_double((long long)kExpTable[tid]);
   if (tid == 0) {
     sh.n_list = 0;
     sh.bin_k = sh.bin_p = 0x7fffffff;
+    sh.win_hi = -INFINITY;
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
@@ -755,31 +992,23 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.warp_sum_f[w]);
   Row R{cl, sh, xs, n, base, rank, ranks, 0, 0.0f, 0.0, 0.0f, 0u, 0x7fffffff};
 
-  // The short way's histogram, from the slice's own largest logit down, and
-  // its weight in f32 where top-p is over the whole row.
+  // The short way's histogram, from the slice's own largest logit down: of masses
+  // where top-p is over the whole row, else of counts.
   const float grid = kGrid / t;
   const int my_top = grid_of(top, grid);
   const bool whole_p = filtered && st.use_p && !st.use_k;
-  float z_sum = 0.0f;
-  if (filtered) {
-    const float c = 1.4426950408889634f / t;
-    float part = 0.0f;
+  if (whole_p) {
+    R.each([&](float v, int) {
+      const int b = grid_of(v, grid), j = my_top - b;
+      if (j < kBins) atomicAdd(&sh.lo[j], mass_of(v, grid, b));
+    });
+  } else if (filtered) {
     R.each([&](float v, int) {
       const int b = my_top - grid_of(v, grid);
       if (b < kBins) atomicAdd(&sh.count2[b >> 1], 1u << ((b & 1) * 16));
-      if (whole_p) part += exp2f((v - top) * c);
     });
-    if (whole_p) {
-#pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) part += __shfl_xor_sync(kFullMask, part, o);
-      __syncthreads();
-      if (lane == 0) sh.warp_sum_f[warp] = part;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) z_sum += sh.warp_sum_f[w];
-    }
   }
-  int par = R.exchange(__float_as_uint(z_sum), __float_as_uint(top));
+  int par = R.exchange(0, __float_as_uint(top));
   for (int r = 0; r < ranks; ++r) top = fmaxf(top, __uint_as_float(sh.ex32[par][r]));
   R.top = top;
 
@@ -809,60 +1038,72 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   R.inv_t = 1.0 / (double)t;
   R.bin_scale = 32.0f / t;
 
-  if (filtered && top < INFINITY) {
+  const float slack = mass_slack(top, grid);
+  if (filtered && top < INFINITY && (!whole_p || slack < 0.01f)) {
     const int top_bin = grid_of(top, grid);
-    // the cluster's counts, two bins per thread, every load before the first is used
+    // the cluster's bins, two per thread, every load before the first is used
     const int j0 = 2 * tid;
     uint32_t got[2 * kMaxCluster];
-    double total = 0.0;
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r) {
       got[2 * r] = got[2 * r + 1] = 0;
       if (r < ranks) {
-        const float rt = __uint_as_float(sh.ex32[par][r]);
-        const int j = j0 - (top_bin - grid_of(rt, grid));
+        const int j = j0 - (top_bin - grid_of(__uint_as_float(sh.ex32[par][r]), grid));
         const Shared* o = cl.map_shared_rank(&sh, r);
-        // bins j and j + 1: one word, or the halves of two
+        // bins j and j + 1: of counts, one word, or the halves of two
         if (j + 1 >= 0) {
-          const int q = (j + 1) >> 1;
-          got[2 * r + 1] = o->count2[q];
-          if (j >= 0 && (j & 1)) got[2 * r] = o->count2[q - 1];
+          const int q = whole_p ? j + 1 : (j + 1) >> 1;
+          got[2 * r + 1] = o->lo[q];
+          if (j >= 0 && (whole_p || (j & 1))) got[2 * r] = o->lo[q - 1];
         }
-        if (whole_p && rt > -INFINITY)
-          total += (double)__uint_as_float((uint32_t)sh.ex64[par][r]) *
-                   (double)exp2f((rt - top) * (1.4426950408889634f / t));
       }
     }
-    uint32_t cnt[2] = {0, 0}, inc[2], all;
-#pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) {
-      if (r < ranks) {
-        const float rt = __uint_as_float(sh.ex32[par][r]);
-        const int j = j0 - (top_bin - grid_of(rt, grid));
-        const bool odd = j & 1;
-        cnt[0] += odd ? got[2 * r] >> 16 : j >= 0 ? got[2 * r + 1] & 0xffffu : 0u;
-        cnt[1] += odd ? got[2 * r + 1] & 0xffffu : got[2 * r + 1] >> 16;
-      }
-    }
-    inc[0] = cnt[0];
-    inc[1] = cnt[1];
-    block_scan2(sh, inc, &all);
-    if (st.use_k) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (inc[e] - cnt[e] < (uint32_t)st.k && (uint32_t)st.k <= inc[e]) sh.bin_k = j0 + e;
-    }
+    int upto[2];  // tokens up to the bin's end; where masses are summed, a bound of them
+    double total = 0.0;
     if (whole_p) {
-      // each bin's weight from below, in units of 2^-30: where it reaches top_p, the cut lies before
-      unsigned long long low[2], lows[2], low_all;
+      uint64_t m[2] = {0, 0};
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        low[e] = lows[e] = cnt[e] * (uint64_t)(exp2f(-(float)(j0 + e + 1) * (1.4426950408889634f / kGrid)) * 1073741824.0f);
-      block_scan2(sh, lows, &low_all);
-      const double want = (double)st.p * total * (1.0 + kSlack) * 1073741824.0;
+      for (int r = 0; r < kMaxCluster; ++r) {
+        m[0] += got[2 * r];
+        m[1] += got[2 * r + 1];
+      }
+      unsigned long long inc[2] = {m[0], m[1]}, all;
+      block_scan2(sh, inc, &all);
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if ((double)(lows[e] - low[e]) < want && want <= (double)lows[e]) sh.bin_p = j0 + e;
+      for (int e = 0; e < 2; ++e) upto[e] = (int)min(inc[e] / kLeastMass, 1ull << 24) + 1;
+      unsigned long long v[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) v[e] = inc[e] = scaled_mass(m[e], j0 + e);
+      block_scan2(sh, inc, &all);
+      // in units of the largest weight
+      total = (double)all * (double)(exp2f(((float)(top_bin + 1) - top * grid) * kStep) * (1.0f / 4294967296.0f));
+      const double cut = (double)st.p * (double)all, want = cut * (1.0 + 4.0 * (double)slack);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const double before = (double)(inc[e] - v[e]);
+        if (before < want && want <= (double)inc[e]) sh.bin_p = j0 + e;
+        if (before < cut && cut <= (double)inc[e])
+          set_window(sh, top_bin - (j0 + e), (float)m[e] / kUnit, (double)v[e], before, cut, (double)all);
+      }
+    } else {
+      uint32_t cnt[2] = {0, 0}, inc[2], all;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        if (r < ranks) {
+          const int j = j0 - (top_bin - grid_of(__uint_as_float(sh.ex32[par][r]), grid));
+          const bool odd = j & 1;
+          cnt[0] += odd ? got[2 * r] >> 16 : j >= 0 ? got[2 * r + 1] & 0xffffu : 0u;
+          cnt[1] += odd ? got[2 * r + 1] & 0xffffu : got[2 * r + 1] >> 16;
+        }
+      }
+      inc[0] = cnt[0];
+      inc[1] = cnt[1];
+      block_scan2(sh, inc, &all);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        upto[e] = (int)inc[e];
+        if (st.use_k && inc[e] - cnt[e] < (uint32_t)st.k && (uint32_t)st.k <= inc[e]) sh.bin_k = j0 + e;
+      }
     }
     __syncthreads();
     // the last bin that min_p keeps a token of, with room for the roundings
@@ -878,7 +1119,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     if (j < kBins) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (j0 + e == j) sh.n_cand = (int)inc[e];
+        if (j0 + e == j) sh.n_cand = upto[e];
       __syncthreads();
       const int n_cand = sh.n_cand;
       if (n_cand <= kCand) {
@@ -904,7 +1145,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         cl.sync();
         bool done = true;
         if (rank == 0)
-          done = finish(R, st, min(sh.n_list, kCand), total, all_min, u, a.token + row,
+          done = finish(R, st, min(sh.n_list, kCand), total, (double)slack, all_min, u, a.token + row,
                         a.logprob ? a.logprob + row : nullptr);
         if (!whole_p) return;  // nothing of another CTA is read any more
         par = R.exchange(0, done);
@@ -919,7 +1160,20 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     R.each([&](float v, int) { atomicAdd(&sh.lo[R.bin_of(v)], 1u); });
     R.select<false>((uint64_t)st.k);
   }
-  if (st.use_p) {
+  // A thread sums a contiguous part of the slice for the draw (an odd number of
+  // elements: no bank conflicts), so the parts are in order of id.
+  const int part = ((n + kThreads - 1) / kThreads) | 1;
+  const int i0 = min(tid * part, n), i1 = min(i0 + part, n);
+  // weights are whole numbers: at least `least` of the largest is at least this
+  const uint64_t min_w = st.use_min ? (uint64_t)ceil((double)st.least * (double)(1ull << kOneBits)) : 0;
+  uint64_t mine = 0;
+  // The middle way: the window is known where top-p is over the whole row.  A window
+  // says nothing of a row whose logits are infinite or whose grid is too coarse.
+  bool summed = false;
+  if (st.use_p && top < INFINITY && slack < 0.01f)
+    summed = (st.use_k ? R.find_window(st.p, grid) : sh.win_hi > -INFINITY) &&
+             R.cut_window(st.p, grid, part, i0, i1, min_w, mine);
+  if (st.use_p && !summed) {
     R.clear_bins();
     // Tokens that even together weigh less than (1 - p) of the largest cannot
     // hold the crossing: they count into the total alone.
@@ -941,11 +1195,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     R.select<true>(target);
   }
 
-  // The draw.  A thread sums a contiguous part of the slice (an odd number of
-  // elements: no bank conflicts), so the parts are in order of id.
-  const int part = ((n + kThreads - 1) / kThreads) | 1;
-  const int i0 = min(tid * part, n), i1 = min(i0 + part, n);
-  const double min_w = (double)st.least * (double)(1ull << kOneBits);
+  // The draw.
   // the scaled logit below which min_p surely drops a token
   const double z_min = st.use_min ? log((double)st.least) - 1e-6 : -INFINITY;
   auto final_weight = [&](int i) -> uint64_t {
@@ -954,10 +1204,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     if (!R.kept(key_of(v), base + i)) return 0;
     if (v != top && ((double)v - (double)top) * R.inv_t < z_min) return 0;
     const uint64_t w = R.weight(v);
-    return (double)w >= min_w ? w : 0;
+    return w >= min_w ? w : 0;
   };
-  uint64_t mine = 0;
-  if (filtered) {
+  if (summed) {
+    // cut_window has done it
+  } else if (filtered) {
 #pragma unroll 2
     for (int i = i0; i < i1; ++i) mine += final_weight(i);
   } else {
