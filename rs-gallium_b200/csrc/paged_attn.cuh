@@ -129,8 +129,8 @@ __device__ __forceinline__ V warp_inclusive(V v) {
 
 // Units per split (see Plan): the same in every CTA.
 __device__ __forceinline__ int split_units(const AttnArgs& a, const Plan& pl, unsigned long long w) {
-  const double t = ceil((double)w * a.b.nkv * (1.25 / pl.target));
-  return max(pl.min_units, (int)fmin(t, 1073741824.0));
+  const unsigned long long t = (w * a.b.nkv * 5 + 4 * pl.target - 1) / (4u * pl.target);
+  return max(pl.min_units, (int)min(t, 1ull << 30));
 }
 
 // Item `j` (of its sequence) of sequence s with `splits` splits per tile; first_group,
@@ -144,7 +144,7 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, const Plan& pl, con
   const uint32_t js = j / (uint32_t)a.b.nkv;
   it.g = (int)(j - js * (uint32_t)a.b.nkv);
   // the last tile, which sees most keys, first
-  const uint32_t back = js / (uint32_t)splits;
+  const uint32_t back = splits > 1 ? js / (uint32_t)splits : js;
   const int split = (int)(js - back * (uint32_t)splits), tile = x.tiles - 1 - (int)back;
   it.row0 = q.row0 + tile * tpt;
   it.tokens = min(tpt, q.q_len - tile * tpt);
@@ -152,11 +152,13 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, const Plan& pl, con
   const int last = it.pos0 + it.tokens - 1;
   const int lo = first_unit(it.pos0, a.window, pl.unit);
   const int n = last < 0 ? 0 : last / pl.unit - lo + 1;
-  const int per = (n + splits - 1) / splits;
-  it.u0 = lo + min(split * per, n);
-  it.u1 = lo + min((split + 1) * per, n);
+  it.u0 = lo;
+  it.u1 = lo + n;
   it.slot = -1;
   if (splits > 1) {
+    const int per = (n + splits - 1) / splits;
+    it.u0 = lo + min(split * per, n);
+    it.u1 = lo + min((split + 1) * per, n);
     const int nth = tile * a.b.nkv + it.g;
     const int slot0 = (int)first_slot + nth * splits;
     it.slot = slot0 + split;
@@ -168,8 +170,8 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, const Plan& pl, con
 
 // Finds the CTA's item among the sequences of one kind (SMALL: at most kRows
 // rows); false: there is none.  Called by the whole CTA of THREADS threads; tpt:
-// tokens per tile.  Up to 128 sequences every warp works it out for itself, four
-// sequences a lane, without a barrier; more take the whole CTA.
+// tokens per tile.  Up to 128 sequences every warp works it out for itself, a lane per
+// sequence, without a barrier; more take the whole CTA.
 template <bool SMALL, int THREADS>
 __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& part, int tpt,
                           Item* out) {
@@ -182,49 +184,46 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       q[i] = Seq{0, 0, 0};
-      const int s = 4 * lane + i;
+      x[i] = SeqWork{0, 0};
+      if (32 * i >= b.n_seqs) continue;
+      const int s = 32 * i + lane;
       if (s < b.n_seqs) q[i] = load_seq(b, s, blockIdx.x == 0 && warp == 0);
       x[i] = seq_work<SMALL>(a, pl, q[i], tpt);
       w += (unsigned long long)x[i].tiles * x[i].units;
     }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) w += __shfl_xor_sync(kFullMask, w, o);
+    // In parts of 24 bits, which add up in 32; with so much work in one lane there are
+    // no splits, whatever the sum.
+    w = min(w, (1ull << 48) - 1);
+    w = (unsigned long long)__reduce_add_sync(kFullMask, (uint32_t)w & 0xffffffu) +
+        ((unsigned long long)__reduce_add_sync(kFullMask, (uint32_t)(w >> 24) & 0xffffffu) << 24);
     const int t = split_units(a, pl, w);
-    uint32_t items[4], mine = 0, mine_groups = 0, mine_slots = 0;
-    int splits[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      splits[i] = x[i].units > t ? (x[i].units + t - 1) / t : 1;
-      items[i] = (uint32_t)x[i].tiles * b.nkv * splits[i];
-      mine += items[i];
-      if (splits[i] > 1) {
-        mine_groups += (uint32_t)x[i].tiles * b.nkv;
-        mine_slots += items[i];
-      }
-    }
-    uint32_t before = warp_inclusive(mine) - mine, groups = 0, slots = 0, all_groups = 0;
-    if (__any_sync(kFullMask, mine_slots)) {  // the same in every warp
-      groups = warp_inclusive(mine_groups);
-      all_groups = __shfl_sync(kFullMask, groups, 31);
-      groups -= mine_groups;
-      slots = warp_inclusive(mine_slots) - mine_slots;
-    }
-    if (blockIdx.x == 0 && tid == 0) *part.n_groups = (int)all_groups;
     Item it{};
     bool found = false;
+    uint32_t base = 0, base_groups = 0, base_slots = 0;  // of the sequences 32 i and on before
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (blockIdx.x >= before && blockIdx.x - before < items[i]) {
-        it = make_item(a, pl, part, tpt, 4 * lane + i, q[i], x[i], splits[i], blockIdx.x - before,
-                       groups, slots, warp == 0);
+      if (32 * i >= b.n_seqs) continue;
+      const int splits = x[i].units > t ? (x[i].units + t - 1) / t : 1;
+      const uint32_t tiles = (uint32_t)x[i].tiles * b.nkv, items = tiles * splits;
+      const uint32_t upto = base + warp_inclusive(items);
+      uint32_t groups = 0, slots = 0;
+      const bool split = __any_sync(kFullMask, splits > 1);
+      if (split) {
+        groups = base_groups + warp_inclusive(splits > 1 ? tiles : 0);
+        slots = base_slots + warp_inclusive(splits > 1 ? items : 0);
+      }
+      if (blockIdx.x < upto && blockIdx.x >= upto - items) {
+        it = make_item(a, pl, part, tpt, 32 * i + lane, q[i], x[i], splits, blockIdx.x - (upto - items),
+                       groups - tiles, slots - items, warp == 0);
         found = true;
       }
-      before += items[i];
-      if (splits[i] > 1) {
-        groups += (uint32_t)x[i].tiles * b.nkv;
-        slots += items[i];
+      base = __shfl_sync(kFullMask, upto, 31);
+      if (split) {
+        base_groups = __shfl_sync(kFullMask, groups, 31);
+        base_slots = __shfl_sync(kFullMask, slots, 31);
       }
     }
+    if (blockIdx.x == 0 && tid == 0) *part.n_groups = (int)base_groups;
     const unsigned m = __ballot_sync(kFullMask, found);
     if (!m) return false;
     const int src = __ffs(m) - 1;

@@ -9,10 +9,10 @@
 //   O_w += P_w V             tcgen05.mma, A in TMEM, V as stored (its keys are
 //                            the MMA's K: B is "MN-major")
 // The tensor cores work on one row tile while another is in its softmax: two
-// tiles of one CTA at head_dim 128 (each K and V tile is read once for both), two
-// CTAs of an SM at 64, which also hide each other's start and end.  Where TMEM
-// has room (64 and 256), S has two buffers, so that the next tile's S is there
-// when a softmax ends.  K and V
+// tiles of one CTA at head_dim 128 (each K and V tile is read once for both), two or
+// four CTAs of an SM at 64, which also hide each other's start and end.  Where TMEM
+// has room (256, and 64 with two CTAs), S has two buffers, so that the next tile's S
+// is there when a softmax ends.  K and V
 // tiles come by TMA from the pages as stored: a box per page and 64 columns (the
 // 128-byte swizzle), the page number read by a lane of the producer warp; a page
 // that is not needed, or bad, is read as out of range, which TMA fills with zeros.
@@ -36,16 +36,19 @@ namespace gb {
 namespace paged {
 namespace {
 
-template <int HD>
+// MANY, at head_dim 64: four CTAs on an SM with one S buffer and a short ring each,
+// instead of two that reach further ahead.  A CTA spends some 8 us on its start and
+// end, which more neighbours hide.
+template <int HD, bool MANY = false>
 struct Cfg {
   static constexpr int NT = HD == 128 ? 2 : 1;            // row tiles
   static constexpr int KT = HD == 128 ? 128 : 64;         // keys per tile
-  static constexpr int kBufs = HD == 128 ? 1 : 2;         // S buffers per row tile
-  static constexpr int kCtas = HD == 64 ? 2 : 1;          // per SM
+  static constexpr int kBufs = HD == 128 || MANY ? 1 : 2;  // S buffers per row tile
+  static constexpr int kCtas = MANY ? 4 : HD == 64 ? 2 : 1;  // per SM
   static constexpr int kSub = HD / 64;                    // 64-column blocks
   static constexpr int kQBytes = NT * 128 * HD * 2;
   static constexpr int kTileBytes = KT * HD * 2;          // a K or V tile
-  static constexpr int kRing = HD == 64 ? 9 : HD == 128 ? 4 : 5;  // K and V tiles in flight
+  static constexpr int kRing = MANY ? 4 : HD == 64 ? 9 : HD == 128 ? 4 : 5;  // K and V tiles in flight
   static constexpr int kSoftmax = NT * 128;               // softmax threads
   // head_dim 128 holds 128 scores per thread: its softmax warps take registers
   // from the other warpgroup, which two idle warps fill (3 x 168 = 2 x 216 + 72).
@@ -172,11 +175,11 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int piece) {
   return (uint32_t)((piece >> 3) * (Cfg<HD>::KT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kCtas)
+template <typename T, int HD, bool MANY>
+__global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
     attn_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a) {
-  using C = Cfg<HD>;
+  using C = Cfg<HD, MANY>;
   constexpr int NT = C::NT, KT = C::KT, kBufs = C::kBufs;
   constexpr int kHalves = kBufs == 1 ? 2 : 1;  // P handed over in parts
   // the buffer of a row tile's step, and the phase of its barriers
@@ -672,9 +675,9 @@ cudaError_t make_map(CUtensorMap* m, int dtype, const void* base, int rank, cons
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool MANY = false>
 cudaError_t launch(const AttnArgs& a, bool pdl, cudaStream_t st) {
-  using C = Cfg<HD>;
+  using C = Cfg<HD, MANY>;
   const int tpt = 128 / a.group;
   constexpr int dt = Elem<T>::kType;
   CUtensorMap mq, mk, mv;
@@ -701,7 +704,7 @@ cudaError_t launch(const AttnArgs& a, bool pdl, cudaStream_t st) {
   const int64_t tiles = std::min<int64_t>(a.b.total_q / per + a.b.n_seqs, a.b.total_q) * a.b.nkv;
   const int64_t grid = grid_bound(a, tile_plan<HD>(), tiles);
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  auto kern = attn_tile_kernel<T, HD>;
+  auto kern = attn_tile_kernel<T, HD, MANY>;
   cudaError_t e = set_smem_limit(kern, C::kSmem);
   if (e != cudaSuccess) return e;
   if (pdl)
@@ -712,6 +715,13 @@ cudaError_t launch(const AttnArgs& a, bool pdl, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch_hd(const AttnArgs& a, int hd, bool pdl, cudaStream_t st) {
+  // Four CTAs per SM from two waves of two on, unless rows see many keys (64 query and 8
+  // KV heads): 1184 tiles of 4 K keys 283 us against 297, 2368 of up to 5 K 262 against
+  // 297, with a window of 128 75 against 86; but 296 tiles of 4 K keys 83 against 70, and
+  // 1184 of 30 K keys 1731 against 1665.
+  const int64_t tiles = ((int64_t)a.b.total_q * a.group / 128 + a.b.n_seqs) * a.b.nkv;
+  const int64_t keys = a.window > 0 ? std::min<int64_t>(a.window, a.b.max_kv) : a.b.max_kv;
+  if (hd == 64 && tiles >= 592 && keys <= 8192) return launch<T, 64, true>(a, pdl, st);
   if (hd == 64) return launch<T, 64>(a, pdl, st);
   if (hd == 128) return launch<T, 128>(a, pdl, st);
   return launch<T, 256>(a, pdl, st);

@@ -287,6 +287,65 @@ def test_later_rows_have_no_part_in_earlier_ones(value):
         assert torch.equal(out[~sees], clean[c.starts[b]:][~sees])
 
 
+# Rows behind the last sequence make a batch one of many tiles (more than 592 of 128
+# rows), whose chunks at head_dim 64 run four to an SM.
+MANY = dict(heads=16, kvh=2, dim=64, spare_rows=4800)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("window", [0, 1, 64, 100])
+def test_attention_of_many_tiles(window, dtype):
+    c = Case([(160, 300), (1, 333), (50, 130), (20, 16), (0, 40), (7, 0), (129, 129)], dtype=dtype, seed=31, **MANY)
+    _check_attention(c, window=window, sinks=np.linspace(-2, 2, 16))
+
+
+@pytest.mark.parametrize("window", [0, 128])
+def test_attention_of_many_tiles_long(window):
+    lens = [(2048, 2048), (1, 3000), (777, 1500), (601, 8000), (1, 5), (64, 4000)]
+    c = Case(lens, heads=64, kvh=8, dim=64, seed=32, page=64)
+    sinks = np.linspace(-2, 2, 64)
+    first = _check_large(c, window=window, sinks=sinks)
+    s = _torch().tensor(sinks, dtype=_torch().float32).cuda()
+    for _ in range(3):  # the same result every time
+        assert _torch().equal(paged.attention(c.batch(), c.q, c.k, c.v, window=window, sinks=s), first)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_many_tiles_keep_values_that_are_not_finite_to_the_rows_that_see_them(value):
+    torch = _torch()
+    for window in (0, 32):
+        c = Case([(200, 300), (40, 40)], seed=33, **MANY)
+        clean = paged.attention(c.batch(), c.q, c.k, c.v, window=window)
+        bad = 300 - 100
+        c.v[c.table_np[0, bad // c.page], bad % c.page] = value
+        out = paged.attention(c.batch(), c.q, c.k, c.v, window=window)
+        pos = torch.arange(100, 300)
+        sees = torch.zeros(240, dtype=torch.bool)
+        sees[:200] = (pos >= bad) & ((pos - bad < window) if window else True)
+        assert torch.equal(out[:240][~sees], clean[:240][~sees])
+        assert not torch.isfinite(out[:240][sees]).any()
+
+
+def test_calls_on_two_streams_at_once():
+    """Batches of few and of many tiles, of different head dims, in flight together."""
+    torch = _torch()
+    cases = [Case([(160, 900), (1, 700)], seed=34, **MANY), Case([(300, 300), (1, 5000)], heads=8, kvh=2, seed=35),
+             Case([(260, 800), (1, 900)], heads=8, kvh=2, dim=128, seed=36)]
+    batches = [c.batch() for c in cases]
+    want = [paged.attention(b, c.q, c.k, c.v, out=torch.zeros_like(c.q)) for b, c in zip(batches, cases)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    for _ in range(10):
+        for i, (b, c) in enumerate(zip(batches, cases)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(paged.attention(b, c.q, c.k, c.v, out=torch.zeros_like(c.q)))
+    torch.cuda.synchronize()
+    for i, b in enumerate(batches):
+        b.check()
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
 def test_large_scores_and_masks_of_the_lowest_value():
     """Scores of +-10^4 (one key takes all), and keys whose scores are all the
     type's lowest value."""
