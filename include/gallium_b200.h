@@ -461,7 +461,10 @@ int gb_decoder_destroy(gb_decoder* d);
  * call's rows and the cached positions 0 .. kv_len[b] - 1, its new tokens
  * included: its row i sits at position kv_len[b] - q_len[b] + i.  Position p
  * lives in slot p % page_size of page page_table[b][p / page_size].  Rows at
- * or past q_start[n_seqs] belong to no sequence and are left as they are. */
+ * or past q_start[n_seqs] belong to no sequence and are left as they are.
+ * Sequences may share pages; a page that new tokens are stored into must
+ * belong to one of them alone (gb_paged_copy makes it so), or either's keys
+ * and values may be the ones that stay. */
 typedef struct gb_paged_batch {
   uint32_t struct_size;          /* sizeof(gb_paged_batch) */
   int32_t dtype;                 /* the pools': GB_DTYPE_BF16 or GB_DTYPE_F16 */
@@ -489,7 +492,9 @@ typedef enum {
   GB_PAGED_BAD_PAGE = 1,     /* a needed page number outside [0, n_pages): its keys count as
                                 masked, its stores are dropped */
   GB_PAGED_BAD_LENGTH = 2,   /* q_start not ascending within [0, total_q], a q_len or kv_len
-                                outside [0, max] or past the page table: clamped to it */
+                                outside [0, max] or past the page table: clamped to it, and
+                                rows of a sequence longer than max_q_len may be left as they
+                                are */
   GB_PAGED_BAD_POSITION = 4, /* a row before position 0 or past the cos / sin tables: the row
                                 is dropped */
   GB_PAGED_TIMEOUT = 8       /* a bounded pipeline wait ran out: the output is invalid */

@@ -1341,9 +1341,14 @@ int gb_decoder_forward_paged(gb_decoder* h, const int32_t* tokens_dev, const gb_
   if (batch->n_seqs > D.d.max_batch || batch->total_q > D.rows_cap)
     return set_error(GB_ERR_INVALID_ARG, "%d sequences with %d rows: at most %d and %lld",
                      batch->n_seqs, batch->total_q, D.d.max_batch, (long long)D.rows_cap);
+  // what gb_paged_attention would refuse, before any layer has stored its keys
+  if (D.d.n_heads > 16 * D.d.n_kv_heads)
+    return set_error(GB_ERR_UNSUPPORTED, "%d query heads per KV head: at most 16",
+                     D.d.n_heads / D.d.n_kv_heads);
   for (int l = 0; l < D.d.n_layers; ++l)
-    if (!k_pools[l] || !v_pools[l])
-      return set_error(GB_ERR_INVALID_ARG, "layer %d: a pool is null", l);
+    if (!k_pools[l] || !v_pools[l] ||
+        ((reinterpret_cast<uintptr_t>(k_pools[l]) | reinterpret_cast<uintptr_t>(v_pools[l])) & 15))
+      return set_error(GB_ERR_INVALID_ARG, "layer %d: a pool is null or not 16-byte aligned", l);
   if (logits_dev && (reinterpret_cast<uintptr_t>(logits_dev) & 15))
     return set_error(GB_ERR_INVALID_ARG, "logits_dev must be 16-byte aligned");
   if (batch->n_seqs == 0 || batch->total_q == 0) return GB_OK;

@@ -52,7 +52,7 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Keys per warp and step; a CTA's four warps take a unit of 64.
+// Keys per warp and step.
 constexpr int kStep = 16;
 constexpr int kWarps = kThreads / 32;
 
@@ -63,12 +63,16 @@ template <int HD>
 constexpr int stages() { return HD == 128 ? 2 : 3; }
 template <int HD>
 constexpr int warp_bytes() { return stages<HD>() * 2 * kStep * HD * 2; }
-// the stages, Q, and the join of the warps' sums
-template <int HD>
-constexpr int smem_bytes() { return kWarps * warp_bytes<HD>() + kRows * HD * 2 + kRows * HD * 4; }
+// the stages, Q where registers do not hold it, and
+// the join of the warps' sums
+template <int HD, int HPC>
+constexpr int smem_bytes() {
+  return kWarps * warp_bytes<HD>() + (HD == 256 ? kRows * HD * 2 : 0) + HPC * kRows * HD * 4;
+}
 
-// Where a CTA's share begins: the units of the decoding sequences' (sequence, KV
-// head) pairs in a row, cut into equal shares of `share` units.
+// Where a CTA's share begins: the units of the decoding sequences' pairs (a sequence and
+// HPC of its KV heads, `pairs` per sequence) in a row, cut into equal shares of `share`
+// units.
 struct Share {
   int64_t begin, units;  // begin < 0: none
   int64_t share, total;
@@ -93,35 +97,37 @@ __device__ __forceinline__ void set_share(const AttnArgs& a, const Plan& pl, uns
   if (sh->units <= 0) sh->begin = -1;
 }
 
-// Up to 128 sequences each warp holds them all, four a lane (mine); else the CTA
+// Up to 128 sequences each warp holds them all, one in 32 a lane (mine); else the CTA
 // works out its share together and sequences are read when they are needed.
-__device__ __forceinline__ Share find_share(const AttnArgs& a, const Plan& pl, Seq (&mine)[4]) {
+__device__ __forceinline__ Share find_share(const AttnArgs& a, const Plan& pl, int pairs, Seq (&mine)[4]) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Batch& b = a.b;
   Share sh;
   sh.seq = 0;
   sh.offset = 0;
   if (b.n_seqs <= 128) {
-    unsigned long long w[4], sum = 0;
+    unsigned long long w[4], upto[4], total = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       mine[i] = Seq{0, 0, 0};
-      if (4 * lane + i < b.n_seqs) mine[i] = load_seq(b, 4 * lane + i, blockIdx.x == 0 && warp == 0);
-      w[i] = (unsigned long long)pair_units(a, pl, mine[i]) * b.nkv;
-      sum += w[i];
+      w[i] = upto[i] = 0;
+      if (32 * i >= b.n_seqs) continue;
+      const int s = 32 * i + lane;
+      if (s < b.n_seqs) mine[i] = load_seq(b, s, blockIdx.x == 0 && warp == 0);
+      w[i] = (unsigned long long)pair_units(a, pl, mine[i]) * pairs;
+      upto[i] = total + warp_inclusive(w[i]);
+      total = __shfl_sync(kFullMask, upto[i], 31);
     }
-    const unsigned long long inc = warp_inclusive(sum);
-    set_share(a, pl, __shfl_sync(kFullMask, inc, 31), &sh);
-    unsigned long long before = inc - sum;
+    set_share(a, pl, total, &sh);
     int seq = -1;
     int64_t off = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (sh.begin >= (int64_t)before && sh.begin < (int64_t)(before + w[i])) {
-        seq = 4 * lane + i;
-        off = sh.begin - (int64_t)before;
+      const int64_t before = (int64_t)(upto[i] - w[i]);
+      if (sh.begin >= before && sh.begin < (int64_t)upto[i]) {
+        seq = 32 * i + lane;
+        off = sh.begin - before;
       }
-      before += w[i];
     }
     const unsigned m = __ballot_sync(kFullMask, seq >= 0);
     if (m) {
@@ -143,13 +149,13 @@ __device__ __forceinline__ Share find_share(const AttnArgs& a, const Plan& pl, S
   sum = 0;
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) sum += part[i];
-  set_share(a, pl, sum * b.nkv, &sh);
+  set_share(a, pl, sum * pairs, &sh);
   if (sh.begin < 0) return sh;
   unsigned long long base = 0;
   for (int s0 = 0; s0 < b.n_seqs; s0 += kThreads) {
     const int s = s0 + tid;
     const unsigned long long w =
-        s < b.n_seqs ? (unsigned long long)pair_units(a, pl, load_seq(b, s, false)) * b.nkv : 0;
+        s < b.n_seqs ? (unsigned long long)pair_units(a, pl, load_seq(b, s, false)) * pairs : 0;
     const unsigned long long inc = warp_inclusive(w);
     __syncthreads();
     if (lane == 31) part[warp] = inc;
@@ -174,38 +180,44 @@ __device__ __forceinline__ Share find_share(const AttnArgs& a, const Plan& pl, S
 
 // A place in the row of units.
 struct Cursor {
-  int seq, g, u, units, lo;  // KV head, unit of the pair, the pair's units, its first key unit
+  int seq, g, u, units, lo;  // pair of the sequence, unit of it, its units, its first key unit
   Seq q;
 };
 
 // Every CTA takes an equal share of the units of all decoding sequences, whatever
 // their lengths; where it cuts a pair, both sides leave partial sums for the
-// joining kernel.  Four warps, each with keys of its own (16 of every unit) and
-// its own pipeline of cp.async stages, which runs on across the pairs; their
-// results are joined in shared memory at the end of each.
-template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
+// joining kernel.  Four warps, each with 16 keys of every unit of one of the pair's HPC
+// heads, and its own pipeline of cp.async stages, which runs on across the pairs; where warps
+// share a head, their results are joined in shared memory at the end of each pair.
+// Two heads side by side at head_dim 128, whose rows of a slot DRAM then gives together
+// (512 bytes of the [page][slot][head][dim] layout): 32 sequences of 100 to 4000 keys 51
+// us against 67, 256 of 300 76 against 87, 32 of 4000 the same.  Four at 64 lost as often
+// as they gained (64 sequences of 300 keys 31 us against 18, 256 of 2000 204 against 217).
+template <typename T, int HD, int HPC>
+__global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
     attn_rows_kernel(const __grid_constant__ AttnArgs a) {
   extern __shared__ __align__(128) unsigned char sm[];
-  constexpr Plan kPlan = rows_plan<HD>();
+  constexpr Plan kPlan = rows_plan<HD, HPC>();
   constexpr int kStages = stages<HD>();
+  constexpr int KW = kWarps / HPC;          // warps per head
   constexpr int C = HD / 8;                 // 16-byte pieces of a row
   constexpr int kStageBytes = 2 * kStep * HD * 2;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Seq held[4];
-  const Share share = find_share(a, kPlan, held);
+  const int hw = warp / KW, kw = warp % KW, pairs = a.b.nkv / HPC;
+  const Share share = find_share(a, kPlan, pairs, held);
   pdl_trigger();
   // the pair that begins in this share and ends in a later one, if there is one
-  if (tid == 0) a.rows.groups[blockIdx.x].splits = 0;
+  if (kw == 0 && lane == 0) a.rows.groups[blockIdx.x * HPC + hw].splits = 0;
   if (share.begin < 0) return;
   auto seq_at = [&](int s) -> Seq {  // the same in every lane
     if (a.b.n_seqs > 128) return load_seq(a.b, s, false);
     Seq q = held[0];
 #pragma unroll
     for (int i = 1; i < 4; ++i)
-      if ((s & 3) == i) q = held[i];
-    return Seq{__shfl_sync(kFullMask, q.row0, s >> 2), __shfl_sync(kFullMask, q.q_len, s >> 2),
-               __shfl_sync(kFullMask, q.kv_len, s >> 2)};
+      if ((s >> 5) == i) q = held[i];
+    return Seq{__shfl_sync(kFullMask, q.row0, s & 31), __shfl_sync(kFullMask, q.q_len, s & 31),
+               __shfl_sync(kFullMask, q.kv_len, s & 31)};
   };
   auto enter = [&](Cursor& c) {  // c.seq and c.q are set
     c.units = pair_units(a, kPlan, c.q);
@@ -213,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
   };
   auto next_pair = [&](Cursor& c) {
     c.u = 0;
-    if (++c.g < a.b.nkv) return;
+    if (++c.g < pairs) return;
     c.g = 0;
     do {
       if (++c.seq >= a.b.n_seqs) return;  // past the last unit: not used
@@ -229,8 +241,9 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
   at.u = (int)(share.offset - (int64_t)at.g * at.units);
   const int total = (int)share.units;
 
+  constexpr bool kQInRegs = HD <= 128;
   unsigned char* qs = sm + kWarps * warp_bytes<HD>();
-  float* os = reinterpret_cast<float*>(qs + kRows * HD * 2);  // [kRows][HD]
+  float* os = reinterpret_cast<float*>(qs + (kQInRegs ? 0 : kRows * HD * 2)) + hw * kRows * HD;  // [kRows][HD]
   __shared__ unsigned bad_keys[kWarps][kStages];  // of each stage, a bit per key
   __shared__ float wm[kWarps][kRows], wl[kWarps][kRows];
   const uint32_t qbase = smem_u32(qs);
@@ -246,13 +259,13 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
   auto look_up = [&]() -> int64_t {
     if (looked >= total) return -1;
     ++looked;
-    const int key = (ld.lo + ld.u) * kPlan.unit + warp * kStep + (lane & 15);
+    const int key = (ld.lo + ld.u) * kPlan.unit + kw * kStep + (lane & 15);
     const int first = a.window > 0 ? max(0, ld.q.kv_len - ld.q.q_len - a.window + 1) : 0;
     int64_t off = -1;
     if (key >= first && key < ld.q.kv_len) {
       const int page = __ldg(a.b.table + ld.seq * a.b.table_stride + (key >> a.b.page_shift));
       if ((unsigned)page < (unsigned)a.b.n_pages) {
-        off = page * a.b.page_stride + (key & page_mask) * a.b.slot_stride + ld.g * a.b.head_stride;
+        off = page * a.b.page_stride + (key & page_mask) * a.b.slot_stride + (ld.g * HPC + hw) * a.b.head_stride;
       } else {
         flag(a.b, GB_PAGED_BAD_PAGE);
         off = -2;
@@ -291,28 +304,38 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
     const int len = min(at.units - at.u, total - done);
     const int n_rows = at.q.q_len * a.group, pos0 = at.q.kv_len - at.q.q_len;
     const int last = at.q.kv_len - 1;
-    __syncthreads();  // the pair before is done with Q
-    // Q rows, piece c of row r at c ^ (r & 7): ldmatrix reads 8 rows without bank conflicts
-    for (int i = tid; i < kRows * C; i += kThreads) {
-      const int r = i / C, c = i % C;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < n_rows) {
-        const int tok = r / a.group, h = at.g * a.group + r - tok * a.group;
-        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
-                                            (at.q.row0 + tok) * a.q_row + h * a.q_head + c * 8);
-      }
-      *reinterpret_cast<uint4*>(qs + r * HD * 2 + ((c ^ (r & 7)) << 4)) = v;
-    }
-    __syncthreads();
-    constexpr bool kQInRegs = HD <= 128;
+    const int head0 = (at.g * HPC + hw) * a.group;  // the KV head's first query head
+    auto q_row = [&](int r) -> const T* {
+      const int tok = r / a.group;
+      return static_cast<const T*>(a.q) + (at.q.row0 + tok) * a.q_row + (head0 + r - tok * a.group) * a.q_head;
+    };
     uint32_t qf[kQInRegs ? HD / 16 : 1][4];
     auto load_q = [&](int ks, uint32_t(&f)[4]) {
       const int r = lane & 15, c = ks * 2 + (lane >> 4);
       ldsm4(f, qbase + r * HD * 2 + ((c ^ (r & 7)) << 4));
     };
     if constexpr (kQInRegs) {
+      // the MMA's fragments: rows lane / 4 and + 8, two columns, and the two 8 on
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) load_q(ks, qf[ks]);
+      for (int h = 0; h < 2; ++h) {
+        const int r = (lane >> 2) + h * 8;
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(q_row(r < n_rows ? r : 0)) + (lane & 3);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          qf[ks][h] = r < n_rows ? __ldg(src + ks * 8) : 0;
+          qf[ks][2 + h] = r < n_rows ? __ldg(src + ks * 8 + 4) : 0;
+        }
+      }
+    } else {
+      __syncthreads();  // the pair before is done with Q
+      // piece c of row r at c ^ (r & 7): ldmatrix reads 8 rows without bank conflicts
+      for (int i = tid; i < kRows * C; i += kThreads) {
+        const int r = i / C, c = i % C;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < n_rows) v = *reinterpret_cast<const uint4*>(q_row(r) + c * 8);
+        *reinterpret_cast<uint4*>(qs + r * HD * 2 + ((c ^ (r & 7)) << 4)) = v;
+      }
+      __syncthreads();
     }
     // this lane's two rows
     const int r0 = lane >> 2, r1 = r0 + 8;
@@ -329,13 +352,15 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 
     for (int k = 0; k < len; ++k) {
+      // heads side by side stay in step, so that DRAM sees their rows together
+      if constexpr (HPC > 1) __syncthreads();
       if (done + k + kStages - 1 < total) issue(fill, next_off);
       cp_commit();
       next_off = look_up();
       cp_wait<kStages - 1>();
       __syncwarp();
       const uint32_t ks_ = wbase + slot * kStageBytes, vs_ = ks_ + kStep * HD * 2;
-      const int key0 = (at.lo + at.u + k) * kPlan.unit + warp * kStep;
+      const int key0 = (at.lo + at.u + k) * kPlan.unit + kw * kStep;
       if (key0 <= last && key0 + kStep > key_lo) {  // the same on the whole warp
         float s[2][4];
 #pragma unroll
@@ -462,7 +487,28 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
     l1 += __shfl_xor_sync(kFullMask, l1, 1);
     l0 += __shfl_xor_sync(kFullMask, l0, 2);
     l1 += __shfl_xor_sync(kFullMask, l1, 2);
-    // ---- the warps' sums, added in their order
+    const bool whole = len == at.units;
+    // A partial result's slot: a share has at most two, in its first pair and its last.
+    const int part = (2 * blockIdx.x + (done ? 1 : 0)) * HPC + hw;
+    // Two elements of row r, and its statistics: a result, or a part of one.
+    auto put = [&](int r, int d, float2 o, float top, float L) {
+      if (!whole) {
+        *reinterpret_cast<float2*>(a.rows.o + ((int64_t)part * kRows + r) * HD + d) = o;
+        if (d == 0) a.rows.ml[part * kRows + r] = make_float2(top, L);
+        return;
+      }
+      const int tok = r / a.group, h = head0 + r - tok * a.group;
+      float f = 1.0f;
+      if (a.sinks) {
+        const float sink = a.sinks[h] * kLog2e, M = fmaxf(top, sink);
+        f = top == -INFINITY ? 0.0f : ex2(top - M);
+        L = L * f + (M == -INFINITY ? 0.0f : ex2(sink - M));
+      }
+      const float inv = L == 0.0f ? 0.0f : f / L;
+      store_out<T>(a, at.q.row0 + tok, h, d, o.x * inv, o.y * inv);
+    };
+    // ---- the head's warps' sums, added in their order
+    __syncthreads();  // the pair before is read
     if ((lane & 3) == 0) {
       wm[warp][r0] = m0;
       wm[warp][r1] = m1;
@@ -472,13 +518,13 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
     __syncthreads();
     float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      M0 = fmaxf(M0, wm[w][r0]);
-      M1 = fmaxf(M1, wm[w][r1]);
+    for (int w = 0; w < KW; ++w) {
+      M0 = fmaxf(M0, wm[hw * KW + w][r0]);
+      M1 = fmaxf(M1, wm[hw * KW + w][r1]);
     }
     const float f0 = m0 == -INFINITY ? 0.0f : ex2(m0 - M0), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - M1);
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) {
+    for (int w = 0; w < KW; ++w) {
+      if (w == kw) {
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) {
           const int d = i * 8 + (lane & 3) * 2;
@@ -500,40 +546,20 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD>().target / 148)
       }
       __syncthreads();
     }
-    const bool whole = len == at.units;
-    // A partial result's slot: a share has at most two, in its first pair and its last.
-    const int part = 2 * blockIdx.x + (done ? 1 : 0);
-    for (int i = tid; i < n_rows * (HD / 2); i += kThreads) {
+    for (int i = kw * 32 + lane; i < n_rows * (HD / 2); i += KW * 32) {
       const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
-      float M = -INFINITY;
+      float M = -INFINITY, L = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, wm[w][r]);
-      const int tok = r / a.group, h = at.g * a.group + r - tok * a.group;
-      const float top = M;
-      float L = 0.0f;
+      for (int w = 0; w < KW; ++w) M = fmaxf(M, wm[hw * KW + w][r]);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        if (wm[w][r] != -INFINITY) L += wl[w][r] * ex2(wm[w][r] - M);
-      const float2 o = *reinterpret_cast<const float2*>(os + r * HD + d);
-      if (!whole) {
-        *reinterpret_cast<float2*>(a.rows.o + ((int64_t)part * kRows + r) * HD + d) = o;
-        if (d == 0) a.rows.ml[part * kRows + r] = make_float2(top, L);
-      } else {
-        float f = 1.0f;
-        if (a.sinks) {
-          const float sink = a.sinks[h] * kLog2e;
-          M = fmaxf(M, sink);
-          f = top == -INFINITY ? 0.0f : ex2(top - M);
-          L = L * f + (M == -INFINITY ? 0.0f : ex2(sink - M));
-        }
-        const float inv = L == 0.0f ? 0.0f : f / L;
-        store_out<T>(a, at.q.row0 + tok, h, d, o.x * inv, o.y * inv);
-      }
+      for (int w = 0; w < KW; ++w)
+        if (wm[hw * KW + w][r] != -INFINITY) L += wl[hw * KW + w][r] * ex2(wm[hw * KW + w][r] - M);
+      put(r, d, *reinterpret_cast<const float2*>(os + r * HD + d), M, L);
     }
-    if (!whole && at.u == 0 && tid == 0) {
+    if (!whole && at.u == 0 && kw == 0 && lane == 0) {
       const int64_t end = share.begin + done + at.units - 1;  // the pair's last unit
-      a.rows.groups[blockIdx.x] =
-          Group{at.q.row0, n_rows, at.g, part, 2 * (int)blockIdx.x, 2,
+      a.rows.groups[blockIdx.x * HPC + hw] =
+          Group{at.q.row0, n_rows, at.g * HPC + hw, part, 2 * (int)blockIdx.x * HPC + hw, 2 * HPC,
                 (int)(end / share.share) - (int)blockIdx.x + 1};
     }
     done += len;
@@ -548,7 +574,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kRows * 32) attn_join_kernel(const __grid_constant__ AttnArgs a) {
   pdl_wait();
   constexpr int kTileRows = tile_plan<HD>().tile_rows, kParts = kTileRows / kRows;
-  const int n_small = a.all_tiles ? 0 : a.rows_grid;
+  const int n_small = a.all_tiles ? 0 : a.rows_grid * a.side;
   const int n_tiles = a.tiles.n_groups ? __ldcg(a.tiles.n_groups) : 0;
   const int lane = threadIdx.x & 31;
   for (int i = blockIdx.x; i < n_small + n_tiles * kParts; i += gridDim.x) {
@@ -623,20 +649,36 @@ size_t workspace_layout(int head_dim, char* base, AttnArgs* a) {
     at += (bytes + 255) & ~(size_t)255;
     return p;
   };
-  auto part = [&](const Plan& pl, Partials* p) {
+  auto part = [&](const Plan& pl, int side, Partials* p) {
     char* n = take(sizeof(int));
-    char* g = take(sizeof(Group) * pl.target);
-    char* ml = take(sizeof(float2) * pl.slots() * pl.tile_rows);
-    char* o = take(sizeof(float) * (size_t)pl.slots() * pl.tile_rows * head_dim);
+    char* g = take(sizeof(Group) * pl.target * side);
+    char* ml = take(sizeof(float2) * pl.slots() * side * pl.tile_rows);
+    char* o = take(sizeof(float) * (size_t)pl.slots() * side * pl.tile_rows * head_dim);
     if (p)
       *p = Partials{reinterpret_cast<int*>(n), reinterpret_cast<Group*>(g),
                     reinterpret_cast<float2*>(ml), reinterpret_cast<float*>(o)};
   };
-  part(head_dim == 64 ? rows_plan<64>() : head_dim == 128 ? rows_plan<128>() : rows_plan<256>(),
-       a ? &a->rows : nullptr);
-  part(head_dim == 64 ? tile_plan<64>() : head_dim == 128 ? tile_plan<128>() : tile_plan<256>(),
+  Partials* rows = a ? &a->rows : nullptr;
+  if (head_dim == 64) part(rows_plan<64, 1>(), heads_side<64>(), rows);
+  else if (head_dim == 128) part(rows_plan<128, 1>(), heads_side<128>(), rows);
+  else part(rows_plan<256, 1>(), heads_side<256>(), rows);
+  part(head_dim == 64 ? tile_plan<64>() : head_dim == 128 ? tile_plan<128>() : tile_plan<256>(), 1,
        a ? &a->tiles : nullptr);
   return at;
+}
+
+template <typename T, int HD, int HPC>
+cudaError_t launch_rows(AttnArgs& a, cudaStream_t st) {
+  // shares, but no more than min_units each would make
+  constexpr Plan pl = rows_plan<HD, HPC>();
+  const int64_t most =
+      (int64_t)std::min(a.b.n_seqs, a.b.total_q) * (a.b.nkv / HPC) * (a.b.max_kv / pl.unit + 1);
+  a.rows_grid = (int)std::min<int64_t>(pl.target, (most + pl.min_units - 1) / pl.min_units);
+  auto kern = attn_rows_kernel<T, HD, HPC>;
+  cudaError_t e = set_smem_limit(kern, smem_bytes<HD, HPC>());
+  if (e != cudaSuccess) return e;
+  kern<<<(unsigned)a.rows_grid, kThreads, smem_bytes<HD, HPC>(), st>>>(a);
+  return cudaGetLastError();
 }
 
 template <typename T, int HD>
@@ -650,14 +692,10 @@ cudaError_t launch_attn(AttnArgs a, int dtype, cudaStream_t st) {
   if (!tiles) a.tiles.n_groups = nullptr;
   cudaError_t e;
   if (!a.all_tiles) {
-    // shares, but no more than min_units each would make
-    constexpr Plan pl = rows_plan<HD>();
-    const int64_t most = (int64_t)std::min(a.b.n_seqs, a.b.total_q) * a.b.nkv * (a.b.max_kv / pl.unit + 1);
-    a.rows_grid = (int)std::min<int64_t>(pl.target, (most + pl.min_units - 1) / pl.min_units);
-    auto kern = attn_rows_kernel<T, HD>;
-    if ((e = set_smem_limit(kern, smem_bytes<HD>())) != cudaSuccess) return e;
-    kern<<<(unsigned)a.rows_grid, kThreads, smem_bytes<HD>(), st>>>(a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    constexpr int kSide = heads_side<HD>();
+    a.side = a.b.nkv % kSide == 0 ? kSide : 1;
+    e = a.side == kSide ? launch_rows<T, HD, kSide>(a, st) : launch_rows<T, HD, 1>(a, st);
+    if (e != cudaSuccess) return e;
   }
   if (tiles && (e = launch_attn_tiles(a, dtype, HD, !a.all_tiles, st)) != cudaSuccess) return e;
   // One share cuts no pair; no tile is split when the longest sequence has too few keys.

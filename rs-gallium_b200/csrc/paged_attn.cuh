@@ -51,10 +51,14 @@ struct Plan {
   int min_units;  // units per split, at least
   __host__ __device__ constexpr int slots() const { return 2 * target; }
 };
-// Shares of attn_rows_kernel: four, three or one CTA on each of 148 SMs.
+// KV heads that a CTA of attn_rows_kernel takes side by side, where their number allows.
 template <int HD>
+__host__ __device__ constexpr int heads_side() { return HD == 128 ? 2 : 1; }
+// Shares of attn_rows_kernel with HPC heads side by side: four, two or one CTA on each of
+// 148 SMs, as shared memory holds; a unit is a step of the four warps, 64 keys in all.
+template <int HD, int HPC>
 __host__ __device__ constexpr Plan rows_plan() {
-  return Plan{kRows, 64, 148 * (HD == 64 ? 4 : HD == 128 ? 3 : 1), 2};
+  return Plan{kRows, 64 / HPC, 148 * (HD == 64 ? 4 : HD == 128 ? 2 : 1), 2};
 }
 template <int HD>
 constexpr Plan tile_plan() {
@@ -80,6 +84,7 @@ struct AttnArgs {
   Batch b;
   int nh, group, window, out_f32;
   int rows_grid;  // CTAs of attn_rows_kernel
+  int side;       // KV heads that each takes side by side
   int all_tiles;  // attn_tile_kernel takes the decoding sequences too
   float scale;  // scale * log2 e
   const void* q;
