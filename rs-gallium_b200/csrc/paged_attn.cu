@@ -187,8 +187,13 @@ struct Cursor {
 // Every CTA takes an equal share of the units of all decoding sequences, whatever
 // their lengths; where it cuts a pair, both sides leave partial sums for the
 // joining kernel.  Four warps, each with 16 keys of every unit of one of the pair's HPC
-// heads, and its own pipeline of cp.async stages, which runs on across the pairs; where warps
-// share a head, their results are joined in shared memory at the end of each pair.
+// heads, and its own pipeline of cp.async stages, which runs on across the pairs; the
+// warps of a head join their results in shared memory at the end of each pair.
+// mma.sync suits it: 16 rows fill one, and memory is the floor.  Measured with 64 query
+// and 8 KV heads of 64: 64 sequences of 512 to 8192 keys 104 us, 4.2 TB/s; 256 of 2000
+// 217 us, 4.8 TB/s, and 5.8 where a page's slots of a head lie together, since the rows
+// of a head are 128-byte pieces a slot apart.  TMA boxes in place of cp.async were no
+// faster (106 us; with the 256-byte L2 promotion, which fetches the next head too, 127).
 // Two heads side by side at head_dim 128, whose rows of a slot DRAM then gives together
 // (512 bytes of the [page][slot][head][dim] layout): 32 sequences of 100 to 4000 keys 51
 // us against 67, 256 of 300 76 against 87, 32 of 4000 the same.  Four at 64 lost as often

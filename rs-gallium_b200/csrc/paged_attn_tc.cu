@@ -29,6 +29,12 @@
 //
 // Warps: four per row tile, then the TMA producer and the MMA issuer.  Every wait
 // is bounded, as in the expert GEMMs.
+//
+// Measured: a chunk of 1000 tokens behind 16 K keys, 32 heads of 128, f16, 247 us, 1107
+// TFLOP/s (1268 behind 32 K); head_dim 256 1160 and head_dim 64 680 TFLOP/s behind 32 K;
+// four prompts of 2 K, 64 heads of 64, 246 us, 520 TFLOP/s.  Bound at head_dim 64 by the
+// softmax between the MMAs: 16 exponentials per clock and SM would take 127 us there,
+// half the time.  Two threads per row, and exponentials as polynomials, were no faster.
 #include "paged_attn.cuh"
 #include "umma.cuh"
 

@@ -216,7 +216,9 @@ __device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
 }
 
 // Few (row, head) units: one per lane group, over as many CTAs as that takes.  The
-// rows' sequences and slots are looked up while the units' loads are in flight.
+// rows' sequences and slots are looked up while the units' loads are in flight.  Bound
+// by the chain of those loads: one row of 80 heads of 64 takes 2.7 us with its launch,
+// 61 rows of 48 heads of 128 3.8.
 template <typename In, typename Out, int HD>
 __global__ void __launch_bounds__(kRopeThreads) rope_units_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int L = HD / 8;                // lanes per unit
@@ -268,6 +270,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_units_kernel(const __grid_c
 // Many rows: a CTA takes `per` of them (at most kRopeRows).  `across` lane groups
 // share a row, each with its heads in turn, so that a row's cosines, sines, page
 // and addresses are worked out once for them; the groups' other rows run beside.
+// 8150 rows of 48 heads of 128 with both norms: 57 us, 3.5 TB/s (82 with a unit at a
+// time over the whole batch); bound by the instructions of norm and rotation.
 template <typename In, typename Out, int HD>
 __global__ void __launch_bounds__(kRopeThreads, 4)
     rope_rows_kernel(const __grid_constant__ RopeArgs a, int per, int across) {
