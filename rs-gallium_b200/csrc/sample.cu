@@ -200,7 +200,8 @@ __device__ __forceinline__ int grid_of(float v, float scale) {
   return max(-(1 << 28), min(1 << 28, g));
 }
 
-// The mass of a logit in its grid bin.
+// The mass of a logit in its grid bin (-inf has none, also where 0 x inf puts it in a bin:
+// the callers leave it out).
 __device__ __forceinline__ uint32_t mass_of(float v, float scale, int bin) {
   const float frac = fminf(fmaxf(v * scale - (float)bin, 0.0f), 1.0f);
   return (uint32_t)__float2int_rn(exp2f((frac - 1.0f) * kStep) * kUnit);
@@ -561,7 +562,7 @@ struct Row {
     __syncthreads();
     each([&](float v, int id) {
       const int b = grid_of(v, scale), j = top_bin - b;
-      if (j < kBins && kept(key_of(v), id)) atomicAdd(&sh.lo[j], mass_of(v, scale, b));
+      if (j < kBins && v > -INFINITY && kept(key_of(v), id)) atomicAdd(&sh.lo[j], mass_of(v, scale, b));
     });
     cl.sync();
     const int j0 = 2 * tid;
@@ -1000,7 +1001,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   if (whole_p) {
     R.each([&](float v, int) {
       const int b = grid_of(v, grid), j = my_top - b;
-      if (j < kBins) atomicAdd(&sh.lo[j], mass_of(v, grid, b));
+      if (j < kBins && v > -INFINITY) atomicAdd(&sh.lo[j], mass_of(v, grid, b));
     });
   } else if (filtered) {
     R.each([&](float v, int) {

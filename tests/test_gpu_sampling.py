@@ -118,6 +118,42 @@ def test_16_bit_logits_with_their_ties(dtype):
     _check(x, rng.random(n), k=rng.integers(2, 5000, n), p=rng.uniform(0.05, 0.95, n), t=rng.uniform(0.3, 2, n))
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("vocab", [1500, 150001])
+@pytest.mark.parametrize("offset", [0.0, 250.0, -1000.0])
+def test_top_p_over_many_tokens(vocab, dtype, offset):
+    """Cuts among thousands of tokens, flat and peaked rows, quantised ones (a
+    tie of many at the cut), offsets that cost the histograms' grid its
+    precision, behind a large top-k and before a min-p."""
+    import torch
+
+    rng = np.random.default_rng(vocab)
+    n = 32
+    x = torch.cat([_rows(n // 4, vocab, sigma=s, peaked=pk, seed=77 + i)
+                   for i, (s, pk) in enumerate(((0.5, False), (2.0, True), (4.0, False), (1.0, True)))])
+    x[::5] = (x[::5] * 4).round() / 4
+    x = (x + offset).to(getattr(torch, dtype))
+    _check(x, rng.random(n), t=rng.choice([0.05, 0.5, 1.0, 2.0, 20.0], n),
+           k=rng.choice([0, 0, 0, 1400, vocab * 3 // 4], n), p=rng.choice([0.05, 0.5, 0.9, 0.99, 0.9999], n),
+           least=rng.choice([0.0, 0.0, 1e-4, 0.5], n))
+
+
+def test_an_infinite_temperature_weighs_what_is_not_masked_equally():
+    import torch
+
+    x = torch.full((3, 5000), -math.inf, device="cuda")
+    ids = torch.arange(0, 4500, 15, device="cuda")  # 300 tokens
+    x[:, ids] = 0.0
+    x[1:, ids] = -torch.arange(300, device="cuda", dtype=torch.float32)
+    for k in (None, [250] * 3):
+        tok, lp = _run(x, [0.999, 0.999, 0.0], t=[math.inf] * 3, k=k, p=[0.2, 0.2, 0.2])
+        # 0.2 as f32 is above a fifth (13421773 2^-26): 300 (250) of them leave the weight of
+        # 60 (50) tokens below top_p of all, so one more is kept
+        kept = 61 if k is None else 51
+        assert list(tok) == [15 * (kept - 1), 15 * (kept - 1), 0]
+        assert np.allclose(lp, -math.log(kept), rtol=2.0 ** -23)
+
+
 def test_equal_logits_are_drawn_by_id():
     import torch
 
