@@ -270,10 +270,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_units_kernel(const __grid_c
 // Many rows: a CTA takes `per` of them (at most kRopeRows).  `across` lane groups
 // share a row, each with its heads in turn, so that a row's cosines, sines, page
 // and addresses are worked out once for them; the groups' other rows run beside.
-// 8150 rows of 48 heads of 128 with both norms: 57 us, 3.5 TB/s (82 with a unit at a
-// time over the whole batch); bound by the instructions of norm and rotation.
+// 8150 rows of 48 heads of 128 with both norms: 55 us, 3.6 TB/s (82 with a unit at a
+// time over the whole batch, 57 with 64 registers and four CTAs on an SM, 62 with the
+// loads a pass ahead); bound by the instructions of norm and rotation.
 template <typename In, typename Out, int HD>
-__global__ void __launch_bounds__(kRopeThreads, 4)
+__global__ void __launch_bounds__(kRopeThreads, 3)
     rope_rows_kernel(const __grid_constant__ RopeArgs a, int per, int across) {
   constexpr int L = HD / 8;
   constexpr int G = kRopeThreads / L;
@@ -346,7 +347,7 @@ cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st) {
   if (a.units <= (int64_t)G * 148 * 4) {
     rope_units_kernel<In, Out, HD><<<(unsigned)((a.units + G - 1) / G), kRopeThreads, 0, st>>>(a);
   } else {
-    // Four CTAs an SM, a few rows each: the look-ups of a row are some 1.5 us of
+    // Several CTAs an SM, a few rows each: the look-ups of a row are some 1.5 us of
     // dependent loads, which other CTAs' rows hide.
     const int64_t rows = a.units / heads;
     const int per = (int)std::max<int64_t>(1, std::min<int64_t>(kRopeRows, rows / (148 * 4 * 4)));
