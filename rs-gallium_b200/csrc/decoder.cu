@@ -1144,8 +1144,10 @@ int run_paged(Decoder& D, const int32_t* tokens, const gb_paged_batch* batch, vo
   const int H = d.hidden, nh = d.n_heads, nkv = d.n_kv_heads, hd = d.head_dim;
   const int rows = batch->total_q, B = batch->n_seqs;
   int rc;
-  dec::embed_kernel<<<rows, 256, 0, st>>>(tokens, D.embed, H, d.vocab, D.h, D.err);
-  DEC_CUDA(cudaGetLastError(), "embedding launch");
+  if (rows > 0) {
+    dec::embed_kernel<<<rows, 256, 0, st>>>(tokens, D.embed, H, d.vocab, D.h, D.err);
+    DEC_CUDA(cudaGetLastError(), "embedding launch");
+  }
   gb_rope_args ra{};
   ra.struct_size = sizeof(ra);
   ra.in_dtype = GB_DTYPE_F32;
@@ -1174,7 +1176,7 @@ int run_paged(Decoder& D, const int32_t* tokens, const gb_paged_batch* batch, vo
   aa.workspace_dev = D.attn_ws;
   aa.workspace_bytes = D.attn_ws_bytes;
   const bool split = linear_tc(D, rows);
-  for (int l = 0; l < d.n_layers; ++l) {
+  for (int l = 0; l < d.n_layers && rows > 0; ++l) {
     DecLayer& L = D.layers[l];
     dec::add_rmsnorm_kernel<<<rows, dec::kNormThreads, 0, st>>>(
         D.h, l ? D.moe_out : nullptr, L.attn_norm, H, d.rms_eps, 1, 0, D.xn,
@@ -1329,12 +1331,12 @@ int gb_decoder_forward_paged(gb_decoder* h, const int32_t* tokens_dev, const gb_
   using namespace gb;
   if (!h) return set_error(GB_ERR_INVALID_ARG, "handle is null");
   Decoder& D = *h->D;
-  if (!tokens_dev || !k_pools || !v_pools)
-    return set_error(GB_ERR_INVALID_ARG, "tokens_dev, k_pools and v_pools must not be null");
+  if (!k_pools || !v_pools) return set_error(GB_ERR_INVALID_ARG, "k_pools and v_pools must not be null");
   DevScope ds(D.device);
   int64_t ws = 0;
   int rc = gb_paged_attention_workspace(batch, D.d.n_heads, &ws);  // checks the batch
   if (rc) return rc;
+  if (!tokens_dev && batch->total_q > 0) return set_error(GB_ERR_INVALID_ARG, "tokens_dev is null");
   if (batch->head_dim != D.d.head_dim || batch->n_kv_heads != D.d.n_kv_heads)
     return set_error(GB_ERR_INVALID_ARG, "the batch's head_dim %d and n_kv_heads %d are not the model's %d, %d",
                      batch->head_dim, batch->n_kv_heads, D.d.head_dim, D.d.n_kv_heads);
@@ -1351,7 +1353,7 @@ int gb_decoder_forward_paged(gb_decoder* h, const int32_t* tokens_dev, const gb_
       return set_error(GB_ERR_INVALID_ARG, "layer %d: a pool is null or not 16-byte aligned", l);
   if (logits_dev && (reinterpret_cast<uintptr_t>(logits_dev) & 15))
     return set_error(GB_ERR_INVALID_ARG, "logits_dev must be 16-byte aligned");
-  if (batch->n_seqs == 0 || batch->total_q == 0) return GB_OK;
+  if (batch->n_seqs == 0) return GB_OK;
   if ((rc = ensure_paged(D, ws, static_cast<cudaStream_t>(stream)))) return rc;
   D.timed = false;
   return run_paged(D, tokens_dev, batch, k_pools, v_pools, logits_dev ? logits_dev : D.logits,

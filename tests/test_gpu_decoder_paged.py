@@ -156,6 +156,24 @@ def test_ragged_prompts_chunks_and_steps(head_dim, dtype):
         sv.step([b], [tok(1)])
 
 
+def test_a_batch_without_new_tokens():
+    import torch
+
+    w = _weights(11, layers=1)
+    with _load(w) as m:
+        sv = Serve(m, w, torch.bfloat16)
+        a, b = sv.add(), sv.add()
+        for rows in (0, 4):  # rows of no sequence
+            torch.full((2, w.vocab), 3.0, device="cuda")  # what an unwritten result would hold
+            batch = paged.PagedBatch(torch.zeros(3, dtype=torch.int32, device="cuda"),
+                                     torch.zeros(2, dtype=torch.int32, device="cuda"),
+                                     torch.full((2, 4), -1, dtype=torch.int32, device="cuda"), page_size=PAGE,
+                                     total_q=rows, max_q_len=0, max_kv_len=MAX_SEQ)
+            logits = m.forward_paged(np.zeros(rows, np.int32), batch, sv.k, sv.v)
+            assert not logits.any() and list(m.last_next.cpu()) == [w.vocab - 1] * 2
+        sv.step([a, b], [np.arange(5), np.arange(3)])
+
+
 def test_own_cache_and_paged_forwards_do_not_disturb_each_other():
     import torch
 

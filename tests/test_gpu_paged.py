@@ -310,6 +310,16 @@ def test_attention_of_many_tiles_long(window):
         assert _torch().equal(paged.attention(c.batch(), c.q, c.k, c.v, window=window, sinks=s), first)
 
 
+@pytest.mark.parametrize("window", [0, 500])
+def test_attention_of_many_tiles_split_and_of_many_sequences(window):
+    _check_large(Case([(48, 8000), (1, 7000), (33, 3333)], seed=37, page=32, **MANY), window=window,
+                 sinks=np.linspace(-2, 2, 16))
+    r = np.random.default_rng(38)
+    lens = [(int(q), int(q + k)) for q, k in zip(np.exp(r.uniform(0, np.log(120), 260)), np.exp(r.uniform(0, np.log(1500), 260)))]
+    lens[3] = lens[200] = (0, 30)
+    _check_large(Case(lens, seed=39, **MANY), window=window)
+
+
 @pytest.mark.parametrize("value", [float("inf"), float("nan")])
 def test_many_tiles_keep_values_that_are_not_finite_to_the_rows_that_see_them(value):
     torch = _torch()
