@@ -589,7 +589,8 @@ int gb_paged_copy(void* const* pools_dev, int32_t n_pools, int64_t n_pages, int6
  * gb_decoder_forward runs B sequences in lockstep on the decoder's own cache.
  * tokens_dev [total_q] i32; k_pools / v_pools: host arrays of n_layers device
  * pointers, a K and a V pool per layer, laid out as the batch says (head_dim and
- * n_kv_heads the model's; head_dim 64, 128 or 256).  Every layer stores its new
+ * n_kv_heads the model's; head_dim 64, 128 or 256, at most 16 query heads per KV
+ * head).  Every layer stores its new
  * keys and values into the pools (gb_paged_rope_append) and attends over the pages
  * (gb_paged_attention); queries, keys and values are rounded to the pools' type,
  * all else is f32 as in gb_decoder_forward.  total_q <= max_batch * max_tokens,
