@@ -563,9 +563,11 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
     }
     if (!whole && at.u == 0 && kw == 0 && lane == 0) {
       const int64_t end = share.begin + done + at.units - 1;  // the pair's last unit
+      // sequences that share rows (q_start going back) may want more CTAs than there are
+      const int last_cta = (int)min(end / share.share, (int64_t)gridDim.x - 1);
       a.rows.groups[blockIdx.x * HPC + hw] =
           Group{at.q.row0, n_rows, at.g * HPC + hw, part, 2 * (int)blockIdx.x * HPC + hw, 2 * HPC,
-                (int)(end / share.share) - (int)blockIdx.x + 1};
+                last_cta - (int)blockIdx.x + 1};
     }
     done += len;
     if (done < total) next_pair(at);

@@ -107,6 +107,9 @@ __device__ __forceinline__ int first_unit(int pos, int window, int unit) {
   return window > 0 && pos >= window ? (pos - window + 1) / unit : 0;
 }
 
+// CTAs of a tile grid, at most: more rows and heads than fit in memory.
+constexpr uint32_t kMaxItems = (1u << 25) - 1;
+
 struct SeqWork {
   int tiles, units;
 };
@@ -132,8 +135,11 @@ __device__ __forceinline__ V warp_inclusive(V v) {
   return v;
 }
 
-// Units per split (see Plan): the same in every CTA.
+// Units per split (see Plan): the same in every CTA.  So much work that the product would
+// not fit (w at its limit) is never split.
+constexpr unsigned long long kMaxWork = 1ull << 48;
 __device__ __forceinline__ int split_units(const AttnArgs& a, const Plan& pl, unsigned long long w) {
+  w = min(w, kMaxWork);
   const unsigned long long t = (w * a.b.nkv * 5 + 4 * pl.target - 1) / (4u * pl.target);
   return max(pl.min_units, (int)min(t, 1ull << 30));
 }
@@ -177,6 +183,10 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, const Plan& pl, con
 // rows); false: there is none.  Called by the whole CTA of THREADS threads; tpt:
 // tokens per tile.  Up to 128 sequences every warp works it out for itself, a lane per
 // sequence, without a barrier; more take the whole CTA.
+// A q_start that goes back makes sequences share rows, and then more items than the
+// host's bound has CTAs: the split tiles of a sequence whose items do not all have one
+// are left out of n_groups (and those after it: the count runs with the items), since
+// nobody may have written their groups.
 template <bool SMALL, int THREADS>
 __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& part, int tpt,
                           Item* out) {
@@ -198,18 +208,21 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
     }
     // In parts of 24 bits, which add up in 32; with so much work in one lane there are
     // no splits, whatever the sum.
-    w = min(w, (1ull << 48) - 1);
+    w = min(w, kMaxWork - 1);
     w = (unsigned long long)__reduce_add_sync(kFullMask, (uint32_t)w & 0xffffffu) +
         ((unsigned long long)__reduce_add_sync(kFullMask, (uint32_t)(w >> 24) & 0xffffffu) << 24);
     const int t = split_units(a, pl, w);
     Item it{};
     bool found = false;
     uint32_t base = 0, base_groups = 0, base_slots = 0;  // of the sequences 32 i and on before
+    uint32_t n_groups = 0;  // of the sequences whose items all have a CTA
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (32 * i >= b.n_seqs) continue;
       const int splits = x[i].units > t ? (x[i].units + t - 1) / t : 1;
-      const uint32_t tiles = (uint32_t)x[i].tiles * b.nkv, items = tiles * splits;
+      // no more than kMaxItems each: 128 of them still add up in 32 bits
+      const uint32_t tiles = (uint32_t)min((unsigned long long)x[i].tiles * b.nkv, (unsigned long long)kMaxItems);
+      const uint32_t items = (uint32_t)min((unsigned long long)tiles * splits, (unsigned long long)kMaxItems);
       const uint32_t upto = base + warp_inclusive(items);
       uint32_t groups = 0, slots = 0;
       const bool split = __any_sync(kFullMask, splits > 1);
@@ -224,11 +237,12 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
       }
       base = __shfl_sync(kFullMask, upto, 31);
       if (split) {
+        n_groups = max(n_groups, __reduce_max_sync(kFullMask, upto <= gridDim.x ? groups : 0));
         base_groups = __shfl_sync(kFullMask, groups, 31);
         base_slots = __shfl_sync(kFullMask, slots, 31);
       }
     }
-    if (blockIdx.x == 0 && tid == 0) *part.n_groups = (int)base_groups;
+    if (blockIdx.x == 0 && tid == 0) *part.n_groups = (int)n_groups;
     const unsigned m = __ballot_sync(kFullMask, found);
     if (!m) return false;
     const int src = __ffs(m) - 1;
@@ -246,19 +260,19 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
   __shared__ unsigned long long red[kW];
   __shared__ unsigned long long run[kW][2];
   __shared__ Item found;
-  __shared__ int have;
+  __shared__ int have, n_groups;
   Seq mine{0, 0, 0};  // of the first THREADS sequences
   unsigned long long w = 0;
   for (int s = tid; s < b.n_seqs; s += THREADS) {
     const Seq q = load_seq(b, s, blockIdx.x == 0);
     if (s == tid) mine = q;
     const SeqWork x = seq_work<SMALL>(a, pl, q, tpt);
-    w += (unsigned long long)x.tiles * x.units;
+    w = min(w + (unsigned long long)x.tiles * x.units, kMaxWork);
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) w += __shfl_xor_sync(kFullMask, w, o);
   if (lane == 0) red[warp] = w;
-  if (tid == 0) have = 0;
+  if (tid == 0) have = n_groups = 0;
   __syncthreads();
   w = 0;
 #pragma unroll
@@ -292,6 +306,7 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
       base_groups += run[i][1];
     }
     const unsigned long long before = bi + ii - items;
+    if (splits > 1 && bi + ii <= gridDim.x) atomicMax(&n_groups, (int)(uint32_t)(bg + gg));
     if (blockIdx.x >= before && blockIdx.x < before + items) {
       const unsigned long long first = bg + gg - groups;
       found = make_item(a, pl, part, tpt, s, q, x, splits, (uint32_t)(blockIdx.x - before),
@@ -299,8 +314,8 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
       have = 1;
     }
   }
-  if (blockIdx.x == 0 && tid == 0) *part.n_groups = (int)(uint32_t)base_groups;
   __syncthreads();
+  if (blockIdx.x == 0 && tid == 0) *part.n_groups = n_groups;
   if (!have) return false;
   *out = found;
   return true;

@@ -709,7 +709,7 @@ cudaError_t launch(const AttnArgs& a, bool pdl, cudaStream_t st) {
   const int64_t per = (int64_t)C::NT * tpt;
   const int64_t tiles = std::min<int64_t>(a.b.total_q / per + a.b.n_seqs, a.b.total_q) * a.b.nkv;
   const int64_t grid = grid_bound(a, tile_plan<HD>(), tiles);
-  if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  if (grid > (int64_t)kMaxItems) return cudaErrorInvalidConfiguration;
   auto kern = attn_tile_kernel<T, HD, MANY>;
   cudaError_t e = set_smem_limit(kern, C::kSmem);
   if (e != cudaSuccess) return e;
