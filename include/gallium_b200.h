@@ -541,7 +541,8 @@ int gb_paged_rope_append(const gb_paged_batch* batch, const gb_rope_args* args, 
  * positions max(0, p - window + 1) .. p (window 0: from 0), scores are
  * (q . k) * scale, and a head's sink logit, when given, joins the softmax's
  * denominator.  Query head h reads KV head h / (n_heads / n_kv_heads).  A row
- * that sees nothing gives zeros.  Positions that no row of a sequence sees
+ * that sees nothing gives zeros (so does one whose scores are all -inf), one
+ * with a NaN among its scores gives NaN.  Positions that no row of a sequence sees
  * are not read: their pages may be gone (any page number, -1 say).  What a
  * row does not see has no part in its result, whatever its bits.  Scores,
  * softmax statistics and sums are f32; each probability is rounded to the

@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
       float f = 1.0f;
       if (a.sinks) {
         const float sink = a.sinks[h] * kLog2e, M = fmaxf(top, sink);
-        f = top == -INFINITY ? 0.0f : ex2(top - M);
+        f = part_factor(top, L, M);
         L = L * f + (M == -INFINITY ? 0.0f : ex2(sink - M));
       }
       const float inv = L == 0.0f ? 0.0f : f / L;
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
       M0 = fmaxf(M0, wm[hw * KW + w][r0]);
       M1 = fmaxf(M1, wm[hw * KW + w][r1]);
     }
-    const float f0 = m0 == -INFINITY ? 0.0f : ex2(m0 - M0), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - M1);
+    const float f0 = part_factor(m0, l0, M0), f1 = part_factor(m1, l1, M1);
     for (int w = 0; w < KW; ++w) {
       if (w == kw) {
 #pragma unroll
@@ -557,8 +557,10 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
 #pragma unroll
       for (int w = 0; w < KW; ++w) M = fmaxf(M, wm[hw * KW + w][r]);
 #pragma unroll
-      for (int w = 0; w < KW; ++w)
-        if (wm[hw * KW + w][r] != -INFINITY) L += wl[hw * KW + w][r] * ex2(wm[hw * KW + w][r] - M);
+      for (int w = 0; w < KW; ++w) {
+        const float l = wl[hw * KW + w][r];
+        L += l * part_factor(wm[hw * KW + w][r], l, M);
+      }
       put(r, d, *reinterpret_cast<const float2*>(os + r * HD + d), M, L);
     }
     if (!whole && at.u == 0 && kw == 0 && lane == 0) {
@@ -617,7 +619,7 @@ __global__ void __launch_bounds__(kRows * 32) attn_join_kernel(const __grid_cons
         if (s0 + lane < g.splits) ml = part.ml[at_part(s0 + lane)];
       }
       // an empty split's sums were written as well, but its weight is 0
-      const float fl = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M), ll = ml.y * fl;
+      const float fl = part_factor(ml.x, ml.y, M), ll = ml.y * fl;
       constexpr int kU = HD == 64 ? 16 : HD == 128 ? 8 : 4;  // splits whose loads are in flight
       const int n = min(32, g.splits - s0);
       for (int s = 0; s < n; s += kU) {

@@ -34,6 +34,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The factor of a part of a row (keys of one warp, of one split) whose sums refer to the
+// maximum m, where all parts' refer to M; l: its sum of weights.  A maximum passes NaN
+// over, so m stays -inf in a part that saw nothing, whose l is 0, and in one whose
+// scores were NaN, whose l is NaN: l is the factor of both.
+__device__ __forceinline__ float part_factor(float m, float l, float M) {
+  return m == -INFINITY ? l : ex2(m - M);
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 16;      // rows of a decoding sequence's tile, and of a joining CTA
 constexpr int kMaxGroup = 16;  // query heads per KV head

@@ -417,9 +417,9 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       if (!split && a.sinks && live) {
         const float sink = a.sinks[head] * kLog2e;
         M = fmaxf(m, sink);
-        L = M == -INFINITY ? 0.0f : l * ex2(m - M) + ex2(sink - M);
+        L = l * part_factor(m, l, M) + (M == -INFINITY ? 0.0f : ex2(sink - M));
       }
-      inv = split ? 1.0f : L == 0.0f || m == -INFINITY ? 0.0f : ex2(m - M) / L;
+      inv = split ? 1.0f : L == 0.0f ? 0.0f : part_factor(m, l, M) / L;
       const int out_row = it.row0 + w * tpt + tok;
       const int64_t part_row = split ? (int64_t)it.slot * kPlan.tile_rows + w * 128 + r : 0;
       if (split && live) a.tiles.ml[part_row] = make_float2(m, l);

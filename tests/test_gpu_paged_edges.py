@@ -66,3 +66,55 @@ def test_sequences_that_share_rows_join_nothing_that_was_not_written(rows, lens,
     _attention_with_workspace(batch, ok, out, 1)
     batch.check()
     assert torch.equal(out, paged.attention(ok.batch(), ok.q, ok.k, ok.v))
+
+
+# -- values that are not finite ------------------------------------------------------
+# (lengths, row of the batch whose scores are all NaN, and whether one key makes them so)
+NAN_LENS = {
+    "decode": [(1, 40), (1, 17)],                # the 17th key is alone with one of the decoding kernel's warps
+    "decode split": [(1, 40), (1, 6000)],
+    "two tokens": [(1, 40), (2, 17)],
+    "tile": [(1, 40), (40, 90)],
+    "tile split": [(1, 40), (40, 9000)],
+    "tile window": [(1, 40), (200, 300)],
+}
+
+
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("heads,kvh,dim", [(8, 2, 64), (8, 2, 128), (6, 3, 128), (4, 2, 256)])
+@pytest.mark.parametrize("lens", list(NAN_LENS))
+def test_nan_reaches_the_rows_that_see_it(lens, heads, kvh, dim, sinks):
+    """A query, or the last key of a sequence, holds NaN: what sees it is NaN, whichever
+    kernel and however many parts worked on it; everything else keeps its bits."""
+    torch = _torch()
+    window = 64 if "window" in lens else 0
+    c = Case(NAN_LENS[lens], heads=heads, kvh=kvh, dim=dim, seed=41)
+    kw = dict(window=window, sinks=torch.linspace(-1, 1, heads).cuda() if sinks else None)
+    clean = paged.attention(c.batch(), c.q, c.k, c.v, **kw)
+    assert torch.isfinite(clean).all()
+    n, kv = c.lens[1]
+    row = int(c.starts[1]) + n // 2
+    q = c.q.clone()
+    q[row, 1, 5] = float("nan")
+    out = paged.attention(c.batch(), q, c.k, c.v, **kw)
+    assert torch.isnan(out[row, 1]).all()
+    out[row, 1] = clean[row, 1]
+    assert torch.equal(out, clean)
+    # the last key, which the last row alone sees; of one KV head
+    c.k[c.table_np[1, (kv - 1) // c.page], (kv - 1) % c.page, 0, 7] = float("nan")
+    out = paged.attention(c.batch(), c.q, c.k, c.v, **kw)
+    last, group = int(c.starts[2]) - 1, heads // kvh
+    assert torch.isnan(out[last, :group]).all()
+    out[last, :group] = clean[last, :group]
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(1, 17)], [(3, 200)], [(60, 60)], [(30, 9000)]])
+def test_all_keys_nan(lens, dim):
+    """Every visible score is NaN: no row is taken for one that sees nothing."""
+    torch = _torch()
+    c = Case(lens, heads=4, kvh=1, dim=dim, seed=42)
+    c.k[...] = float("nan")
+    out = paged.attention(c.batch(), c.q, c.k, c.v)
+    assert torch.isnan(out).all()
