@@ -574,6 +574,14 @@ int gb_paged_attention(const gb_paged_batch* batch, const gb_attn_args* args, vo
  * arrays are not read), the same on every device of this library. */
 int gb_paged_attention_workspace(const gb_paged_batch* batch, int32_t n_heads, int64_t* bytes);
 
+/* Failure-handling test hooks of gb_paged_attention, for the later calls of the
+ * calling thread until reset with (0, 0).  wait_limit_us: how long each bounded
+ * wait of the kernel for chunks of new tokens may last (0 = the default, 2 s).
+ * withhold_q != 0: its first CTA leaves its queries unread, so what needs them
+ * waits until the limit; that call's output is invalid and its batch's error
+ * word reports GB_PAGED_TIMEOUT. */
+int gb_paged_set_test_hooks(int64_t wait_limit_us, int32_t withhold_q);
+
 /* Copies page src[i] to page dst[i], i < n, in each of n_pools pools of
  * n_pages pages of page_bytes bytes, page_stride bytes apart (multiples of
  * 16; pools start on 16 bytes): the K and V pools of every layer in one call,

@@ -328,6 +328,7 @@ extern "C" {
                               stream: *mut c_void) -> c_int;
     pub fn gb_paged_attention_workspace(batch: *const gb_paged_batch, n_heads: i32,
                                         bytes: *mut i64) -> c_int;
+    pub fn gb_paged_set_test_hooks(wait_limit_us: i64, withhold_q: i32) -> c_int;
     pub fn gb_paged_copy(pools_dev: *const *mut c_void, n_pools: i32, n_pages: i64,
                          page_bytes: i64, page_stride: i64, src: *const i32, dst: *const i32,
                          n: i32, stream: *mut c_void) -> c_int;

@@ -102,6 +102,8 @@ struct AttnArgs {
   void* out;
   int64_t o_row, o_head;
   Partials rows, tiles;
+  uint64_t wait_ns;  // the tile kernel's test hooks (gb_paged_set_test_hooks)
+  int withhold_q;
 };
 
 // What a CTA does: `tokens` tokens of sequence seq from row row0, the first at
@@ -353,7 +355,7 @@ inline int64_t grid_bound(const AttnArgs& a, const Plan& pl, int64_t tiles) {
 
 // The tile kernel (paged_attn_tc.cu).  pdl: launched while attn_rows_kernel, on
 // the same stream, still runs; it ends after it.
-cudaError_t launch_attn_tiles(const AttnArgs& a, int dtype, int hd, bool pdl, cudaStream_t st);
+cudaError_t launch_attn_tiles(AttnArgs a, int dtype, int hd, bool pdl, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace gb

@@ -264,8 +264,11 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
   auto edge = [&](int j) { return j * KT + KT - 1 > it.pos0 || j * KT < all_lo; };
 
   const uint32_t tmem = tmem_slot;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_wait(bar, parity & 1, abort_flag, &err_word);
+  // For a whole warp, and the same in all its lanes: where a wait has run out, or another
+  // warp's has, some lanes may still have seen the phase end, and none may go on alone to
+  // what the warp does together (TMEM accesses, votes).
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    return __all_sync(kFullMask, mbar_wait(bar, parity & 1, abort_flag, &err_word, a.wait_ns)) != 0;
   };
 
   if (warp < C::kSoftmax / 32) {
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       ok = wait_o(steps - 1);
       tc_fence_after();
     }
-    if (!*abort_flag && ok && (w == 0 || n1 > 0)) {
+    if (!__any_sync(kFullMask, *abort_flag) && ok && (w == 0 || n1 > 0)) {
       const bool split = it.slot >= 0;
       float M = m, L = l, inv;
       if (!split && a.sinks && live) {
@@ -427,6 +430,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
 #pragma unroll(HD == 64 ? 2 : 1)
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
+        __syncwarp();  // rows that are not live skip the stores
         if (steps) {
           tmem_ld32(o_addr + c, o);
           tmem_wait_ld();
@@ -489,7 +493,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
     if (warp == C::kSoftmax / 32) {
       // ---------------- TMA producer: Q, then K and V tiles in turn ---------------
       bool ok = true;
-      if (lane == 0) {
+      if (lane == 0 && !(a.withhold_q && blockIdx.x == 0)) {
         // a box holds the tokens of a row tile with the group's heads: row = token * group + head
         const uint32_t bytes = (uint32_t)(n1 > 0 ? 2 : 1) * C::kSub * tpt * a.group * 128;
         mbar_arrive_expect_tx(q_full, bytes);
@@ -544,9 +548,6 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       }
     } else if (warp == C::kSoftmax / 32 + 1) {
       // ---------------- MMA issuer -------------------------------------------------
-      auto all_wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(kFullMask, wait(bar, parity)) != 0;
-      };
       const int u0 = uniform(it.u0), n = uniform(it.u1) - u0;
       const int act0 = uniform(hi0) - u0;                            // row tile 0: j < act0
       const int act1 = uniform(n1 > 0 ? lo1 - it.u0 : 0x7fffffff);   // row tile 1: j >= act1
@@ -557,7 +558,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       const uint32_t q_lo = k_major_lo(smem_u32(smem)), ring_base = smem_u32(ring);
       auto on = [&](int w, int j) { return w == 0 ? j < act0 : j >= act1; };
       auto at_edge = [&](int j) { return j >= edge_hi || j < edge_lo; };
-      bool ok = all_wait(q_full, 0);
+      bool ok = wait(q_full, 0);
       // Ring tile t (K of key tile j: 2 j, V: 2 j + 1) is in slot t % kRing, of phase t / kRing.
       int k_slot = 0, v_slot = 1;
       uint32_t k_phase = 0, v_phase = 0;
@@ -588,7 +589,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
         const uint32_t first = step ? 1u : 0u;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-          if (!all_wait(&p_full[kHalves == 2 ? 2 * w + h : buf], phase_of(step))) return false;
+          if (!wait(&p_full[kHalves == 2 ? 2 * w + h : buf], phase_of(step))) return false;
           tc_fence_after();
           if (elect()) {
 #pragma unroll
@@ -609,7 +610,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
         advance(slot, phase);
       };
       auto k_tile = [&](uint32_t* k_lo) -> bool {
-        if (!all_wait(&kv_full[k_slot], k_phase)) return false;
+        if (!wait(&kv_full[k_slot], k_phase)) return false;
         tc_fence_after();
         *k_lo = k_major_lo(ring_base + k_slot * C::kTileBytes);
         return true;
@@ -623,12 +624,12 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       }
       for (int j = 0; j < n && ok; ++j) {
         const bool more = j + 1 < n;
-        ok = all_wait(&kv_full[v_slot], v_phase);
+        ok = wait(&kv_full[v_slot], v_phase);
         if (at_edge(j)) {
 #pragma unroll
           for (int w = 0; w < NT; ++w)
             if (on(w, j)) {
-              ok = ok && all_wait(&v_clean[2 * w + (edges[w] & 1)], edges[w] >> 1);
+              ok = ok && wait(&v_clean[2 * w + (edges[w] & 1)], edges[w] >> 1);
               ++edges[w];
             }
         }
@@ -735,10 +736,26 @@ cudaError_t launch_hd(const AttnArgs& a, int hd, bool pdl, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_attn_tiles(const AttnArgs& a, int dtype, int hd, bool pdl, cudaStream_t st) {
+namespace {
+thread_local uint64_t t_wait_ns = kMbarWaitNs;
+thread_local bool t_withhold_q = false;
+}  // namespace
+
+cudaError_t launch_attn_tiles(AttnArgs a, int dtype, int hd, bool pdl, cudaStream_t st) {
+  a.wait_ns = t_wait_ns;
+  a.withhold_q = t_withhold_q;
   return dtype == GB_DTYPE_BF16 ? launch_hd<__nv_bfloat16>(a, hd, pdl, st)
                                 : launch_hd<__half>(a, hd, pdl, st);
 }
 
 }  // namespace paged
 }  // namespace gb
+
+extern "C" int gb_paged_set_test_hooks(int64_t wait_limit_us, int32_t withhold_q) {
+  using namespace gb;
+  if (wait_limit_us < 0 || wait_limit_us > 10000000)
+    return set_error(GB_ERR_INVALID_ARG, "wait_limit_us %lld outside [0, 1e7]", (long long)wait_limit_us);
+  paged::t_wait_ns = wait_limit_us ? (uint64_t)wait_limit_us * 1000ull : kMbarWaitNs;
+  paged::t_withhold_q = withhold_q != 0;
+  return GB_OK;
+}

@@ -288,6 +288,7 @@ SIGNATURES = {
     "gb_paged_rope_append": (c_int, [POINTER(PagedBatchDesc), POINTER(RopeArgs), c_void_p]),
     "gb_paged_attention": (c_int, [POINTER(PagedBatchDesc), POINTER(AttnArgs), c_void_p]),
     "gb_paged_attention_workspace": (c_int, [POINTER(PagedBatchDesc), c_int32, POINTER(c_int64)]),
+    "gb_paged_set_test_hooks": (c_int, [c_int64, c_int32]),
     "gb_paged_copy": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p,
                               c_int32, c_void_p]),
     "gb_decoder_forward_paged": (c_int, [c_void_p, c_void_p, POINTER(PagedBatchDesc), POINTER(c_void_p),
