@@ -334,8 +334,9 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
         mbar_arrive(&v_clean[2 * w + (edges++ & 1)]);
       }
       tc_fence_after();
-      // set by the producer before the tile that S is of was copied
-      const unsigned bad = *(volatile int*)&any_bad ? bad_pages(j) : 0;
+      // set by the producer before the tile that S is of was copied; for a later tile it
+      // may be set at any time, so the lanes agree on what they read
+      const unsigned bad = __any_sync(kFullMask, *(volatile int*)&any_bad) ? bad_pages(j) : 0;
       uint32_t sb[KT];
 #pragma unroll
       for (int c = 0; c < KT; c += 32) tmem_ld32(s_addr + c, sb + c);

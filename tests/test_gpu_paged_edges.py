@@ -8,7 +8,7 @@ import pytest
 
 from gallium_b200 import GalliumError, _lib, paged
 
-from test_gpu_paged import Case
+from test_gpu_paged import SMALL, Case, U
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,42 @@ def test_all_keys_nan(lens, dim):
     c.k[...] = float("nan")
     out = paged.attention(c.batch(), c.q, c.k, c.v)
     assert torch.isnan(out).all()
+
+
+# -- bad pages -----------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(200, 6000)], [(150, 400), (1, 900), (90, 2500)]])
+def test_bad_pages_in_many_tiles_are_masked_where_they_are(lens, dim):
+    """Pages outside the pool here and there among a chunk's keys, found by the producer
+    while other warps work on earlier tiles: their keys alone are masked."""
+    torch = _torch()
+    c = Case(lens, heads=4, kvh=2, dim=dim, seed=45)
+    r = np.random.default_rng(46)
+    keep = []
+    for b, (_, kv) in enumerate(lens):
+        pages = -(-kv // c.page)
+        gone = r.choice(pages, pages // 6, replace=False)
+        keep.append(~np.isin(np.arange(kv) // c.page, gone))
+        c.table_np[b, gone] = r.choice([-1, c.n_pages, 2 ** 31 - 1, -2 ** 31], len(gone))
+    outs = []
+    for _ in range(3):
+        batch = c.batch()
+        outs.append(paged.attention(batch, c.q, c.k, c.v))
+        with pytest.raises(GalliumError, match="page"):
+            batch.check()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    for b, (n, kv) in enumerate(lens):
+        table = np.where(keep[b][np.arange(-(-kv // c.page)) * c.page], c.table_np[b, :-(-kv // c.page)], 0)
+        pages = torch.from_numpy(table).long().cuda()
+        K, V = (x[pages].reshape(-1, c.kvh, c.dim)[:kv].double() for x in (c.k, c.v))
+        hidden = torch.arange(kv, device="cuda")[None] > torch.arange(kv - n, kv, device="cuda")[:, None]
+        hidden = hidden | ~torch.from_numpy(keep[b]).cuda()
+        K[~torch.from_numpy(keep[b]).cuda()] = 0
+        V[~torch.from_numpy(keep[b]).cuda()] = 0
+        for h in range(c.heads):
+            q, k, v = c.q[c.starts[b]:c.starts[b] + n, h].double(), K[:, h // 2], V[:, h // 2]
+            w = torch.softmax((q @ k.T * dim ** -0.5).masked_fill(hidden, -float("inf")), 1)
+            e = (q.abs() @ k.abs().T).amax(1, keepdim=True) * dim ** -0.5 * (dim + 4) * U["f32"]
+            tol = (w @ v.abs()) * (U[c.dtype] + 2 * (e + 2.0 ** -20) + kv * U["f32"]) + U[c.dtype] * (w @ v).abs()
+            got = outs[0][c.starts[b]:c.starts[b] + n, h].double()
+            assert ((got - w @ v).abs() <= tol + SMALL[U[c.dtype]]).all(), (b, h)
