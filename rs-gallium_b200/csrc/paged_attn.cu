@@ -416,14 +416,15 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
         x1 = fmaxf(x1, __shfl_xor_sync(kFullMask, x1, 2));
         // The reference (a maximum less kTop) moves only when a score passes the
         // maximum by 2^6: the weights then stay below 2^(kTop + 6), which the
-        // 16-bit types hold as exactly as 1.
+        // 16-bit types hold as exactly as 1.  Each row's moves by itself, so that no
+        // other row has a part in its rounding.
         constexpr float kTop = Elem<T>::kTop;
-        if (__any_sync(kFullMask, x0 > m0 + (kTop + 6.0f) || x1 > m1 + (kTop + 6.0f))) {
-          const float n0 = fmaxf(m0, x0 - kTop), n1 = fmaxf(m1, x1 - kTop);
-          const float c0 = n0 == -INFINITY ? 1.0f : ex2(m0 - n0);
-          const float c1 = n1 == -INFINITY ? 1.0f : ex2(m1 - n1);
-          m0 = n0;
-          m1 = n1;
+        const bool moves0 = x0 > m0 + (kTop + 6.0f), moves1 = x1 > m1 + (kTop + 6.0f);
+        if (__any_sync(kFullMask, moves0 || moves1)) {
+          const float c0 = moves0 ? ex2(m0 - (x0 - kTop)) : 1.0f;
+          const float c1 = moves1 ? ex2(m1 - (x1 - kTop)) : 1.0f;
+          m0 = moves0 ? x0 - kTop : m0;
+          m1 = moves1 ? x1 - kTop : m1;
           l0 *= c0;
           l1 *= c1;
 #pragma unroll

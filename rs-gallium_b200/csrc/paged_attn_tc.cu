@@ -359,11 +359,13 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       for (int i = 4; i < KT; i += 4)
 #pragma unroll
         for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[i + c]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale - kTop;
-      if (__any_sync(kFullMask, top > m + 6.0f)) {
-        const float nm = fmaxf(m, top);
-        const float f = nm == -INFINITY ? 1.0f : ex2(m - nm);
-        m = nm;
+      // A row that is no token's holds whatever queries, or shared memory, were there.
+      const float top =
+          live ? fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale - kTop : -INFINITY;
+      const bool moves = top > m + 6.0f;
+      if (__any_sync(kFullMask, moves)) {  // only the row that must: its rounding is its own
+        const float f = moves ? ex2(m - top) : 1.0f;
+        m = moves ? top : m;
         l *= f;
         if (steps) {  // after the last MMAs into this O
           ok = wait_o(steps - 1);

@@ -157,3 +157,22 @@ def test_bad_pages_in_many_tiles_are_masked_where_they_are(lens, dim):
             tol = (w @ v.abs()) * (U[c.dtype] + 2 * (e + 2.0 ** -20) + kv * U["f32"]) + U[c.dtype] * (w @ v).abs()
             got = outs[0][c.starts[b]:c.starts[b] + n, h].double()
             assert ((got - w @ v).abs() <= tol + SMALL[U[c.dtype]]).all(), (b, h)
+
+
+# -- rows beside rows ----------------------------------------------------------------
+@pytest.mark.parametrize("heads,kvh,dim", [(8, 2, 64), (3, 1, 64), (5, 1, 128), (6, 2, 128), (14, 2, 256), (9, 1, 64)])
+@pytest.mark.parametrize("lens", [[(2, 150), (1, 300)], [(20, 700), (25, 25)], [(150, 2000), (30, 300), (1, 9)]])
+def test_a_row_keeps_its_bits_whatever_its_neighbours_hold(lens, heads, kvh, dim):
+    """Larger queries in other rows, of its own tile too, and what earlier work left in
+    shared memory have no part in a row's rounding."""
+    torch = _torch()
+    c = Case(lens, heads=heads, kvh=kvh, dim=dim, dtype="f16", seed=44)
+    want = paged.attention(c.batch(), c.q, c.k, c.v)
+    other = c.batch()
+    for keep in (0, c.total // 2, c.total - 1):
+        q = c.q * 60
+        q[keep] = c.q[keep]
+        for _ in range(3):
+            out = paged.attention(other, q, c.k, c.v)
+            assert torch.equal(out[keep], want[keep])
+            assert torch.equal(paged.attention(c.batch(), c.q, c.k, c.v), want)
