@@ -454,7 +454,10 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
           ldsm4_t(vf, vs_ + r * HD * 2 + ((c ^ (r & 7)) << 4));
           if (masked && __any_sync(kFullMask, any_nonfinite<T>(vf[0]) || any_nonfinite<T>(vf[1]) ||
                                                   any_nonfinite<T>(vf[2]) || any_nonfinite<T>(vf[3]))) {
-            // 0 x inf is NaN: add the visible products alone, key by key
+            // 0 x inf is NaN: what is not finite is left out of the MMAs (whose sums round
+            // the same without it) and added key by key to the rows that see it
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vf[i] = finite_only<T>(vf[i]);
             for (int kk = 0; kk < kStep; ++kk) {
               const int own = (lane & ~3) | ((kk & 7) >> 1), nt = kk >> 3;
               const uint32_t sb = __shfl_sync(kFullMask, seen, own) >> (nt * 4 + (kk & 1));
@@ -469,20 +472,21 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
                     sm + (vs_ - smem_u32(sm)) + kk * HD * 2 + (((col >> 3) ^ (kk & 7)) << 4) +
                     (col & 7) * 2);
                 const float2 v = Elem<T>::unpack(vw);
+                constexpr uint32_t em = Elem<T>::kExpMask;
+                const bool bx = (vw & em) == em, by = (vw & (em << 16)) == (em << 16);
                 if (sb & 1) {
-                  acc[dt * 2 + h][0] += w0 * v.x;
-                  acc[dt * 2 + h][1] += w0 * v.y;
+                  if (bx) acc[dt * 2 + h][0] += w0 * v.x;
+                  if (by) acc[dt * 2 + h][1] += w0 * v.y;
                 }
                 if (sb & 4) {
-                  acc[dt * 2 + h][2] += w1 * v.x;
-                  acc[dt * 2 + h][3] += w1 * v.y;
+                  if (bx) acc[dt * 2 + h][2] += w1 * v.x;
+                  if (by) acc[dt * 2 + h][3] += w1 * v.y;
                 }
               }
             }
-          } else {
-            mma16816<T>(acc[dt * 2], pf, vf[0], vf[1]);
-            mma16816<T>(acc[dt * 2 + 1], pf, vf[2], vf[3]);
           }
+          mma16816<T>(acc[dt * 2], pf, vf[0], vf[1]);
+          mma16816<T>(acc[dt * 2 + 1], pf, vf[2], vf[3]);
         }
       }
       __syncwarp();  // the stage is read before a later issue overwrites it

@@ -337,6 +337,15 @@ __device__ __forceinline__ bool any_nonfinite(uint32_t w) {
   return (w & m) == m || (w & (m << 16)) == (m << 16);
 }
 
+// A pair of elements with what is not finite replaced by 0.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  constexpr uint32_t m = Elem<T>::kExpMask;
+  if ((w & m) == m) w &= 0xffff0000u;
+  if ((w & (m << 16)) == (m << 16)) w &= 0xffffu;
+  return w;
+}
+
 template <typename T>
 __device__ __forceinline__ void store_out(const AttnArgs& a, int row, int head, int d, float x,
                                           float y) {

@@ -317,14 +317,8 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
             const uint4 x = *p;
             if (any_nonfinite<T>(x.x) || any_nonfinite<T>(x.y) || any_nonfinite<T>(x.z) ||
                 any_nonfinite<T>(x.w)) {
-              uint32_t e[4] = {x.x, x.y, x.z, x.w};
-              constexpr uint32_t em = Elem<T>::kExpMask;
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                if ((e[c] & em) == em) e[c] &= 0xffff0000u;
-                if ((e[c] & (em << 16)) == (em << 16)) e[c] &= 0xffffu;
-              }
-              *p = make_uint4(e[0], e[1], e[2], e[3]);
+              *p = make_uint4(finite_only<T>(x.x), finite_only<T>(x.y), finite_only<T>(x.z),
+                              finite_only<T>(x.w));
               found = true;
             }
           }

@@ -120,6 +120,28 @@ def test_all_keys_nan(lens, dim):
     assert torch.isnan(out).all()
 
 
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("heads,kvh,dim", [(8, 2, 64), (8, 2, 128), (6, 3, 128), (4, 2, 256)])
+def test_values_of_single_tokens_that_are_not_finite(heads, kvh, dim, value):
+    """Rows of one decoding tile see different keys: a value that is not finite in the
+    last position, or in one that the window has left behind for the later row, changes
+    no bit of the rows that do not see it."""
+    torch = _torch()
+    for window in (0, 50):
+        c = Case([(1, 33), (3, 121)], heads=heads, kvh=kvh, dim=dim, seed=43)
+        wide = lambda v: paged.attention(c.batch(), c.q, c.k, v, window=window, out=torch.empty_like(c.q, dtype=torch.float32))  # noqa: E731
+        clean = wide(c.v)
+        for bad in [120, 119] + ([118 - 49] if window else []):
+            v = c.v.clone()
+            v[c.table_np[1, bad // c.page], bad % c.page, 0, 3] = value
+            out = wide(v)
+            for i, pos in enumerate((118, 119, 120)):
+                if pos >= bad and (not window or pos - bad < window):
+                    assert not torch.isfinite(out[1 + i, :heads // kvh, 3]).any()
+                    out[1 + i, :heads // kvh, 3] = clean[1 + i, :heads // kvh, 3]
+            assert torch.equal(out, clean), (window, bad)
+
+
 # -- bad pages -----------------------------------------------------------------------
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("lens", [[(200, 6000)], [(150, 400), (1, 900), (90, 2500)]])
