@@ -1040,7 +1040,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   R.bin_scale = 32.0f / t;
 
   const float slack = mass_slack(top, grid);
-  if (filtered && top < INFINITY && (!whole_p || slack < 0.01f)) {
+  // A grid so fine (t below 10^-37) that a bin has no number puts a logit of 0 nowhere.
+  if (filtered && top < INFINITY && grid < INFINITY && (!whole_p || slack < 0.01f)) {
     const int top_bin = grid_of(top, grid);
     // the cluster's bins, two per thread, every load before the first is used
     const int j0 = 2 * tid;
