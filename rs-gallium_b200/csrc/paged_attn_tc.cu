@@ -149,6 +149,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
       GB_W8(v, 8), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : GB_R8(v, 0)
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::GB_W8(v, 0),
+               "r"(addr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -207,7 +217,11 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
   uint64_t* o_done = p_full + 2 * NT;      // [2 NT]: the PVs of a row tile in turn
   uint64_t* v_clean = o_done + 2 * NT;     // [2 NT]: a row tile's edge tiles in turn
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word, err_word, poisoned, any_bad;
+  // The bad pages of key tile j, a bit each, at j % 8: written by the producer once a slot
+  // is free for K of j, when every softmax warp is within the ring of it (at most four
+  // tiles behind), and read where S of j is there.
+  __shared__ volatile uint32_t bad_pages[8];
+  __shared__ int abort_word, poisoned;
   volatile int* abort_flag = &abort_word;
 
   if (tid == 0) {
@@ -222,7 +236,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       mbar_init(&o_done[i], 1);
       mbar_init(&v_clean[i], 128);
     }
-    abort_word = err_word = poisoned = any_bad = 0;
+    abort_word = poisoned = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tmem_alloc(&tmem_slot, C::kTmem);
@@ -253,28 +267,27 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
   // a tile with a key that some row does not see
   const int32_t* table = a.b.table + it.seq * a.b.table_stride;
   const int page_size = 1 << a.b.page_shift;
-  // keys of the tile on bad pages, a bit per page of the tile (lane = page)
-  auto bad_pages = [&](int j) -> unsigned {
-    bool bad = false;
-    const int key = j * KT + lane * page_size;
-    if (lane * page_size < KT && key <= last && key + page_size > key_lo)
-      bad = (unsigned)__ldg(table + (key >> a.b.page_shift)) >= (unsigned)a.b.n_pages;
-    return __ballot_sync(kFullMask, bad);
-  };
   auto edge = [&](int j) { return j * KT + KT - 1 > it.pos0 || j * KT < all_lo; };
 
   const uint32_t tmem = tmem_slot;
-  // For a whole warp, and the same in all its lanes: where a wait has run out, or another
-  // warp's has, some lanes may still have seen the phase end, and none may go on alone to
-  // what the warp does together (TMEM accesses, votes).
+  // A bounded wait of a whole warp, with one result for it: where it has run out, or
+  // another warp's has, some lanes may still have seen the phase end, and none may go on
+  // alone to what the warp does together (TMEM accesses, votes).
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    return __all_sync(kFullMask, mbar_wait(bar, parity & 1, abort_flag, &err_word, a.wait_ns)) != 0;
+    if (__all_sync(kFullMask, mbar_try_wait(bar, parity & 1))) return true;
+    const uint64_t t0 = globaltimer();
+    while (!__all_sync(kFullMask, mbar_try_wait(bar, parity & 1)))
+      if (__any_sync(kFullMask, *abort_flag || globaltimer() - t0 > a.wait_ns)) {
+        *abort_flag = 1;
+        return false;
+      }
+    return true;
   };
 
   if (warp < C::kSoftmax / 32) {
     if constexpr (C::kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------- softmax: thread = row ---------------------------------------
-    const int w = warp >> 2;               // row tile
+    const int w = NT == 1 ? 0 : warp >> 2;  // row tile
     const int r = tid & 127;               // row of the tile
     const int tok = r / a.group;           // token of the tile
     const bool live = tok < (w ? n1 : n0) && r < tpt * a.group;
@@ -288,12 +301,17 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
     // neighbours: S of a step comes after PV of the step two before, so with two
     // barriers in turn the phase before n's is always complete.
     auto wait_o = [&](int n) { return wait(&o_done[2 * w + (n & 1)], n >> 1); };
-    float m = -INFINITY, l = 0.0f;  // reference maximum, sum of weights
-    int steps = 0, edges = 0;
+    // Reference maximum, sum of weights.  A row that is no token's holds whatever queries,
+    // or shared memory, were there: its reference never moves.
+    float m = live ? -INFINITY : INFINITY, l = 0.0f;
+    // the key tiles that the row tile sees any key of
+    const int j0 = w ? lo1 : it.u0, j1 = w ? (n1 > 0 ? it.u1 : lo1) : hi0;
+    const int all_steps = max(j1 - j0, 0);
+    int edges = 0;
     bool ok = true;
-    for (int j = it.u0; j < it.u1 && ok; ++j) {
+    for (int j = j0; j < j1; ++j) {
+      const int steps = j - j0;
       const bool at_edge = edge(j);
-      if (!active(w, j)) continue;
       const int buf = buf_of(w, steps);
       const uint32_t s_addr = tmem + buf * KT + lane_base;
       ok = wait(&s_full[buf], phase_of(steps));
@@ -328,9 +346,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
         mbar_arrive(&v_clean[2 * w + (edges++ & 1)]);
       }
       tc_fence_after();
-      // set by the producer before the tile that S is of was copied; for a later tile it
-      // may be set at any time, so the lanes agree on what they read
-      const unsigned bad = __any_sync(kFullMask, *(volatile int*)&any_bad) ? bad_pages(j) : 0;
+      const unsigned bad = bad_pages[j & 7];
       uint32_t sb[KT];
 #pragma unroll
       for (int c = 0; c < KT; c += 32) tmem_ld32(s_addr + c, sb + c);
@@ -353,9 +369,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       for (int i = 4; i < KT; i += 4)
 #pragma unroll
         for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[i + c]);
-      // A row that is no token's holds whatever queries, or shared memory, were there.
-      const float top =
-          live ? fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale - kTop : -INFINITY;
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale - kTop;
       const bool moves = top > m + 6.0f;
       if (__any_sync(kFullMask, moves)) {  // only the row that must: its rounding is its own
         const float f = moves ? ex2(m - top) : 1.0f;
@@ -366,13 +380,13 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(o_addr + c, o);
+          for (int c = 0; c < HD; c += 8) {
+            uint32_t o[8];
+            tmem_ld8(o_addr + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st16(o_addr + c, o);
+            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st8(o_addr + c, o);
           }
           tmem_wait_st();
         }
@@ -404,11 +418,10 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
         const float2 v = unpair(add2(sum[0], sum[1]));
         l += v.x + v.y;
       }
-      ++steps;
     }
     // ---- the row's result
-    if (ok && steps) {
-      ok = wait_o(steps - 1);
+    if (ok && all_steps) {
+      ok = wait_o(all_steps - 1);
       tc_fence_after();
     }
     if (!__any_sync(kFullMask, *abort_flag) && ok && (w == 0 || n1 > 0)) {
@@ -428,7 +441,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
         __syncwarp();  // rows that are not live skip the stores
-        if (steps) {
+        if (all_steps) {
           tmem_ld32(o_addr + c, o);
           tmem_wait_ld();
         } else {
@@ -506,6 +519,7 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
       for (int j = it.u0; j < it.u1 && ok; ++j) {
         // lane b holds the page of the tile's keys [b box, b box + box)
         int page = a.b.n_pages, in_page = 0;
+        bool bad = false;
         {
           const int key = j * KT + lane * box;
           in_page = key & (page_size - 1);
@@ -514,15 +528,19 @@ __global__ void __launch_bounds__(Cfg<HD, MANY>::kThreads, Cfg<HD, MANY>::kCtas)
             if ((unsigned)p < (unsigned)a.b.n_pages) {
               page = p;
             } else {
-              *(volatile int*)&any_bad = 1;
+              bad = true;
               flag(a.b, GB_PAGED_BAD_PAGE);
             }
           }
         }
+        const unsigned bad_mask = __ballot_sync(kFullMask, bad);
         for (int kv = 0; kv < 2 && ok; ++kv) {
           ok = wait(&kv_empty[slot], phase ^ 1);
           if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], C::kTileBytes);
+          if (lane == 0) {
+            if (kv == 0) bad_pages[j & 7] = bad_mask;
+            mbar_arrive_expect_tx(&kv_full[slot], C::kTileBytes);
+          }
           __syncwarp();
           const uint32_t dst = smem_u32(ring + slot * C::kTileBytes);
           const CUtensorMap* map = kv ? &map_v : &map_k;
