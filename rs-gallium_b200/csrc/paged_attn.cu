@@ -105,7 +105,7 @@ __device__ __forceinline__ Share find_share(const AttnArgs& a, const Plan& pl, i
   Share sh;
   sh.seq = 0;
   sh.offset = 0;
-  if (b.n_seqs <= 128) {
+  if (b.n_seqs <= kLaneSeqs) {
     unsigned long long w[4], upto[4], total = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -190,7 +190,7 @@ struct Cursor {
 // heads, and its own pipeline of cp.async stages, which runs on across the pairs; the
 // warps of a head join their results in shared memory at the end of each pair.
 // mma.sync suits it: 16 rows fill one, and memory is the floor.  Measured with 64 query
-// and 8 KV heads of 64: 64 sequences of 512 to 8192 keys 104 us, 4.2 TB/s; 256 of 2000
+// and 8 KV heads of 64: 64 sequences of 512 to 8192 keys 102 us, 4.3 TB/s; 256 of 2000
 // 217 us, 4.8 TB/s, and 5.8 where a page's slots of a head lie together, since the rows
 // of a head are 128-byte pieces a slot apart.  TMA boxes in place of cp.async were no
 // faster (106 us; with the 256-byte L2 promotion, which fetches the next head too, 127).
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
   if (kw == 0 && lane == 0) a.rows.groups[blockIdx.x * HPC + hw].splits = 0;
   if (share.begin < 0) return;
   auto seq_at = [&](int s) -> Seq {  // the same in every lane
-    if (a.b.n_seqs > 128) return load_seq(a.b, s, false);
+    if (a.b.n_seqs > kLaneSeqs) return load_seq(a.b, s, false);
     Seq q = held[0];
 #pragma unroll
     for (int i = 1; i < 4; ++i)

@@ -117,7 +117,9 @@ __device__ __forceinline__ int first_unit(int pos, int window, int unit) {
   return window > 0 && pos >= window ? (pos - window + 1) / unit : 0;
 }
 
-// CTAs of a tile grid, at most: more rows and heads than fit in memory.
+// Sequences that a warp holds, a lane for every 32nd, and the items that they may have
+// then: as many rows and heads do not fit in memory.
+constexpr int kLaneSeqs = 128;
 constexpr uint32_t kMaxItems = (1u << 25) - 1;
 
 struct SeqWork {
@@ -202,7 +204,7 @@ __device__ bool find_item(const AttnArgs& a, const Plan& pl, const Partials& par
                           Item* out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Batch& b = a.b;
-  if (b.n_seqs <= 128) {
+  if (b.n_seqs <= kLaneSeqs) {
     Seq q[4];
     SeqWork x[4];
     unsigned long long w = 0;

@@ -30,9 +30,10 @@
 // Warps: four per row tile, then the TMA producer and the MMA issuer.  Every wait
 // is bounded, as in the expert GEMMs.
 //
-// Measured: a chunk of 1000 tokens behind 16 K keys, 32 heads of 128, f16, 247 us, 1107
-// TFLOP/s (1268 behind 32 K); head_dim 256 1160 and head_dim 64 680 TFLOP/s behind 32 K;
-// four prompts of 2 K, 64 heads of 64, 246 us, 520 TFLOP/s.  Bound at head_dim 64 by the
+// Measured, in a captured step: a chunk of 1000 tokens behind 16 K keys, 32 heads of 128,
+// f16, 247-249 us, 1100 TFLOP/s (276-292 alone with cold caches; 1268 TFLOP/s behind 32
+// K); head_dim 256 1160 and head_dim 64 680 TFLOP/s behind 32 K; four prompts of 2 K, 64
+// heads of 64, 240-246 us, 520-534 TFLOP/s.  Bound at head_dim 64 by the
 // softmax between the MMAs: 16 exponentials per clock and SM would take 127 us there,
 // half the time.  Two threads per row, and exponentials as polynomials, were no faster.
 #include "paged_attn.cuh"
@@ -725,7 +726,8 @@ cudaError_t launch(const AttnArgs& a, bool pdl, cudaStream_t st) {
   const int64_t per = (int64_t)C::NT * tpt;
   const int64_t tiles = std::min<int64_t>(a.b.total_q / per + a.b.n_seqs, a.b.total_q) * a.b.nkv;
   const int64_t grid = grid_bound(a, tile_plan<HD>(), tiles);
-  if (grid > (int64_t)kMaxItems) return cudaErrorInvalidConfiguration;
+  if (grid > (a.b.n_seqs <= kLaneSeqs ? (int64_t)kMaxItems : 0x7fffffffll))
+    return cudaErrorInvalidConfiguration;
   auto kern = attn_tile_kernel<T, HD, MANY>;
   cudaError_t e = set_smem_limit(kern, C::kSmem);
   if (e != cudaSuccess) return e;
