@@ -270,9 +270,12 @@ __global__ void __launch_bounds__(kRopeThreads) rope_units_kernel(const __grid_c
 // Many rows: a CTA takes `per` of them (at most kRopeRows).  `across` lane groups
 // share a row, each with its heads in turn, so that a row's cosines, sines, page
 // and addresses are worked out once for them; the groups' other rows run beside.
-// 8150 rows of 48 heads of 128 with both norms: 55 us, 3.6 TB/s (82 with a unit at a
-// time over the whole batch, 57 with 64 registers and four CTAs on an SM, 62 with the
-// loads a pass ahead); bound by the instructions of norm and rotation.
+// 8150 rows of 48 heads of 128 with both norms: 54-55 us, 3.6 TB/s (82 with a unit at a
+// time over the whole batch, 62 with the loads a pass ahead).  With room for three CTAs
+// 16-bit rows still take 64 registers, so that four fit; f32 rows take more, three fit,
+// 72 us.  Bounded to four, 56, and 69 with 40 bytes of spills.  59 % of the issue slots
+// and about half of DRAM are busy: neither bounds it alone, and what the warps wait for
+// between has not been told apart.
 template <typename In, typename Out, int HD>
 __global__ void __launch_bounds__(kRopeThreads, 3)
     rope_rows_kernel(const __grid_constant__ RopeArgs a, int per, int across) {

@@ -79,7 +79,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile
 // Programmatic dependent launch.  pdl_wait: wait until the grids this one
 // depends on have completed and their writes are visible (returns at once for
 // an ordinary launch); every kernel launched with launch_pdl calls it before
-// its first global-memory access.  pdl_trigger: let the next grid on the
+// its first global-memory access, but for attn_tile_kernel, which waits at its
+// end: the kernel it is launched beside (attn_rows_kernel, itself an ordinary
+// launch, so all that came before is complete) writes nothing that it reads or
+// writes, and what follows must find both complete.  pdl_trigger: let the next grid on the
 // stream begin launching (it still waits in its own pdl_wait).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -6,7 +6,8 @@ whose last dimension is contiguous, so a [page][head][slot][dim] pool is a
 transposed view), bf16 or f16; ``PagedBatch`` describes the ragged batch that
 a step works on and serves all layers of it.  Every call runs on torch's
 current stream of the tensors' device and synchronises nothing:
-``PagedBatch.check`` reads what the kernels flagged.
+``PagedBatch.check`` reads what the kernels flagged.  There is no backward
+form: results carry no graph, whether or not an input requires a gradient.
 """
 from __future__ import annotations
 
@@ -79,6 +80,12 @@ class PagedBatch:
     long as they keep within total_q (rows of q), max_q_len and max_kv_len.
     The tensors are used as they are (no copies) and must be contiguous; rows
     of page_table may be strided.
+
+    The error word is zeroed here, on the current stream, and read and zeroed by
+    check() on the stream current then: calls on another stream are ordered after
+    the one and before the other by the caller, like the tensors above, or a flag
+    may be lost.  A batch holds the descriptor of the call being made, so two
+    threads take one each.
     """
 
     def __init__(self, q_start, kv_len, page_table, *, page_size: int, total_q: int, max_q_len: int,
