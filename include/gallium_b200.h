@@ -494,7 +494,8 @@ typedef enum {
   GB_PAGED_BAD_LENGTH = 2,   /* q_start not ascending within [0, total_q], a q_len or kv_len
                                 outside [0, max] or past the page table: clamped to it, and
                                 rows of a sequence longer than max_q_len may be left as they
-                                are */
+                                are; rows that a q_start going back gives to several
+                                sequences hold nothing of meaning */
   GB_PAGED_BAD_POSITION = 4, /* a row before position 0 or past the cos / sin tables: the row
                                 is dropped */
   GB_PAGED_TIMEOUT = 8       /* a bounded pipeline wait ran out: the output is invalid */

@@ -445,6 +445,8 @@ __global__ void __launch_bounds__(kThreads, rows_plan<HD, HPC>().target / 148)
           l0 += s[nt][0] + s[nt][1];
           l1 += s[nt][2] + s[nt][3];
         }
+        // P in the pool's type, as the MMA takes it beside V: half a step of that type per
+        // weight, where the sums of weights keep f32.
         const uint32_t pf[4] = {Elem<T>::pack(s[0][0], s[0][1]), Elem<T>::pack(s[0][2], s[0][3]),
                                 Elem<T>::pack(s[1][0], s[1][1]), Elem<T>::pack(s[1][2], s[1][3])};
 #pragma unroll
