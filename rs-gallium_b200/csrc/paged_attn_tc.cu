@@ -746,15 +746,16 @@ cudaError_t launch_hd(const AttnArgs& a, int hd, bool pdl, cudaStream_t st) {
   // bounds, there are as many chunks as the rows need when every other sequence has one.
   // While keys are few, though, the small CTAs start sooner beside those of many decoding
   // sequences, which then count like tiles: 250 of 500 keys and a chunk of 200 behind 1 K
-  // keys 124 us against 134 (of 500 behind 100: 112 against 122); with more keys they
-  // lose: 74 of 2 K and a chunk of 500 behind 4 K 202 against 147, behind 8 K 296 against
-  // 194, of 500 behind 1.7 K 142 against 120, but of 200 120 against 122.
+  // keys 124 us against 134 (of 500 behind 100: 112 against 122), behind 2 K, of 350 145
+  // against 155, of 500 148 against 140.  With more keys they lose the more, the more tiles
+  // there are: 74 of 2 K and a chunk of 280 behind 4 K 167 against 142, of 500 202 against
+  // 147, behind 8 K 296 against 194 (but 74 of 300 keys, 200 behind 4 K, 91 against 97).
   const int64_t chunks = std::min<int64_t>(
       a.b.n_seqs, std::max<int64_t>(1, (a.b.total_q - a.b.n_seqs + a.b.max_q - 2) / (a.b.max_q - 1)));
   const int64_t rows = std::max<int64_t>(0, a.b.total_q - (a.b.n_seqs - chunks));
   const int64_t keys = a.window > 0 ? std::min<int64_t>(a.window, a.b.max_kv) : a.b.max_kv;
   int64_t tiles = (rows * a.group / 128 + chunks) * a.b.nkv;
-  if (keys <= (tiles < 148 ? 4096 : 2048)) tiles += (a.b.n_seqs - chunks) * a.b.nkv;
+  if (keys <= (tiles < 222 ? 4096 : 2048)) tiles += (a.b.n_seqs - chunks) * a.b.nkv;
   if (hd == 64 && tiles >= 592 && keys <= 8192) return launch<T, 64, true>(a, pdl, st);
   if (hd == 64) return launch<T, 64>(a, pdl, st);
   if (hd == 128) return launch<T, 128>(a, pdl, st);

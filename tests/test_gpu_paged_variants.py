@@ -30,6 +30,7 @@ def _kernels(c, tmp_path, **kw):
     ([(1, 60)] * 74 + [(500, 4500)], False),   # one chunk: 256 tiles of many keys, whatever decodes beside it
     ([(1, 60)] * 74 + [(500, 700)], True),     # of few keys
     ([(1, 60)] * 74 + [(100, 2500)], True),    # few tiles
+    ([(1, 60)] * 74 + [(350, 2500)], True),
     ([(1, 60)] * 74 + [(100, 4500)], False),
     ([(1, 60)] * 2 + [(1200, 4500)], True),    # 600 tiles of their own
     ([(1200, 9000)], False),                   # of very many keys
